@@ -18,11 +18,13 @@
 #include "fxr.h"
 #include "fxr_attention.cuh"
 #include "fxr_attention2.cuh"
+#include "fxr_attention_q8.cuh"
 #include "fxr_compat_kernels.cuh"
 #include "fxr_dense_kernels.cuh"
 #include "fxr_device.cuh"
 #include "fxr_gemm.cuh"
 #include "fxr_mem_kernels.cuh"
+#include "fxr_q8.cuh"
 
 #include <nvtx3/nvToolsExt.h>
 
@@ -2333,3 +2335,5 @@ int32_t fxr_ipc_free(void* ptr) {
 }
 
 }  // extern "C"
+
+#include "fxr_q8_api.cuh"

@@ -1,0 +1,420 @@
+// fxr_q8.cuh — the 8-bit spatial cache (sm_100a): codes, scales and the kernels that move rows.
+//
+// A head vector x (128 values of one token's K' or V) is held as 128 codes of 8 bits and one scale of
+// the frame's 16-bit type T:
+//   s    = up_T(max|x| / Q)            Q = 127 (int8) or 448 (e4m3); up_T rounds up to T
+//   code = rint(x / s) in [-127, 127]  or  e4m3(x / s), nearest even, saturating
+//   read = T(code * s)                 one rounding
+// The scale is a number of T, so that the read-back is one packed multiply with one rounding, in the
+// read kernel and in the attention alike; rounding it up keeps |x / s| <= Q, at a cost of at most
+// 2^-8 (bf16) or 2^-11 (f16) of the range. Where Q * s would pass the largest f16 the scale is
+// rounded down instead and the largest codes saturate. A vector of zeros has scale 0; one that holds
+// an infinity or NaN has scale NaN and codes 0, and reads back as NaN.
+//   q8_write_kernel     executed rows: gather + QK-RMSNorm + RoPE + quantised cache rows, or (raw)
+//                       the quantised rows of an attention-ready 16-bit cache
+//   q8_read_kernel      rows back in 16 bits
+//   q8_restore_kernel   puts back the cache rows of mask==1 tokens
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "fxr_mem_kernels.cuh"
+
+namespace fxr {
+namespace q8 {
+
+constexpr int kInt8 = 0, kE4m3 = 1;
+
+// One cache, as a kernel argument. Code rows: [n_rows, ld] bytes; scales: [n_heads, ld_scale] of T.
+struct Cache {
+    uint8_t* k;
+    uint8_t* v;
+    void* ks;
+    void* vs;
+    int64_t ld, ld_scale;
+};
+
+// ---- codes --------------------------------------------------------------------------------------
+template <int F> __device__ __forceinline__ constexpr float top_code() { return F == kInt8 ? 127.f : 448.f; }
+
+template <typename T> __device__ __forceinline__ float scale_up(float t);
+template <> __device__ __forceinline__ float scale_up<__nv_bfloat16>(float t) {
+    return __uint_as_float((__float_as_uint(t) + 0xffffu) & 0xffff0000u);   // t >= 0
+}
+template <> __device__ __forceinline__ float scale_up<__half>(float t) { return __half2float(__float2half_ru(t)); }
+
+// Scale of a head vector whose largest magnitude has the bits `amax` (NaN and infinities compare
+// above every finite value).
+template <typename T, int F>
+__device__ __forceinline__ float scale_of(uint32_t amax) {
+    if (amax >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+    const float t = __fdiv_rn(__uint_as_float(amax), top_code<F>());
+    float s = scale_up<T>(t);
+    if (sizeof(T) == 2 && StoreT<T>::kUmmaFormat == 0) {   // f16
+        if (s > 65504.f) return __uint_as_float(0x7fc00000u);   // no f16 scale holds this vector
+        if (s * top_code<F>() > 65504.f && __uint_as_float(amax) <= 65504.f)
+            s = __half2float(__float2half_rd(t));
+    }
+    return s;
+}
+
+// Codes of 8 values as 8 bytes. s = 0 or NaN: codes 0.
+template <int F>
+__device__ __forceinline__ uint2 encode8(const float* x, float s) {
+    const bool zero = !(s > 0.f);
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = zero ? 0.f : __fdiv_rn(x[e], s);
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (F == kInt8) {
+            int32_t c[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[e] = min(127, max(-127, __float2int_rn(y[4 * h + e])));
+            const uint32_t lo = __byte_perm((uint32_t)c[0], (uint32_t)c[1], 0x0040);
+            const uint32_t hi = __byte_perm((uint32_t)c[2], (uint32_t)c[3], 0x0040);
+            w[h] = __byte_perm(lo, hi, 0x5410);
+        } else {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h], y[4 * h + 1]), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h + 2], y[4 * h + 3]), __NV_SATFINITE, __NV_E4M3);
+            w[h] = lo | (hi << 16);
+        }
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// Byte a of wa and byte b of wb as a packed pair of T, exact up to the factor 1 / code_scale():
+//   int8 -> bf16: 0x4300 | low 7 bits is 128 + low7, 0x4300 | sign bit is 128 or 256; the difference
+//                 is the two's complement value (bf16 holds 8 significant bits, so both are exact)
+//   int8 -> f16:  0x6400 | (x ^ 0x80) is 1024 + 128 + x
+//   e4m3 -> f16:  sign, exponent and mantissa fields moved into place: the value times 2^-8,
+//                 subnormals included
+//   e4m3 -> bf16: the same gives the value times 2^-120, multiplied back (bf16 products keep
+//                 subnormal operands)
+// The e4m3 NaN codes, which the write never produces, are not told apart from +-480.
+template <typename T, int F> __device__ __forceinline__ constexpr float code_scale() {
+    return (F == kE4m3 && StoreT<T>::kUmmaFormat == 0) ? 256.f : 1.f;
+}
+template <typename T, int F>
+__device__ __forceinline__ uint32_t decode2(uint32_t wa, uint32_t wb, int a, int b) {
+    if constexpr (F == kInt8) {
+        const uint32_t u = __byte_perm(wa, wb, (uint32_t)(a | ((4 + b) << 8)));
+        if constexpr (StoreT<T>::kUmmaFormat == 1) {
+            const uint32_t p = (u & 0x007f007fu) | 0x43004300u, n = (u & 0x00800080u) | 0x43004300u;
+            const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&p),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&n));
+            return *reinterpret_cast<const uint32_t*>(&r);
+        } else {
+            const uint32_t p = (u & 0x00ff00ffu) ^ 0x64806480u, n = 0x64806480u;
+            const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&p), *reinterpret_cast<const __half2*>(&n));
+            return *reinterpret_cast<const uint32_t*>(&r);
+        }
+    } else {
+        const uint32_t u = __byte_perm(wa, wb, (uint32_t)((a << 4) | ((4 + b) << 12)));
+        if constexpr (StoreT<T>::kUmmaFormat == 1) {
+            const uint32_t p = ((u >> 4) & 0x07f007f0u) | (u & 0x80008000u), c = 0x7b807b80u;
+            const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&p),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&c));
+            return *reinterpret_cast<const uint32_t*>(&r);
+        } else {
+            return ((u >> 1) & 0x3f803f80u) | (u & 0x80008000u);
+        }
+    }
+}
+
+template <typename T> __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t mul2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <> __device__ __forceinline__ uint32_t mul2<__half>(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// The scale as the multiplier of decode2's pairs, twice in a register. Exact: a code_scale of 256
+// belongs to f16 scales of at most 146.25.
+template <typename T, int F>
+__device__ __forceinline__ uint32_t scale_pair(float s) {
+    s *= code_scale<T, F>();
+    return StoreT<T>::pack2(s, s);
+}
+
+// 16 codes -> 16 values of T in two 16-byte vectors (lo: codes 0-7, hi: 8-15).
+template <typename T, int F>
+__device__ __forceinline__ void decode16(const uint4& c, uint32_t s2, uint4& lo, uint4& hi) {
+    lo = make_uint4(mul2<T>(decode2<T, F>(c.x, c.x, 0, 1), s2), mul2<T>(decode2<T, F>(c.x, c.x, 2, 3), s2),
+                    mul2<T>(decode2<T, F>(c.y, c.y, 0, 1), s2), mul2<T>(decode2<T, F>(c.y, c.y, 2, 3), s2));
+    hi = make_uint4(mul2<T>(decode2<T, F>(c.z, c.z, 0, 1), s2), mul2<T>(decode2<T, F>(c.z, c.z, 2, 3), s2),
+                    mul2<T>(decode2<T, F>(c.w, c.w, 0, 1), s2), mul2<T>(decode2<T, F>(c.w, c.w, 2, 3), s2));
+}
+
+// ---- write --------------------------------------------------------------------------------------
+struct WriteArgs {
+    const void* q;               // unused by the raw form
+    const void* k;
+    const void* v;
+    const int32_t* mask;         // NULL in the raw form
+    const int32_t* idx;          // NULL: row m is token m
+    const int32_t* count;        // NULL: host_count
+    int32_t host_count;
+    const int32_t* pos;
+    const float* norm_q;
+    const float* norm_k;
+    void* qc;
+    uint8_t* save;               // per compact row: K codes, V codes, K scales, V scales of mask==1 rows
+    int64_t ld_save;             // bytes
+    Cache c;
+    int64_t ld_qkv, ld_qc;
+    int32_t n_tokens, n_heads, n_axes;
+    float eps;
+    float2 turns[kPairs];        // revolutions per position of each rotary pair, as a sum of two floats; 0: not rotated
+    int8_t axis[kPairs];
+};
+
+// cos and sin of a rotary pair at position `pos`: the angle in revolutions, pos * turns, keeps its
+// fraction to ~2^-30 for every position up to 2^24 (the product's rounding error is recovered by an
+// fma), where a product in radians is off by pos * 2^-25. The codes are worth that: a K' near the
+// border of two codes moves by a whole step.
+__device__ __forceinline__ void rope_turn(float pos, float2 turns, float* sn, float* cs) {
+    const float t = pos * turns.x;
+    const float err = fmaf(pos, turns.x, -t);
+    const float frac = (t - rintf(t)) + fmaf(pos, turns.y, err);
+    sincospif(2.f * frac, sn, cs);
+}
+
+// RMSNorm + RoPE of one lane's 8 elements of a half-warp's head vector, in 32 bits.
+template <typename T>
+__device__ __forceinline__ void norm_rope8(const uint4& x, const float2* w2, float eps, const float* cs,
+                                           const float* sn, float* y) {
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+    float2 p[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) p[t] = StoreT<T>::unpack2(u[t]);
+    float2 s2 = f2mul(p[0], p[0]);
+#pragma unroll
+    for (int t = 1; t < 4; ++t) s2 = f2fma(p[t], p[t], s2);
+    float ss = s2.x + s2.y;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float r = rsqrtf(ss * (1.0f / kHeadDim) + eps);
+    const float2 r2 = make_float2(r, r);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const float2 ab = f2mul(f2mul(p[t], r2), w2[t]);
+        y[2 * t] = ab.x * cs[t] - ab.y * sn[t];
+        y[2 * t + 1] = ab.y * cs[t] + ab.x * sn[t];
+    }
+}
+
+// Quantises a half-warp's head vector (8 values per lane) and stores its codes and scale.
+template <typename T, int F>
+__device__ __forceinline__ void quantise_store(const float* y, uint8_t* codes, T* scale, int sub, bool active) {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(y[e]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float s = scale_of<T, F>(amax);
+    const uint2 w = encode8<F>(y, s);
+    if (active) {
+        *reinterpret_cast<uint2*>(codes + 8 * sub) = w;
+        if (sub == 0) {
+            const uint32_t p = StoreT<T>::pack2(s, s);
+            *reinterpret_cast<uint16_t*>(scale) = (uint16_t)p;
+        }
+    }
+}
+
+constexpr int kWriteThreads = 256;
+constexpr int kWriteWarps = kWriteThreads / 32;
+
+// Executed rows into the 8-bit cache. A half-warp holds a 128-wide head vector, 8 values per lane, so
+// that rotary pairs are lane-local and the sum of squares and the largest magnitude are 4-step
+// shuffles; a warp runs two heads of Q, K and V at a time. A row's heads are divided over `parts`
+// warps, as many as give every warp of the grid work (a few rows: one head pair per warp).
+// Bound by memory: 3 rows of T read, one of T and two of bytes written, per token.
+template <typename T, int F, bool kRaw>
+__global__ void __launch_bounds__(kWriteThreads) q8_write_kernel(const __grid_constant__ WriteArgs a) {
+    const int lane = threadIdx.x & 31, sub = lane & 15, half = lane >> 4;
+    const int32_t warp = blockIdx.x * kWriteWarps + (threadIdx.x >> 5), warps = gridDim.x * kWriteWarps;
+    float2 turns[4];
+    int axis[4];
+    float2 wq[4], wk[4];
+    if (!kRaw) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            turns[t] = a.turns[4 * sub + t];
+            axis[t] = a.axis[4 * sub + t];
+        }
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+    if (!kRaw) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            wq[t] = make_float2(a.norm_q[8 * sub + 2 * t], a.norm_q[8 * sub + 2 * t + 1]);
+            wk[t] = make_float2(a.norm_k[8 * sub + 2 * t], a.norm_k[8 * sub + 2 * t + 1]);
+        }
+    }
+    const int32_t m_all = min(a.count ? *a.count : a.host_count, a.n_tokens);
+    if (m_all <= 0) return;
+    const int32_t pairs = (a.n_heads + 1) >> 1;
+    const int32_t parts = max(1, min(pairs, warps / m_all));
+    const int64_t items = (int64_t)m_all * parts;
+    for (int64_t item = warp; item < items; item += warps) {
+        const int32_t m = (int32_t)(item / parts), part = (int32_t)(item - (int64_t)m * parts);
+        const int32_t i = a.idx ? a.idx[m] : m;
+        if (i < 0 || i >= a.n_tokens) {
+            if (lane == 0) atomicOr(&g_error_word, kErrBounds);
+            continue;
+        }
+        const bool keep = !kRaw && a.save != nullptr && a.mask[i] == 1;
+        float cs[4], sn[4];
+        if (!kRaw) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float at = a.n_axes > 0 ? (float)a.pos[(int64_t)i * a.n_axes + axis[t]] : 0.f;
+                rope_turn(at, turns[t], &sn[t], &cs[t]);
+            }
+        }
+        for (int32_t pr = part; pr < pairs; pr += parts) {
+            const int32_t h = 2 * pr + half;
+            const bool active = h < a.n_heads;
+            const int64_t col = (int64_t)(active ? h : 0) * kHeadDim + 8 * sub;
+            const int64_t at = (int64_t)i * a.ld_qkv + col;
+            uint4 xq;
+            if (!kRaw) xq = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at));
+            const uint4 xk = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.k) + at));
+            const uint4 xv = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + at));
+            uint8_t* ck = a.c.k + (int64_t)i * a.c.ld + (col - 8 * sub);
+            uint8_t* cv = a.c.v + (int64_t)i * a.c.ld + (col - 8 * sub);
+            T* ks = static_cast<T*>(a.c.ks) + (int64_t)(active ? h : 0) * a.c.ld_scale + i;
+            T* vs = static_cast<T*>(a.c.vs) + (int64_t)(active ? h : 0) * a.c.ld_scale + i;
+            if (keep && active) {
+                uint8_t* sv = a.save + (int64_t)m * a.ld_save;
+                const int64_t C = (int64_t)a.n_heads * kHeadDim;
+                *reinterpret_cast<uint2*>(sv + col) = *reinterpret_cast<const uint2*>(ck + 8 * sub);
+                *reinterpret_cast<uint2*>(sv + C + col) = *reinterpret_cast<const uint2*>(cv + 8 * sub);
+                if (sub == 0) {
+                    T* ss = reinterpret_cast<T*>(sv + 2 * C);
+                    ss[h] = *ks;
+                    ss[a.n_heads + h] = *vs;
+                }
+            }
+            float y[8];
+            if (!kRaw) {
+                norm_rope8<T>(xq, wq, a.eps, cs, sn, y);
+                if (active) {
+                    const uint4 o = make_uint4(StoreT<T>::pack2(y[0], y[1]), StoreT<T>::pack2(y[2], y[3]),
+                                               StoreT<T>::pack2(y[4], y[5]), StoreT<T>::pack2(y[6], y[7]));
+                    *reinterpret_cast<uint4*>(static_cast<T*>(a.qc) + (int64_t)m * a.ld_qc + col) = o;
+                }
+                norm_rope8<T>(xk, wk, a.eps, cs, sn, y);
+            } else {
+                const uint32_t u[4] = {xk.x, xk.y, xk.z, xk.w};
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const float2 p = StoreT<T>::unpack2(u[t]);
+                    y[2 * t] = p.x;
+                    y[2 * t + 1] = p.y;
+                }
+            }
+            quantise_store<T, F>(y, ck, ks, sub, active);
+            const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float2 p = StoreT<T>::unpack2(u[t]);
+                y[2 * t] = p.x;
+                y[2 * t + 1] = p.y;
+            }
+            quantise_store<T, F>(y, cv, vs, sub, active);
+        }
+    }
+}
+
+// ---- read ---------------------------------------------------------------------------------------
+struct ReadArgs {
+    Cache c;
+    const int32_t* idx;          // NULL: output row m is cache row m
+    const int32_t* count;        // NULL: host_count
+    int32_t host_count;
+    void* k;
+    void* v;
+    int64_t ld;
+    int32_t n_rows, n_heads;
+};
+
+constexpr int kReadThreads = 256;
+
+// Rows back in T: each thread turns 16 codes (16 bytes) into two 16-byte vectors. Bound by memory.
+template <typename T, int F>
+__global__ void __launch_bounds__(kReadThreads) q8_read_kernel(const __grid_constant__ ReadArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int32_t m_all = min(a.count ? *a.count : a.host_count, a.n_rows);
+    const int32_t per_row = a.n_heads * (kHeadDim / 16);   // 16-code chunks of a row
+    const int64_t total = (int64_t)m_all * per_row;
+    for (int64_t e = (int64_t)blockIdx.x * kReadThreads + threadIdx.x; e < total; e += (int64_t)gridDim.x * kReadThreads) {
+        const int32_t m = (int32_t)(e / per_row), c = (int32_t)(e - (int64_t)m * per_row);
+        const int32_t i = a.idx ? a.idx[m] : m;
+        if (i < 0 || i >= a.n_rows) {
+            if (c == 0) atomicOr(&g_error_word, kErrBounds);
+            continue;
+        }
+        const int64_t src = (int64_t)i * a.c.ld + c * 16, at = (int64_t)(c >> 3) * a.c.ld_scale + i;
+        const int64_t dst = (int64_t)m * a.ld + c * 16;
+        const uint4 ck = __ldcs(reinterpret_cast<const uint4*>(a.c.k + src));
+        const uint4 cv = __ldcs(reinterpret_cast<const uint4*>(a.c.v + src));
+        const uint32_t sk = scale_pair<T, F>(StoreT<T>::to_f(static_cast<const T*>(a.c.ks)[at]));
+        const uint32_t sv = scale_pair<T, F>(StoreT<T>::to_f(static_cast<const T*>(a.c.vs)[at]));
+        uint4 lo, hi;
+        decode16<T, F>(ck, sk, lo, hi);
+        uint4* ko = reinterpret_cast<uint4*>(static_cast<T*>(a.k) + dst);
+        __stcs(ko, lo);
+        __stcs(ko + 1, hi);
+        decode16<T, F>(cv, sv, lo, hi);
+        uint4* vo = reinterpret_cast<uint4*>(static_cast<T*>(a.v) + dst);
+        __stcs(vo, lo);
+        __stcs(vo + 1, hi);
+    }
+}
+
+// ---- restore ------------------------------------------------------------------------------------
+struct RestoreArgs {
+    Cache c;
+    const int32_t* mask;
+    const int32_t* idx;
+    const int32_t* count;
+    const uint8_t* save;
+    int64_t ld_save;
+    int32_t n_tokens, n_heads;
+};
+
+// Codes and scales of mask==1 rows back from `save`: a warp per executed row, which leaves at once
+// where the row keeps its new codes.
+__global__ void __launch_bounds__(256) q8_restore_kernel(const __grid_constant__ RestoreArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int32_t m_all = min(*a.count, a.n_tokens);
+    const int64_t C = (int64_t)a.n_heads * kHeadDim;
+    for (int32_t m = blockIdx.x * 8 + (threadIdx.x >> 5); m < m_all; m += gridDim.x * 8) {
+        const int32_t i = a.idx[m];
+        if (i < 0 || i >= a.n_tokens || a.mask[i] != 1) continue;   // a bad index: flagged by the write
+        const uint8_t* sv = a.save + (int64_t)m * a.ld_save;
+        for (int64_t e = lane * 16; e < C; e += 32 * 16) {
+            *reinterpret_cast<uint4*>(a.c.k + (int64_t)i * a.c.ld + e) = *reinterpret_cast<const uint4*>(sv + e);
+            *reinterpret_cast<uint4*>(a.c.v + (int64_t)i * a.c.ld + e) = *reinterpret_cast<const uint4*>(sv + C + e);
+        }
+        const uint16_t* ss = reinterpret_cast<const uint16_t*>(sv + 2 * C);
+        for (int32_t h = lane; h < a.n_heads; h += 32) {
+            static_cast<uint16_t*>(a.c.ks)[(int64_t)h * a.c.ld_scale + i] = ss[h];
+            static_cast<uint16_t*>(a.c.vs)[(int64_t)h * a.c.ld_scale + i] = ss[a.n_heads + h];
+        }
+    }
+}
+
+}  // namespace q8
+}  // namespace fxr

@@ -1,0 +1,348 @@
+// fxr_q8_api.cuh — extern "C" entry points of the 8-bit spatial cache (include/fxr.h): argument
+// checks and launches. Part of fxr_capi.cu's translation unit, whose helpers it uses.
+#pragma once
+
+namespace {
+
+int32_t check_q8_cache(const fxr_frame_desc* d, const fxr_q8_cache* c, int32_t rows, const char* what) {
+    if (!c) return fail(FXR_ERR_INVALID, "%s: null cache", what);
+    if (c->format != FXR_Q8_INT8 && c->format != FXR_Q8_E4M3)
+        return fail(FXR_ERR_INVALID, "%s: format %d is neither FXR_Q8_INT8 nor FXR_Q8_E4M3", what, c->format);
+    if (c->n_rows < rows) return fail(FXR_ERR_INVALID, "%s: %d rows, %d needed", what, c->n_rows, rows);
+    const int64_t C = (int64_t)d->n_heads * d->head_dim;
+    if (c->ld < C || (c->ld % 16)) return fail(FXR_ERR_INVALID, "%s: ld must be a multiple of 16, >= %lld", what, (long long)C);
+    if (c->ld_scale < c->n_rows || (c->ld_scale % 8))
+        return fail(FXR_ERR_INVALID, "%s: ld_scale must be a multiple of 8, >= n_rows", what);
+    if (c->n_rows == 0) return FXR_OK;
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(FXR_ERR_INVALID, "%s: null pointer", what);
+    if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_scale) || !aligned16(c->v_scale))
+        return fail(FXR_ERR_INVALID, "%s: codes and scales must be 16-byte aligned", what);
+    return FXR_OK;
+}
+
+fxr::q8::Cache q8_arg(const fxr_q8_cache* c) {
+    return fxr::q8::Cache{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), c->k_scale, c->v_scale, c->ld, c->ld_scale};
+}
+
+// f(T, F) for the frame's type and the cache's format.
+template <typename Fn>
+int32_t q8_dispatch(int32_t dtype, int32_t format, Fn&& f) {
+    using I8 = std::integral_constant<int, fxr::q8::kInt8>;
+    using E4 = std::integral_constant<int, fxr::q8::kE4m3>;
+    if (dtype == FXR_BF16) return format == FXR_Q8_INT8 ? f(__nv_bfloat16{}, I8{}) : f(__nv_bfloat16{}, E4{});
+    return format == FXR_Q8_INT8 ? f(__half{}, I8{}) : f(__half{}, E4{});
+}
+
+int64_t q8_save_bytes(const fxr_frame_desc* d) {
+    return (int64_t)align_up((size_t)d->n_heads * ((size_t)d->head_dim * 2 + 4), 16);
+}
+
+int32_t launch_q8_write(const fxr_frame_desc* d, const fxr_q8_cache* cache, fxr::q8::WriteArgs a, bool raw, int64_t max_rows,
+                        cudaStream_t s) {
+    NvtxRange nvtx_("fxr:q8_write");
+    a.c = q8_arg(cache);
+    a.n_tokens = d->n_tokens;
+    a.n_heads = d->n_heads;
+    a.n_axes = d->rope_n_axes;
+    a.eps = d->eps;
+    a.ld_save = q8_save_bytes(d);
+    for (int j = 0; j < fxr::kPairs; ++j) a.turns[j] = make_float2(0.f, 0.f);
+    for (int x = 0, j = 0; x < d->rope_n_axes; ++x) {
+        for (int jj = 0; jj < d->rope_axes_dim[x] / 2; ++jj, ++j) {
+            const double w = std::pow((double)d->rope_theta, -2.0 * jj / d->rope_axes_dim[x]) / 6.283185307179586;
+            const float hi = (float)w;
+            a.turns[j] = make_float2(hi, (float)(w - (double)hi));
+            a.axis[j] = (int8_t)x;
+        }
+    }
+    const int64_t units = max_rows * ((d->n_heads + 1) / 2);
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((units + fxr::q8::kWriteWarps - 1) / fxr::q8::kWriteWarps,
+                                                                (int64_t)sm_count() * 4));
+    return q8_dispatch(d->dtype, cache->format, [&](auto t, auto f) -> int32_t {
+        using T = decltype(t);
+        constexpr int F = decltype(f)::value;
+        const cudaError_t e = raw ? launch_pdl(fxr::q8::q8_write_kernel<T, F, true>, dim3(grid), dim3(fxr::q8::kWriteThreads), 0, s, a)
+                                  : launch_pdl(fxr::q8::q8_write_kernel<T, F, false>, dim3(grid), dim3(fxr::q8::kWriteThreads), 0, s, a);
+        return cuda_status(e, "q8_write_kernel launch");
+    });
+}
+
+// Workspace of the attention: arrivals, then partial results.
+struct Q8Work {
+    int32_t* cnt;
+    float* part;
+    int32_t slots;
+    size_t zero_bytes;    // from the start: what has to be zero before a launch
+    size_t total;
+};
+
+Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, int32_t max_rows, void* ws) {
+    Q8Work w{};
+    const int64_t R = max_rows > 0 ? std::min(max_rows, d->n_tokens) : d->n_tokens;
+    const int64_t S = std::min<int32_t>(n_streams, FXR_MAX_BATCH);
+    const int64_t tile = fxr::attn8::kRowsTile;
+    const int64_t groups = (n_prefix > 0 ? (S * R + tile - 1) / tile : 0) + S * ((R + tile - 1) / tile);
+    w.slots = (int32_t)std::min<int64_t>(INT32_MAX, sm_count() + groups * d->n_heads);
+    char* b = static_cast<char*>(ws);
+    w.cnt = reinterpret_cast<int32_t*>(b);
+    w.zero_bytes = align_up((size_t)d->n_heads * sizeof(int32_t), 256);
+    w.part = reinterpret_cast<float*>(b ? b + w.zero_bytes : nullptr);
+    w.total = w.zero_bytes + (size_t)w.slots * fxr::attn8::kRowsSlotFloats * sizeof(float);
+    return w;
+}
+
+template <typename T, int F>
+int32_t launch_q8_rows(const fxr::attn8::Params& p, cudaStream_t s) {
+    static bool configured[kMaxDevices] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= kMaxDevices) return fail(FXR_ERR_CUDA, "device %d", dev);
+    if (!configured[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(fxr::attn8::rows_kernel<T, F>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)fxr::attn8::kRowsSmem);
+        if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(rows_kernel)");
+        configured[dev] = true;
+    }
+    return cuda_status(launch_pdl(fxr::attn8::rows_kernel<T, F>, dim3(sm_count()), dim3(fxr::attn8::kRowsThreads),
+                                  fxr::attn8::kRowsSmem, s, p),
+                       "rows_kernel launch");
+}
+
+int32_t check_groups(const uint32_t* g, const char* what) {
+    return (reinterpret_cast<uintptr_t>(g) & 3u) ? fail(FXR_ERR_INVALID, "%s must be 4-byte aligned", what) : FXR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fxr_q8_save_row_bytes(const fxr_frame_desc* desc) {
+    if (!desc || desc->n_heads <= 0 || desc->head_dim <= 0) return 0;
+    return (size_t)q8_save_bytes(desc);
+}
+
+int32_t fxr_gather_norm_rope_q8(const fxr_frame_desc* desc, const void* q, const void* k, const void* v,
+                                const int32_t* mask, const int32_t* idx, const int32_t* count, const int32_t* pos,
+                                const float* norm_q, const float* norm_k, void* qc, int64_t ld_qc,
+                                const fxr_q8_cache* cache, void* save, void* stream) {
+    int32_t st = check_desc(desc, false);
+    if (st != FXR_OK) return st;
+    if ((st = check_q8_cache(desc, cache, desc->n_tokens, "fxr_gather_norm_rope_q8")) != FXR_OK) return st;
+    if (desc->n_tokens == 0) return FXR_OK;
+    if (!q || !k || !v || !mask || !idx || !count || !norm_q || !norm_k || !qc || (desc->rope_n_axes > 0 && !pos))
+        return fail(FXR_ERR_INVALID, "null pointer argument");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(qc) || (save && !aligned16(save)))
+        return fail(FXR_ERR_INVALID, "Q/K/V/qc/save must be 16-byte aligned");
+    if (ld_qc < (int64_t)desc->n_heads * desc->head_dim || (ld_qc % 8))
+        return fail(FXR_ERR_INVALID, "ld_qc must be a multiple of 8, >= n_heads*head_dim");
+    fxr::q8::WriteArgs a{};
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.mask = mask;
+    a.idx = idx;
+    a.count = count;
+    a.pos = pos;
+    a.norm_q = norm_q;
+    a.norm_k = norm_k;
+    a.qc = qc;
+    a.ld_qc = ld_qc;
+    a.ld_qkv = desc->ld_qkv;
+    a.save = static_cast<uint8_t*>(save);
+    return launch_q8_write(desc, cache, a, false, desc->n_tokens, static_cast<cudaStream_t>(stream));
+}
+
+int32_t fxr_cache_write_q8(const fxr_frame_desc* desc, const void* cache_k, const void* cache_v, const int32_t* idx,
+                           const int32_t* count, int32_t host_count, const fxr_q8_cache* cache, void* stream) {
+    int32_t st = check_desc(desc, false);
+    if (st != FXR_OK) return st;
+    if ((st = check_q8_cache(desc, cache, desc->n_tokens, "fxr_cache_write_q8")) != FXR_OK) return st;
+    if (!count && host_count < 0) return fail(FXR_ERR_INVALID, "neither count nor host_count");
+    if (!count && host_count > desc->n_tokens) return fail(FXR_ERR_INVALID, "host_count %d > n_tokens", host_count);
+    if (desc->n_tokens == 0 || (!count && host_count == 0)) return FXR_OK;
+    if (!cache_k || !cache_v) return fail(FXR_ERR_INVALID, "null pointer argument");
+    if (!aligned16(cache_k) || !aligned16(cache_v)) return fail(FXR_ERR_INVALID, "cache_k/cache_v must be 16-byte aligned");
+    fxr::q8::WriteArgs a{};
+    a.k = cache_k;
+    a.v = cache_v;
+    a.idx = idx;
+    a.count = count;
+    a.host_count = host_count;
+    a.ld_qkv = desc->ld_cache;
+    return launch_q8_write(desc, cache, a, true, count ? desc->n_tokens : host_count, static_cast<cudaStream_t>(stream));
+}
+
+int32_t fxr_cache_read_q8(const fxr_frame_desc* desc, const fxr_q8_cache* cache, const int32_t* idx, const int32_t* count,
+                          int32_t host_count, void* k, void* v, int64_t ld, void* stream) {
+    NvtxRange nvtx_("fxr:q8_read");
+    int32_t st = check_desc(desc, false);
+    if (st != FXR_OK) return st;
+    if ((st = check_q8_cache(desc, cache, 0, "fxr_cache_read_q8")) != FXR_OK) return st;
+    if (!count && host_count < 0) return fail(FXR_ERR_INVALID, "neither count nor host_count");
+    if (!count && host_count > cache->n_rows) return fail(FXR_ERR_INVALID, "host_count %d > %d cache rows", host_count, cache->n_rows);
+    if (cache->n_rows == 0 || (!count && host_count == 0)) return FXR_OK;
+    if (!k || !v) return fail(FXR_ERR_INVALID, "null pointer argument");
+    if (!aligned16(k) || !aligned16(v)) return fail(FXR_ERR_INVALID, "k/v must be 16-byte aligned");
+    if (ld < (int64_t)desc->n_heads * desc->head_dim || (ld % 8))
+        return fail(FXR_ERR_INVALID, "ld must be a multiple of 8, >= n_heads*head_dim");
+    fxr::q8::ReadArgs a{q8_arg(cache), idx, count, host_count, k, v, ld, cache->n_rows, desc->n_heads};
+    const int64_t units = (int64_t)(count ? cache->n_rows : host_count) * desc->n_heads * (fxr::kHeadDim / 16);
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((units + fxr::q8::kReadThreads - 1) / fxr::q8::kReadThreads,
+                                                                (int64_t)sm_count() * 8));
+    return q8_dispatch(desc->dtype, cache->format, [&](auto t, auto f) -> int32_t {
+        using T = decltype(t);
+        constexpr int F = decltype(f)::value;
+        return cuda_status(launch_pdl(fxr::q8::q8_read_kernel<T, F>, dim3(grid), dim3(fxr::q8::kReadThreads), 0,
+                                      static_cast<cudaStream_t>(stream), a),
+                           "q8_read_kernel launch");
+    });
+}
+
+int32_t fxr_restore_rows_q8(const fxr_frame_desc* desc, const int32_t* mask, const int32_t* idx, const int32_t* count,
+                            const void* save, const fxr_q8_cache* cache, void* stream) {
+    NvtxRange nvtx_("fxr:q8_restore");
+    int32_t st = check_desc(desc, false);
+    if (st != FXR_OK) return st;
+    if ((st = check_q8_cache(desc, cache, desc->n_tokens, "fxr_restore_rows_q8")) != FXR_OK) return st;
+    if (desc->n_tokens == 0) return FXR_OK;
+    if (!mask || !idx || !count || !save) return fail(FXR_ERR_INVALID, "null pointer argument");
+    if (!aligned16(save)) return fail(FXR_ERR_INVALID, "save must be 16-byte aligned");
+    fxr::q8::RestoreArgs a{q8_arg(cache), mask, idx, count, static_cast<const uint8_t*>(save), q8_save_bytes(desc),
+                           desc->n_tokens, desc->n_heads};
+    return cuda_status(launch_pdl(fxr::q8::q8_restore_kernel, dim3(grid_rows(desc->n_tokens, 8)), dim3(256), 0,
+                                  static_cast<cudaStream_t>(stream), a),
+                       "q8_restore_kernel launch");
+}
+
+size_t fxr_attention_q8_workspace_size(const fxr_frame_desc* desc, int32_t n_streams, int32_t n_prefix, int32_t max_rows) {
+    if (!desc || desc->n_heads <= 0 || desc->n_tokens < 0 || n_streams <= 0 || n_prefix < 0) return 0;
+    return carve_q8(desc, n_streams, n_prefix, max_rows, nullptr).total;
+}
+
+int32_t fxr_attention_q8(const fxr_frame_desc* desc, int32_t n_streams, const fxr_q8_stream* streams,
+                         const fxr_q8_cache* prefix, const uint32_t* prefix_groups, int32_t max_rows, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+    NvtxRange nvtx_("fxr:attention_q8");
+    int32_t st = check_desc(desc, true);
+    if (st != FXR_OK) return st;
+    if (n_streams < 0) return fail(FXR_ERR_INVALID, "n_streams < 0");
+    if (n_streams == 0 || desc->n_tokens == 0) return FXR_OK;
+    if (!streams) return fail(FXR_ERR_INVALID, "null streams");
+    const int32_t n_prefix = prefix ? prefix->n_rows : 0;
+    if (prefix && (st = check_q8_cache(desc, prefix, 0, "prefix")) != FXR_OK) return st;
+    if ((st = check_groups(prefix_groups, "prefix_groups")) != FXR_OK) return st;
+    const int64_t C = (int64_t)desc->n_heads * desc->head_dim;
+    for (int32_t b = 0; b < n_streams; ++b) {
+        const fxr_q8_stream& s = streams[b];
+        if ((st = check_q8_cache(desc, &s.cache, desc->n_tokens, "stream cache")) != FXR_OK) return st;
+        if (s.cache.format != streams[0].cache.format || (prefix && s.cache.format != prefix->format))
+            return fail(FXR_ERR_INVALID, "stream %d: the caches of a call share one format", b);
+        if (!s.qc || !s.idx || !s.count || !s.out) return fail(FXR_ERR_INVALID, "stream %d: null pointer", b);
+        if (!aligned16(s.qc) || !aligned16(s.out)) return fail(FXR_ERR_INVALID, "stream %d: qc/out must be 16-byte aligned", b);
+        if (s.ld_qc < C || (s.ld_qc % 8)) return fail(FXR_ERR_INVALID, "stream %d: ld_qc must be a multiple of 8, >= n_heads*head_dim", b);
+        if ((st = check_groups(s.q_groups, "q_groups")) != FXR_OK || (st = check_groups(s.k_groups, "k_groups")) != FXR_OK) return st;
+    }
+    const Q8Work w = carve_q8(desc, n_streams, n_prefix, max_rows, workspace);
+    if (!workspace) return fail(FXR_ERR_INVALID, "null workspace");
+    if (!aligned16(workspace)) return fail(FXR_ERR_INVALID, "workspace must be 16-byte aligned");
+    if (workspace_bytes < w.total) return fail(FXR_ERR_WORKSPACE, "workspace %zu < required %zu", workspace_bytes, w.total);
+    for (int32_t b0 = 0; b0 < n_streams; b0 += FXR_MAX_BATCH) {
+        fxr::attn8::Params p{};
+        p.n_streams = std::min(n_streams - b0, FXR_MAX_BATCH);
+        for (int32_t b = 0; b < p.n_streams; ++b) {
+            const fxr_q8_stream& s = streams[b0 + b];
+            p.s[b] = fxr::attn8::Stream{s.qc, s.idx, s.count, s.out, s.q_groups, s.k_groups, s.ld_qc, q8_arg(&s.cache)};
+        }
+        if (prefix) p.prefix = q8_arg(prefix);
+        p.pg = prefix_groups;
+        p.n_tokens = desc->n_tokens;
+        p.n_prefix = n_prefix;
+        p.n_heads = desc->n_heads;
+        p.max_rows = max_rows > 0 ? std::min(max_rows, desc->n_tokens) : desc->n_tokens;
+        p.ld_out = desc->ld_out;
+        p.scale_log2 = (desc->softmax_scale > 0.f ? desc->softmax_scale : 1.0f / std::sqrt((float)desc->head_dim)) * 1.4426950408889634f;
+        p.part = w.part;
+        p.cnt = w.cnt;
+        p.slots = w.slots;
+        st = q8_dispatch(desc->dtype, streams[0].cache.format, [&](auto t, auto f) -> int32_t {
+            return launch_q8_rows<decltype(t), decltype(f)::value>(p, static_cast<cudaStream_t>(stream));
+        });
+        if (st != FXR_OK) return st;
+    }
+    return FXR_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+struct Q8FrameViews {
+    int32_t* count;
+    int32_t* idx;
+    void* qc;
+    void* save;
+    char* attn;
+    size_t attn_bytes, total;
+};
+
+Q8FrameViews carve_q8_frame(const fxr_frame_desc* d, int32_t n_prefix, int32_t max_rows, void* ws) {
+    Q8FrameViews v{};
+    const size_t N = (size_t)(d->n_tokens > 0 ? d->n_tokens : 1), C = (size_t)d->n_heads * d->head_dim;
+    size_t off = 0;
+    char* b = static_cast<char*>(ws);
+    auto take = [&](size_t bytes) {
+        char* p = b ? b + off : nullptr;
+        off = align_up(off + bytes, 256);
+        return p;
+    };
+    v.count = reinterpret_cast<int32_t*>(take(sizeof(int32_t)));
+    v.idx = reinterpret_cast<int32_t*>(take(N * sizeof(int32_t)));
+    v.qc = take(N * C * dtype_bytes(d->dtype));
+    v.save = take(N * (size_t)q8_save_bytes(d));
+    v.attn_bytes = carve_q8(d, 1, n_prefix, max_rows, nullptr).total;
+    v.attn = take(v.attn_bytes);
+    v.total = off;
+    return v;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fxr_frame_q8_workspace_size(const fxr_frame_desc* desc, int32_t n_prefix, int32_t max_rows) {
+    if (!desc || dtype_bytes(desc->dtype) == 0 || desc->n_heads <= 0 || desc->head_dim <= 0 || desc->n_tokens < 0 || n_prefix < 0)
+        return 0;
+    return carve_q8_frame(desc, n_prefix, max_rows, nullptr).total;
+}
+
+int32_t fxr_frame_forward_q8(const fxr_frame_desc* desc, const void* q, const void* k, const void* v, int32_t* mask,
+                             const uint8_t* valid, const int32_t* pos, const float* norm_q, const float* norm_k,
+                             const fxr_q8_cache* cache, const uint32_t* q_groups, const uint32_t* k_groups,
+                             const fxr_q8_cache* prefix, const uint32_t* prefix_groups, int32_t max_rows, void* out,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+    NvtxRange nvtx_("fxr:frame_q8");
+    int32_t st = check_desc(desc, true);
+    if (st != FXR_OK) return st;
+    if (desc->n_tokens == 0) return FXR_OK;
+    if (!cache || !mask || !out) return fail(FXR_ERR_INVALID, "null pointer argument");
+    if (!workspace) return fail(FXR_ERR_INVALID, "null workspace");
+    if (!aligned16(workspace)) return fail(FXR_ERR_INVALID, "workspace must be 16-byte aligned");
+    const int32_t n_prefix = prefix ? prefix->n_rows : 0;
+    if (n_prefix < 0) return fail(FXR_ERR_INVALID, "prefix: n_rows < 0");
+    const Q8FrameViews w = carve_q8_frame(desc, n_prefix, max_rows, workspace);
+    if (workspace_bytes < w.total) return fail(FXR_ERR_WORKSPACE, "workspace %zu < required %zu", workspace_bytes, w.total);
+    const int64_t C = (int64_t)desc->n_heads * desc->head_dim;
+    fxr::CompactArgs ca{};
+    ca.s[0] = fxr::CompactStream{mask, valid, w.idx, w.count, fxr::RestoreList{}};
+    // the compaction also zeroes the attention's arrivals
+    st = launch_compact_streams(ca, 1, desc->n_tokens, SplitArea{}, stream, w.attn,
+                                carve_q8(desc, 1, n_prefix, max_rows, nullptr).zero_bytes);
+    if (st != FXR_OK) return st;
+    if ((st = fxr_gather_norm_rope_q8(desc, q, k, v, mask, w.idx, w.count, pos, norm_q, norm_k, w.qc, C, cache, w.save, stream)) != FXR_OK)
+        return st;
+    const fxr_q8_stream s{w.qc, C, w.idx, w.count, out, q_groups, k_groups, *cache};
+    if ((st = fxr_attention_q8(desc, 1, &s, prefix, prefix_groups, max_rows, w.attn, w.attn_bytes, stream)) != FXR_OK) return st;
+    return fxr_restore_rows_q8(desc, mask, w.idx, w.count, w.save, cache, stream);
+}
+
+}  // extern "C"

@@ -45,9 +45,14 @@ EXPORTED = [
     "fxr_double_block_workspace_size", "fxr_double_block_forward",
     "fxr_single_block_workspace_size", "fxr_single_block_forward",
     "fxr_block_host_workspace_size", "fxr_double_block_forward_host", "fxr_single_block_forward_host",
+    "fxr_q8_save_row_bytes", "fxr_gather_norm_rope_q8", "fxr_cache_write_q8", "fxr_cache_read_q8",
+    "fxr_restore_rows_q8", "fxr_attention_q8_workspace_size", "fxr_attention_q8",
+    "fxr_frame_q8_workspace_size", "fxr_frame_forward_q8",
 ]
 
 FXR_ACT_NONE, FXR_ACT_GELU_TANH = 0, 1
+
+FXR_Q8_INT8, FXR_Q8_E4M3 = 0, 1
 
 FXR_MAX_BATCH = 8
 
@@ -119,6 +124,20 @@ class TensorDesc(ctypes.Structure):
 class StreamFrame(ctypes.Structure):
     """Mirror of fxr_stream_frame (include/fxr.h)."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "mask", "valid", "cache_k", "cache_v", "out")]
+
+
+class Q8CacheStruct(ctypes.Structure):
+    """Mirror of fxr_q8_cache (include/fxr.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("ld", ctypes.c_int64), ("ld_scale", ctypes.c_int64),
+                ("n_rows", ctypes.c_int32), ("format", ctypes.c_int32)]
+
+
+class Q8StreamStruct(ctypes.Structure):
+    """Mirror of fxr_q8_stream (include/fxr.h)."""
+    _fields_ = [("qc", ctypes.c_void_p), ("ld_qc", ctypes.c_int64), ("idx", ctypes.c_void_p),
+                ("count", ctypes.c_void_p), ("out", ctypes.c_void_p), ("q_groups", ctypes.c_void_p),
+                ("k_groups", ctypes.c_void_p), ("cache", Q8CacheStruct)]
 
 
 class HeadGroup(ctypes.Structure):
@@ -223,6 +242,21 @@ def load(path: str | None = None) -> ctypes.CDLL:
     L.fxr_batch_workspace_size.restype = ctypes.c_size_t
     L.fxr_frame_forward_batch.argtypes = [ctypes.POINTER(FrameDesc), _i32, ctypes.POINTER(StreamFrame),
                                           _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]
+    _fd, _qc = ctypes.POINTER(FrameDesc), ctypes.POINTER(Q8CacheStruct)
+    L.fxr_q8_save_row_bytes.argtypes = [_fd]
+    L.fxr_q8_save_row_bytes.restype = ctypes.c_size_t
+    L.fxr_gather_norm_rope_q8.argtypes = [_fd] + [_vp] * 10 + [_i64, _qc, _vp, _vp]
+    L.fxr_cache_write_q8.argtypes = [_fd, _vp, _vp, _vp, _vp, _i32, _qc, _vp]
+    L.fxr_cache_read_q8.argtypes = [_fd, _qc, _vp, _vp, _i32, _vp, _vp, _i64, _vp]
+    L.fxr_restore_rows_q8.argtypes = [_fd, _vp, _vp, _vp, _vp, _qc, _vp]
+    L.fxr_attention_q8_workspace_size.argtypes = [_fd, _i32, _i32, _i32]
+    L.fxr_attention_q8_workspace_size.restype = ctypes.c_size_t
+    L.fxr_attention_q8.argtypes = [_fd, _i32, ctypes.POINTER(Q8StreamStruct), _qc, _vp, _i32, _vp,
+                                   ctypes.c_size_t, _vp]
+    L.fxr_frame_q8_workspace_size.argtypes = [_fd, _i32, _i32]
+    L.fxr_frame_q8_workspace_size.restype = ctypes.c_size_t
+    L.fxr_frame_forward_q8.argtypes = [_fd] + [_vp] * 8 + [_qc, _vp, _vp, _qc, _vp, _i32, _vp, _vp,
+                                                           ctypes.c_size_t, _vp]
     _hg = ctypes.POINTER(HeadGroup)
     L.fxr_head_group_init.argtypes = [_hg, _i32, _i32, _i32, _i32]
     L.fxr_frame_forward_heads.argtypes = [ctypes.POINTER(FrameDesc), _hg] + [_vp] * 11 + \
@@ -720,6 +754,193 @@ def frame_forward_batch(cfg: FrameConfig, streams, pos, norm_q, norm_k, workspac
                                           _ptr(norm_k), _ptr(workspace),
                                           workspace.numel() * workspace.element_size(),
                                           _stream(stream)))
+
+
+# ---- the 8-bit spatial cache ---------------------------------------------------------------------
+def _refuse(msg: str):
+    raise FxrError(FXR_ERR_INVALID, msg)
+
+
+def _here(*tensors):
+    """Refuses tensors of another device than the current one, whose stream the call would use."""
+    import torch
+    at = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != at:
+            _refuse(f"tensor on {t.device}, the current device is cuda:{at}")
+
+
+def _groups(t, rows: int, what: str):
+    import torch
+    if t is not None and (t.dtype not in (torch.int32, torch.uint32) or not t.is_contiguous() or t.numel() < rows):
+        _refuse(f"{what}: at least {rows} contiguous 32-bit words")
+
+
+class CacheQ8:
+    """An 8-bit K/V cache (fxr_q8_cache). k, v: codes [n_rows, >= heads * 128], int8 or float8_e4m3fn;
+    k_scale, v_scale: [heads, ld_scale >= n_rows, a multiple of 8] of the frame's 16-bit type. The
+    tensors are the caller's; the object keeps references to them."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        import torch
+        formats = {torch.int8: FXR_Q8_INT8, torch.float8_e4m3fn: FXR_Q8_E4M3}
+        if k.dtype not in formats or v.dtype != k.dtype:
+            _refuse(f"codes are int8 or float8_e4m3fn, K and V alike: got {k.dtype}, {v.dtype}")
+        if k_scale.dtype not in (torch.bfloat16, torch.float16) or v_scale.dtype != k_scale.dtype:
+            _refuse(f"scales are bfloat16 or float16, K and V alike: got {k_scale.dtype}, {v_scale.dtype}")
+        if k.dim() != 2 or k.shape != v.shape or k.stride() != v.stride() or k.stride(1) != 1:
+            _refuse("K and V codes: [n_rows, columns] of one shape and row stride")
+        if k_scale.dim() != 2 or k_scale.shape != v_scale.shape or k_scale.stride() != v_scale.stride() or \
+                k_scale.stride(1) != 1 or k_scale.shape[1] < k.shape[0] or k_scale.shape[0] * 128 > k.shape[1]:
+            _refuse("K and V scales: [heads, >= n_rows] of one shape and row stride, 128 code columns per head")
+        if len({t.device for t in (k, v, k_scale, v_scale)}) > 1:
+            _refuse("codes and scales on one device")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_rows, self.n_heads = k.shape[0], k_scale.shape[0]
+        # a single row or head has no stride of its own
+        ld = k.stride(0) if k.shape[0] > 1 else max(k.stride(0), k.shape[1])
+        ld_scale = k_scale.stride(0) if k_scale.shape[0] > 1 else k_scale.shape[1] // 8 * 8
+        self.struct = Q8CacheStruct(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), ld, ld_scale, k.shape[0],
+                                    formats[k.dtype])
+
+    @classmethod
+    def empty(cls, cfg: FrameConfig, n_rows: int | None = None, fmt: str = "int8", device="cuda") -> "CacheQ8":
+        """A cache of n_rows (default: the frame's tokens), codes and scales 0. fmt: "int8" | "e4m3"."""
+        import torch
+        n = cfg.n_tokens if n_rows is None else n_rows
+        code = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}[fmt]
+        scale = {"bf16": torch.bfloat16, "f16": torch.float16}[cfg.dtype]
+        kv = [torch.zeros(n, cfg.n_heads * cfg.head_dim, dtype=torch.int8, device=device).view(code) for _ in range(2)]
+        sc = [torch.zeros(cfg.n_heads, max(8, -(-n // 8) * 8), dtype=scale, device=device) for _ in range(2)]
+        return cls(*kv, *sc)
+
+    def check(self, cfg: FrameConfig, rows: int, what: str = "cache"):
+        import torch
+        if self.n_heads < cfg.n_heads or self.n_rows < rows or \
+                self.k_scale.dtype != {"bf16": torch.bfloat16, "f16": torch.float16}.get(cfg.dtype):
+            _refuse(f"{what}: {self.n_rows} rows, {self.n_heads} heads, {self.k_scale.dtype} scales for a frame of "
+                    f"{rows} rows, {cfg.n_heads} heads, {cfg.dtype}")
+        _here(self.k)
+
+
+def q8_save_row_bytes(cfg: FrameConfig) -> int:
+    return int(load().fxr_q8_save_row_bytes(ctypes.byref(cfg.desc())))
+
+
+def gather_norm_rope_q8(cfg: FrameConfig, q, k, v, mask, idx, count, pos, norm_q, norm_k, qc, cache: CacheQ8,
+                        save=None, stream=None):
+    """gather_norm_rope into an 8-bit cache (fxr_gather_norm_rope_q8). save: uint8 [N, q8_save_row_bytes(cfg)]."""
+    d = cfg.desc()
+    cache.check(cfg, cfg.n_tokens)
+    _check(load().fxr_gather_norm_rope_q8(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(mask), _ptr(idx),
+                                          _ptr(count), _ptr(pos), _ptr(norm_q), _ptr(norm_k), _ptr(qc), qc.stride(0),
+                                          ctypes.byref(cache.struct), _ptr(save), _stream(stream)))
+
+
+def cache_write_q8(cfg: FrameConfig, cache_k, cache_v, cache: CacheQ8, idx=None, count=None, host_count: int = -1,
+                   stream=None):
+    """Rows of a 16-bit cache (row stride cfg.ld_cache) into an 8-bit one, listed by idx / count or, by
+    default, all of the frame's tokens."""
+    d = cfg.desc()
+    cache.check(cfg, cfg.n_tokens)
+    if idx is None and count is None and host_count < 0:
+        host_count = cfg.n_tokens
+    _check(load().fxr_cache_write_q8(ctypes.byref(d), _ptr(cache_k), _ptr(cache_v), _ptr(idx), _ptr(count), host_count,
+                                     ctypes.byref(cache.struct), _stream(stream)))
+
+
+def cache_read_q8(cfg: FrameConfig, cache: CacheQ8, k, v, idx=None, count=None, host_count: int = -1, stream=None):
+    """Cache rows back in the frame's type: k[m], v[m] = row idx[m], or by default every row of the cache."""
+    d = cfg.desc()
+    cache.check(cfg, 0)
+    if k.stride() != v.stride():
+        _refuse("k and v: one row stride")
+    if idx is None and count is None and host_count < 0:
+        host_count = cache.n_rows
+    _check(load().fxr_cache_read_q8(ctypes.byref(d), ctypes.byref(cache.struct), _ptr(idx), _ptr(count), host_count,
+                                    _ptr(k), _ptr(v), k.stride(0), _stream(stream)))
+
+
+def restore_rows_q8(cfg: FrameConfig, mask, idx, count, save, cache: CacheQ8, stream=None):
+    d = cfg.desc()
+    cache.check(cfg, cfg.n_tokens)
+    _check(load().fxr_restore_rows_q8(ctypes.byref(d), _ptr(mask), _ptr(idx), _ptr(count), _ptr(save),
+                                      ctypes.byref(cache.struct), _stream(stream)))
+
+
+class Q8Streams:
+    """The streams of an attention_q8 call, built once by q8_streams() and used as often as wanted."""
+
+    def __init__(self, streams):
+        self.streams = streams                  # keeps the tensors alive
+        self.array = (Q8StreamStruct * max(len(streams), 1))()
+        for b, f in enumerate(streams):
+            self.array[b] = Q8StreamStruct(_ptr(f["qc"]), f["qc"].stride(0) if f["qc"].shape[0] > 1 else f["qc"].shape[1],
+                                           _ptr(f["idx"]), _ptr(f["count"]), _ptr(f["out"]), _ptr(f.get("q_groups")),
+                                           _ptr(f.get("k_groups")), f["cache"].struct)
+
+    def check(self, cfg: FrameConfig):
+        n = cfg.n_tokens
+        for f in self.streams:
+            f["cache"].check(cfg, n, "stream cache")
+            _groups(f.get("q_groups"), n, "q_groups")
+            _groups(f.get("k_groups"), n, "k_groups")
+            if f["out"].dtype != f["cache"].k_scale.dtype or f["qc"].dtype != f["out"].dtype:
+                _refuse("qc, out and the scales are of one type")
+            _here(f["qc"], f["idx"], f["count"], f["out"], f.get("q_groups"), f.get("k_groups"))
+
+
+def q8_streams(streams) -> Q8Streams:
+    """streams: list of dicts with qc, idx, count, out tensors, cache (CacheQ8) and, optionally, q_groups
+    and k_groups (int32 or uint32 [N])."""
+    return Q8Streams(list(streams))
+
+
+def attention_q8_workspace_size(cfg: FrameConfig, n_streams: int = 1, n_prefix: int = 0, max_rows: int = 0) -> int:
+    d = cfg.desc()
+    return int(load().fxr_attention_q8_workspace_size(ctypes.byref(d), n_streams, n_prefix, max_rows))
+
+
+def attention_q8(cfg: FrameConfig, streams, workspace, prefix: CacheQ8 | None = None, prefix_groups=None,
+                 max_rows: int = 0, stream=None):
+    """Attention of each stream's executed rows over the prefix and its own 8-bit cache
+    (fxr_attention_q8). streams: a list of dicts as for q8_streams(), or what it returned. workspace: a
+    zeroed uint8 tensor of attention_q8_workspace_size() bytes, reused as is."""
+    d = cfg.desc()
+    if not isinstance(streams, Q8Streams):
+        streams = q8_streams(streams)
+    streams.check(cfg)
+    if prefix is not None:
+        prefix.check(cfg, 0, "prefix")
+        _groups(prefix_groups, prefix.n_rows, "prefix_groups")
+    _here(workspace)
+    _check(load().fxr_attention_q8(ctypes.byref(d), len(streams.streams), streams.array,
+                                   ctypes.byref(prefix.struct) if prefix is not None else None, _ptr(prefix_groups),
+                                   max_rows, _ptr(workspace), workspace.numel() * workspace.element_size(),
+                                   _stream(stream)))
+
+
+def frame_q8_workspace_size(cfg: FrameConfig, n_prefix: int = 0, max_rows: int = 0) -> int:
+    d = cfg.desc()
+    return int(load().fxr_frame_q8_workspace_size(ctypes.byref(d), n_prefix, max_rows))
+
+
+def frame_forward_q8(cfg: FrameConfig, q, k, v, mask, valid, pos, norm_q, norm_k, cache: CacheQ8, out, workspace,
+                     prefix: CacheQ8 | None = None, prefix_groups=None, q_groups=None, k_groups=None,
+                     max_rows: int = 0, stream=None):
+    """One frame over an 8-bit cache (fxr_frame_forward_q8)."""
+    d = cfg.desc()
+    cache.check(cfg, cfg.n_tokens)
+    _groups(q_groups, cfg.n_tokens, "q_groups")
+    _groups(k_groups, cfg.n_tokens, "k_groups")
+    if prefix is not None:
+        prefix.check(cfg, 0, "prefix")
+        _groups(prefix_groups, prefix.n_rows, "prefix_groups")
+    _check(load().fxr_frame_forward_q8(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(mask), _ptr(valid), _ptr(pos),
+                                       _ptr(norm_q), _ptr(norm_k), ctypes.byref(cache.struct), _ptr(q_groups),
+                                       _ptr(k_groups), ctypes.byref(prefix.struct) if prefix is not None else None,
+                                       _ptr(prefix_groups), max_rows, _ptr(out), _ptr(workspace),
+                                       workspace.numel() * workspace.element_size(), _stream(stream)))
 
 
 def qkv_project(cfg: FrameConfig, hidden, w_qkv, bias, idx, count, q, k, v, scratch=None,

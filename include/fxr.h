@@ -623,6 +623,101 @@ int32_t fxr_frame_forward_heads_nccl(const fxr_frame_desc* desc, const fxr_head_
                                      void* cache_k, void* cache_v, void* out,
                                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- the 8-bit spatial cache --------------------------------------------------------------------
+ * A frame's K/V cache held in 8 bits: half the memory of a stream's caches and half the bytes that an
+ * attention of few rows reads. Each head vector (128 values of one token's K' or V) has its codes and
+ * one scale of the frame's type T (desc->dtype):
+ *   scale = max|x| / Q rounded up to T, Q = 127 (FXR_Q8_INT8) or 448 (FXR_Q8_E4M3)
+ *   code  = x / scale rounded to nearest even: a whole number in [-127, 127], or e4m3 (saturating)
+ *   read  = code * scale, rounded once to T
+ * A vector of zeros has scale 0. One that holds an infinity or NaN (or whose scale T cannot hold) has
+ * scale NaN and codes 0: it reads back as NaN, and an attention row that sees it is NaN. K' is
+ * quantised from its 32-bit value. (f16: the scale is rounded down where Q * scale would pass the
+ * largest f16 value, so that every finite vector reads back finite.) */
+typedef enum fxr_q8_format { FXR_Q8_INT8 = 0, FXR_Q8_E4M3 = 1 } fxr_q8_format;
+
+typedef struct fxr_q8_cache {
+    void* k;                 /* [n_rows, ld] codes, one byte each; head h at columns [h*D, (h+1)*D) */
+    void* v;
+    void* k_scale;           /* [n_heads, ld_scale] of the frame's type: entry (h, row) */
+    void* v_scale;
+    int64_t ld;              /* bytes between rows: a multiple of 16, >= n_heads*head_dim */
+    int64_t ld_scale;        /* elements between heads: a multiple of 8, >= n_rows */
+    int32_t n_rows;
+    int32_t format;          /* fxr_q8_format */
+} fxr_q8_cache;              /* all four pointers 16-byte aligned */
+
+/* fxr_gather_norm_rope with an 8-bit cache: for m < *count, token i = idx[m]:
+ *   qc[m] = rope(rmsnorm(Q[i], norm_q))     (angles exact to ~1e-8 for positions up to 2^24)
+ *   if mask[i] == 1: save[m] = the cache row's codes and scales (put back by fxr_restore_rows_q8)
+ *   cache row i = quantised rope(rmsnorm(K[i], norm_k)) and V[i]
+ * save: [N] rows of fxr_q8_save_row_bytes(desc) bytes, 16-byte aligned; may be NULL when no mask value
+ * is 1. cache->n_rows >= n_tokens; cache rows of tokens that are not listed keep what they hold. A
+ * token is listed at most once. An index outside [0, n_tokens) is skipped (FXR_ERR_BOUNDS from
+ * fxr_check_device_error). desc->ld_cache is not used. */
+size_t fxr_q8_save_row_bytes(const fxr_frame_desc* desc);
+int32_t fxr_gather_norm_rope_q8(const fxr_frame_desc* desc, const void* q, const void* k, const void* v,
+                                const int32_t* mask, const int32_t* idx, const int32_t* count, const int32_t* pos,
+                                const float* norm_q, const float* norm_k, void* qc, int64_t ld_qc,
+                                const fxr_q8_cache* cache, void* save, void* stream);
+
+/* Rows of an attention-ready 16-bit cache (cache_k / cache_v, row stride desc->ld_cache) into an 8-bit
+ * one: row i of the first becomes row i of the second, for the listed rows i = idx[m] < n_tokens, or
+ * for rows [0, count) when idx is NULL. count: device count, or NULL with host_count >= 0. */
+int32_t fxr_cache_write_q8(const fxr_frame_desc* desc, const void* cache_k, const void* cache_v, const int32_t* idx,
+                           const int32_t* count, int32_t host_count, const fxr_q8_cache* cache, void* stream);
+
+/* Cache rows back in T: row m of k and v (stride ld elements) = cache row idx[m], or row m when idx is
+ * NULL, for m < *count (or host_count when count is NULL; at most cache->n_rows). An index outside
+ * [0, n_rows) is skipped and reported, its output row left untouched. */
+int32_t fxr_cache_read_q8(const fxr_frame_desc* desc, const fxr_q8_cache* cache, const int32_t* idx, const int32_t* count,
+                          int32_t host_count, void* k, void* v, int64_t ld, void* stream);
+
+/* Puts back the cache rows of mask==1 tokens from `save` (fxr_gather_norm_rope_q8). */
+int32_t fxr_restore_rows_q8(const fxr_frame_desc* desc, const int32_t* mask, const int32_t* idx, const int32_t* count,
+                            const void* save, const fxr_q8_cache* cache, void* stream);
+
+/* Attention of each stream's compact queries over an 8-bit cache, scattered: for m < *count,
+ *   out[idx[m], h*D..] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * qc[m, h] . k_j)
+ * over the rows of `prefix` (may be NULL: none; read-only, shared by every stream of the call, such as
+ * a prompt's and a reference picture's rows) and then rows [0, n_tokens) of the stream's own cache.
+ * Visibility groups (document masks, padded prompts): 32-bit sets per token, and a query sees a key
+ * where q_groups[idx[m]] & k_groups[j] (prefix_groups[j] for prefix rows) is not 0; NULL stands for
+ * all bits. A row that sees no key gets zeros. Masked keys contribute nothing, whatever they hold.
+ * max_rows: the caller's bound of *count for every stream (<= 0: n_tokens). Rows past it are not
+ * computed and set the device error word (FXR_ERR_BOUNDS). A tight bound lets calls of few rows take
+ * the kernel made for them. Rows of out that are not listed are left as they are.
+ * More than FXR_MAX_BATCH streams run as consecutive groups. workspace: at least
+ * fxr_attention_q8_workspace_size() bytes, 16-byte aligned, ZERO before its first use and then reused
+ * as is by calls on one stream (each call leaves its counters at zero; after FXR_ERR_TIMEOUT zero it
+ * again). Calls that may run at the same time need a workspace each. The caches of a call share one
+ * format. The result of a call does not depend on the order in which its CTAs run. */
+typedef struct fxr_q8_stream {
+    const void* qc;          /* [>= *count, ld_qc] compact queries (fxr_gather_norm_rope_q8), 16-byte aligned */
+    int64_t ld_qc;           /* elements, a multiple of 8 */
+    const int32_t* idx;
+    const int32_t* count;
+    void* out;               /* [n_tokens, desc->ld_out], 16-byte aligned */
+    const uint32_t* q_groups;/* [n_tokens] or NULL */
+    const uint32_t* k_groups;/* [n_tokens] or NULL */
+    fxr_q8_cache cache;      /* n_rows >= n_tokens */
+} fxr_q8_stream;
+
+size_t fxr_attention_q8_workspace_size(const fxr_frame_desc* desc, int32_t n_streams, int32_t n_prefix, int32_t max_rows);
+int32_t fxr_attention_q8(const fxr_frame_desc* desc, int32_t n_streams, const fxr_q8_stream* streams,
+                         const fxr_q8_cache* prefix, const uint32_t* prefix_groups, int32_t max_rows, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* One frame over an 8-bit cache: compact -> gather/norm/RoPE/quantised cache write -> attention +
+ * scatter -> restore of mask==1 rows; fxr_frame_forward with fxr_attention_q8's prefix, groups and
+ * max_rows. workspace: fxr_frame_q8_workspace_size() bytes, 16-byte aligned, of any content. */
+size_t fxr_frame_q8_workspace_size(const fxr_frame_desc* desc, int32_t n_prefix, int32_t max_rows);
+int32_t fxr_frame_forward_q8(const fxr_frame_desc* desc, const void* q, const void* k, const void* v, int32_t* mask,
+                             const uint8_t* valid, const int32_t* pos, const float* norm_q, const float* norm_k,
+                             const fxr_q8_cache* cache, const uint32_t* q_groups, const uint32_t* k_groups,
+                             const fxr_q8_cache* prefix, const uint32_t* prefix_groups, int32_t max_rows, void* out,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
 /* Device memory shareable between the processes of one node (CUDA IPC), for the output buffers and
  * arrival counters of a head group. fxr_ipc_alloc zero-fills `bytes` on the current device and
  * returns a 64-byte handle; fxr_ipc_open maps another process's handle (peer access enabled on
