@@ -67,27 +67,57 @@ int32_t launch_q8_write(const fxr_frame_desc* d, const fxr_q8_cache* cache, fxr:
     });
 }
 
-// Workspace of the attention: arrivals, then partial results.
+// Streams of at most this many rows take the kernel for few rows.
+constexpr int32_t kQ8RowsLimit = 64;
+
+// Workspace of the attention: arrivals (zero before and after a call), then partial results, then the
+// visible steps of the kernel for many rows.
 struct Q8Work {
     int32_t* cnt;
     float* part;
-    int32_t slots;
+    int32_t* steps;
+    uint16_t* list;
+    uint32_t* groups;
+    int32_t rows;         // bound of a stream's rows
+    bool few;             // the kernel for few rows
+    int32_t slots;        // its partial results
+    int32_t units;        // 256-row units of a stream, key tiles: the kernel for many
+    int32_t n_pre, n_own;
     size_t zero_bytes;    // from the start: what has to be zero before a launch
     size_t total;
 };
 
 Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, int32_t max_rows, void* ws) {
     Q8Work w{};
-    const int64_t R = max_rows > 0 ? std::min(max_rows, d->n_tokens) : d->n_tokens;
-    const int64_t S = std::min<int32_t>(n_streams, FXR_MAX_BATCH);
-    const int64_t tile = fxr::attn8::kRowsTile;
-    const int64_t groups = (n_prefix > 0 ? (S * R + tile - 1) / tile : 0) + S * ((R + tile - 1) / tile);
-    w.slots = (int32_t)std::min<int64_t>(INT32_MAX, sm_count() + groups * d->n_heads);
+    w.rows = max_rows > 0 ? std::min(max_rows, d->n_tokens) : d->n_tokens;
+    w.few = w.rows <= kQ8RowsLimit;
+    const int64_t S = std::min<int32_t>(n_streams, FXR_MAX_BATCH), R = w.rows;
+    size_t off = 0;
     char* b = static_cast<char*>(ws);
-    w.cnt = reinterpret_cast<int32_t*>(b);
-    w.zero_bytes = align_up((size_t)d->n_heads * sizeof(int32_t), 256);
-    w.part = reinterpret_cast<float*>(b ? b + w.zero_bytes : nullptr);
-    w.total = w.zero_bytes + (size_t)w.slots * fxr::attn8::kRowsSlotFloats * sizeof(float);
+    auto take = [&](size_t bytes) {
+        char* p = b ? b + off : nullptr;
+        off = align_up(off + bytes, 256);
+        return p;
+    };
+    // one place and size for the arrivals of either kernel: calls with other bounds may share a workspace
+    const size_t ctas = (size_t)sm_count();
+    w.cnt = reinterpret_cast<int32_t*>(take(std::max(ctas * fxr::attn8::kPartWarps, (size_t)d->n_heads) * sizeof(int32_t)));
+    w.zero_bytes = off;
+    if (w.few) {
+        const int64_t tile = fxr::attn8::kRowsTile;
+        const int64_t groups = (n_prefix > 0 ? (S * R + tile - 1) / tile : 0) + S * ((R + tile - 1) / tile);
+        w.slots = (int32_t)std::min<int64_t>(INT32_MAX, sm_count() + groups * d->n_heads);
+        w.part = reinterpret_cast<float*>(take((size_t)w.slots * fxr::attn8::kRowsSlotFloats * sizeof(float)));
+    } else {
+        w.units = (w.rows + fxr::attn8::kUnitRows - 1) / fxr::attn8::kUnitRows;
+        w.n_pre = (n_prefix + fxr::attn8::kBN - 1) / fxr::attn8::kBN;
+        w.n_own = (d->n_tokens + fxr::attn8::kBN - 1) / fxr::attn8::kBN;
+        w.part = reinterpret_cast<float*>(take(ctas * fxr::attn8::kPartSlots * fxr::attn8::kPartFloats * sizeof(float)));
+        w.steps = reinterpret_cast<int32_t*>(take((size_t)(S * w.units) * sizeof(int32_t)));
+        w.list = reinterpret_cast<uint16_t*>(take((size_t)(S * w.units) * (size_t)(w.n_pre + w.n_own) * sizeof(uint16_t)));
+        w.groups = reinterpret_cast<uint32_t*>(take((size_t)(w.n_pre + S * w.n_own) * fxr::attn8::kBN * sizeof(uint32_t)));
+    }
+    w.total = off;
     return w;
 }
 
@@ -106,6 +136,73 @@ int32_t launch_q8_rows(const fxr::attn8::Params& p, cudaStream_t s) {
     return cuda_status(launch_pdl(fxr::attn8::rows_kernel<T, F>, dim3(sm_count()), dim3(fxr::attn8::kRowsThreads),
                                   fxr::attn8::kRowsSmem, s, p),
                        "rows_kernel launch");
+}
+
+// 2-D map over rows of 8-bit codes: boxes of 128 rows x 128 bytes (a head), 128-byte swizzle.
+int32_t make_code_tmap(CUtensorMap* map, const void* ptr, int64_t cols, int64_t rows, int64_t ld) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(FXR_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {(cuuint32_t)fxr::attn8::kD, (cuuint32_t)fxr::attn8::kBN};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(FXR_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return FXR_OK;
+}
+
+template <typename T, int F>
+int32_t launch_q8_tiles(const fxr_frame_desc* d, const fxr::attn8::Params& p, const Q8Work& w, cudaStream_t s) {
+    static bool configured[kMaxDevices] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= kMaxDevices) return fail(FXR_ERR_CUDA, "device %d", dev);
+    if (!configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(fxr::attn8::tile_kernel<T, F>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)fxr::attn8::kTileSmem);
+        cudaFuncAttributes fa{};
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, fxr::attn8::tile_kernel<T, F>);
+        if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(tile_kernel)");
+        // the warpgroups redistribute the launch's registers: it must have been compiled to hold them
+        if ((uint32_t)fa.numRegs * fxr::attn8::kTileThreads < fxr::attn8::kTileRegPool)
+            return fail(FXR_ERR_UNSUPPORTED, "tile_kernel compiled to %d registers", fa.numRegs);
+        configured[dev] = true;
+    }
+    const int64_t C = (int64_t)d->n_heads * d->head_dim;
+    fxr::attn8::TileMaps maps;
+    std::memset(&maps, 0, sizeof(maps));
+    int32_t rc;
+    bool groups = p.pg != nullptr && p.n_prefix > 0;
+    for (int32_t b = 0; b < p.n_streams; ++b) {
+        if ((rc = make_tmap(&maps.q[b], p.s[b].qc, d->dtype, C, p.max_rows, p.s[b].ld_qc)) != FXR_OK) return rc;
+        if ((rc = make_code_tmap(&maps.k[b], p.s[b].c.k, C, p.n_tokens, p.s[b].c.ld)) != FXR_OK) return rc;
+        if ((rc = make_code_tmap(&maps.v[b], p.s[b].c.v, C, p.n_tokens, p.s[b].c.ld)) != FXR_OK) return rc;
+        groups = groups || p.s[b].qg != nullptr || p.s[b].kg != nullptr;
+    }
+    if (p.n_prefix > 0) {
+        if ((rc = make_code_tmap(&maps.pk, p.prefix.k, C, p.n_prefix, p.prefix.ld)) != FXR_OK) return rc;
+        if ((rc = make_code_tmap(&maps.pv, p.prefix.v, C, p.n_prefix, p.prefix.ld)) != FXR_OK) return rc;
+    }
+    fxr::attn8::TileParams a{};
+    a.p = p;
+    a.n_pre = w.n_pre;
+    a.n_own = w.n_own;
+    a.units_cap = w.units;
+    a.part = w.part;
+    a.cnt = w.cnt;
+    if (groups) {
+        const cudaError_t e = launch_pdl(fxr::attn8::visible_steps_kernel, dim3(w.units, p.n_streams), dim3(fxr::attn8::kVisThreads), 0,
+                                         s, a, w.steps, w.list, w.groups);
+        if (e != cudaSuccess) return cuda_status(e, "visible_steps_kernel launch");
+        a.steps = w.steps;
+        a.list = w.list;
+        a.groups = w.groups;
+    }
+    return cuda_status(launch_pdl(fxr::attn8::tile_kernel<T, F>, dim3(sm_count()), dim3(fxr::attn8::kTileThreads),
+                                  fxr::attn8::kTileSmem, s, maps, a),
+                       "tile_kernel launch");
 }
 
 int32_t check_groups(const uint32_t* g, const char* what) {
@@ -246,6 +343,8 @@ int32_t fxr_attention_q8(const fxr_frame_desc* desc, int32_t n_streams, const fx
     if (!workspace) return fail(FXR_ERR_INVALID, "null workspace");
     if (!aligned16(workspace)) return fail(FXR_ERR_INVALID, "workspace must be 16-byte aligned");
     if (workspace_bytes < w.total) return fail(FXR_ERR_WORKSPACE, "workspace %zu < required %zu", workspace_bytes, w.total);
+    if (!w.few && w.n_pre + w.n_own > 0x7fff)
+        return fail(FXR_ERR_UNSUPPORTED, "%d key rows: more than 32767 tiles of 128", n_prefix + desc->n_tokens);
     for (int32_t b0 = 0; b0 < n_streams; b0 += FXR_MAX_BATCH) {
         fxr::attn8::Params p{};
         p.n_streams = std::min(n_streams - b0, FXR_MAX_BATCH);
@@ -258,14 +357,16 @@ int32_t fxr_attention_q8(const fxr_frame_desc* desc, int32_t n_streams, const fx
         p.n_tokens = desc->n_tokens;
         p.n_prefix = n_prefix;
         p.n_heads = desc->n_heads;
-        p.max_rows = max_rows > 0 ? std::min(max_rows, desc->n_tokens) : desc->n_tokens;
+        p.max_rows = w.rows;
         p.ld_out = desc->ld_out;
         p.scale_log2 = (desc->softmax_scale > 0.f ? desc->softmax_scale : 1.0f / std::sqrt((float)desc->head_dim)) * 1.4426950408889634f;
         p.part = w.part;
         p.cnt = w.cnt;
-        p.slots = w.slots;
         st = q8_dispatch(desc->dtype, streams[0].cache.format, [&](auto t, auto f) -> int32_t {
-            return launch_q8_rows<decltype(t), decltype(f)::value>(p, static_cast<cudaStream_t>(stream));
+            using T = decltype(t);
+            constexpr int F = decltype(f)::value;
+            return w.few ? launch_q8_rows<T, F>(p, static_cast<cudaStream_t>(stream))
+                         : launch_q8_tiles<T, F>(desc, p, w, static_cast<cudaStream_t>(stream));
         });
         if (st != FXR_OK) return st;
     }

@@ -879,9 +879,12 @@ class Q8Streams:
                                            _ptr(f["idx"]), _ptr(f["count"]), _ptr(f["out"]), _ptr(f.get("q_groups")),
                                            _ptr(f.get("k_groups")), f["cache"].struct)
 
-    def check(self, cfg: FrameConfig):
+    def check(self, cfg: FrameConfig, max_rows: int = 0):
         n = cfg.n_tokens
+        rows = min(max_rows, n) if max_rows > 0 else n
         for f in self.streams:
+            if f["qc"].shape[0] < rows:
+                _refuse(f"qc holds {f['qc'].shape[0]} rows, the bound is {rows}")
             f["cache"].check(cfg, n, "stream cache")
             _groups(f.get("q_groups"), n, "q_groups")
             _groups(f.get("k_groups"), n, "k_groups")
@@ -909,7 +912,7 @@ def attention_q8(cfg: FrameConfig, streams, workspace, prefix: CacheQ8 | None = 
     d = cfg.desc()
     if not isinstance(streams, Q8Streams):
         streams = q8_streams(streams)
-    streams.check(cfg)
+    streams.check(cfg, max_rows)
     if prefix is not None:
         prefix.check(cfg, 0, "prefix")
         _groups(prefix_groups, prefix.n_rows, "prefix_groups")

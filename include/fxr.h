@@ -685,15 +685,15 @@ int32_t fxr_restore_rows_q8(const fxr_frame_desc* desc, const int32_t* mask, con
  * where q_groups[idx[m]] & k_groups[j] (prefix_groups[j] for prefix rows) is not 0; NULL stands for
  * all bits. A row that sees no key gets zeros. Masked keys contribute nothing, whatever they hold.
  * max_rows: the caller's bound of *count for every stream (<= 0: n_tokens). Rows past it are not
- * computed and set the device error word (FXR_ERR_BOUNDS). A tight bound lets calls of few rows take
- * the kernel made for them. Rows of out that are not listed are left as they are.
+ * computed and set the device error word (FXR_ERR_BOUNDS). qc has to hold max_rows rows: those past
+ * *count are read, never used. A tight bound lets calls of few rows take the kernel made for them. Rows of out that are not listed are left as they are.
  * More than FXR_MAX_BATCH streams run as consecutive groups. workspace: at least
  * fxr_attention_q8_workspace_size() bytes, 16-byte aligned, ZERO before its first use and then reused
  * as is by calls on one stream (each call leaves its counters at zero; after FXR_ERR_TIMEOUT zero it
  * again). Calls that may run at the same time need a workspace each. The caches of a call share one
  * format. The result of a call does not depend on the order in which its CTAs run. */
 typedef struct fxr_q8_stream {
-    const void* qc;          /* [>= *count, ld_qc] compact queries (fxr_gather_norm_rope_q8), 16-byte aligned */
+    const void* qc;          /* [max_rows, ld_qc] compact queries (fxr_gather_norm_rope_q8), 16-byte aligned */
     int64_t ld_qc;           /* elements, a multiple of 8 */
     const int32_t* idx;
     const int32_t* count;

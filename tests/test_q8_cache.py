@@ -135,14 +135,14 @@ def filled_cache(g, cfg, rows, fmt, pad=0, extra_scale=0):
     return fxr.CacheQ8(made[0][0], made[1][0], made[0][1], made[1][1])
 
 
-def stream_of(g, cfg, m, cap=None, ld_extra=0, out_extra=0, idx=None):
-    """A stream's queries, list, count and output, the output filled with 7 (rows behind stay so)."""
+def stream_of(g, cfg, m, ld_extra=0, out_extra=0, idx=None):
+    """A stream's queries (NaN behind the live rows), list, count and output, the output filled with 7 (rows
+    that are not listed stay so)."""
     t, h, n = TDT[cfg.dtype], cfg.n_heads, cfg.n_tokens
-    rows = max(m, 1) if cap is None else cap
-    q = randn(g, rows, h, D)
-    q = (q / q.square().mean(-1, keepdim=True).sqrt()).view(rows, h * D).to(t)
-    store = torch.full((rows, h * D + ld_extra), math.nan, dtype=t, device="cuda")
-    store[:, :h * D] = q
+    q = randn(g, m, h, D)
+    q = (q / q.square().mean(-1, keepdim=True).sqrt()).view(m, h * D).to(t) if m else q.view(0, h * D).to(t)
+    store = torch.full((n, h * D + ld_extra), math.nan, dtype=t, device="cuda")
+    store[:m, :h * D] = q
     if idx is None:
         idx = torch.randperm(n, generator=g, device="cuda")[:m].sort().values.int()
     out = torch.full((n, h * D + out_extra), 7.0, dtype=t, device="cuda")
@@ -288,6 +288,10 @@ def test_binding_refuses_other_types():
     k = torch.zeros(16, 256, dtype=torch.int8)
     s = torch.zeros(2, 16, dtype=torch.bfloat16)
     fxr.CacheQ8(k, k.clone(), s, s.clone())
+    few = fxr.q8_streams([{"qc": torch.zeros(3, 256, dtype=torch.bfloat16), "idx": k, "count": k, "out": k,
+                           "cache": fxr.CacheQ8(k, k, s, s)}])
+    with pytest.raises(fxr.FxrError, match="qc holds 3 rows"):
+        few.check(cfg_of(16, 2, "bf16"), 4)
     for bad in ((k.float(), k, s, s), (k, k.view(torch.float8_e4m3fn), s, s), (k, k, s.float(), s.float()), (k, k, s, s.half()),
                 (k, k[:8], s, s), (k, k, s[:, :8], s[:, :8]), (k[:, :128], k[:, :128], s, s), (k.t(), k.t(), s, s)):
         with pytest.raises(fxr.FxrError):
