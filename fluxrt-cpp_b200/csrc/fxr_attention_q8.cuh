@@ -91,6 +91,9 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
     uint32_t v;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -765,6 +768,9 @@ __global__ void __launch_bounds__(kVisThreads) visible_steps_kernel(const __grid
         : "r"(taddr), "r"((taddr) + 32u), "r"((taddr) + 64u), "r"((taddr) + 96u)                                      \
         : "memory")
 
+// Orders this thread's shared-memory writes before the asynchronous proxy's reads of them.
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 // ---- pieces of the tile kernel --------------------------------------------------------------------
 // Maximum that is NaN where an operand is (a NaN score must reach its row).
 __device__ __forceinline__ float max3n(float a, float b, float c) {
@@ -957,20 +963,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
             const T* pre_k = static_cast<const T*>(p.prefix.ks) + (int64_t)it->head * p.prefix.ld_scale;
             const T* pre_v = static_cast<const T*>(p.prefix.vs) + (int64_t)it->head * p.prefix.ld_scale;
             uint32_t word, next_word = list ? list[s0] : (uint32_t)s0;
-            float sk, sv, next_k, next_v;
-            auto scales = [&](uint32_t w, float& k_, float& v_) {
+            // the next step's scales are on their way, as bits, while this step is converted
+            uint16_t next_k, next_v;
+            auto scales = [&](uint32_t w, uint16_t& k_, uint16_t& v_) {
                 const int32_t tile = (int32_t)(list ? w & 0x7fffu : w);
                 const bool pre = tile < a.n_pre;
                 const int32_t key = (pre ? tile : tile - a.n_pre) * kBN + (int32_t)r;
                 const bool in_src = key < (pre ? p.n_prefix : p.n_tokens);
-                k_ = in_src ? StoreT<T>::to_f((pre ? pre_k : own_k)[key]) : 0.f;
-                v_ = in_src ? StoreT<T>::to_f((pre ? pre_v : own_v)[key]) : 0.f;
+                k_ = v_ = 0;
+                if (in_src) {
+                    k_ = __ldg(reinterpret_cast<const uint16_t*>(pre ? pre_k : own_k) + key);
+                    v_ = __ldg(reinterpret_cast<const uint16_t*>(pre ? pre_v : own_v) + key);
+                }
             };
             scales(next_word, next_k, next_v);
             for (int32_t j = 0; ok && j < n; ++j, ++step) {
                 word = next_word;
-                sk = next_k;
-                sv = next_v;
+                float sk = StoreT<T>::unpack2(next_k).x, sv = StoreT<T>::unpack2(next_v).x;
                 if (j + 1 < n) {
                     next_word = list ? list[s0 + j + 1] : (uint32_t)(s0 + j + 1);
                     scales(next_word, next_k, next_v);
@@ -982,7 +991,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                 for (int kv = 0; kv < 2; ++kv, ++in) {
                     const uint32_t rs = in % kRaws, ts = in % kTiles;
                     if (!wwait(bar(kRawFull + rs), (in / kRaws) & 1)) { ok = false; break; }
-                    if (in >= kTiles && !wwait(bar(kEmpty + ts), (in / kTiles - 1) & 1)) { ok = false; break; }
                     const uint32_t src = base + kSmRaw + rs * kSpan + r * 128;
                     const uint32_t dst = base + kSmTiles + ts * kTile + r * 128;
                     const uint32_t s2 = q8::scale_pair<T, F>(kv == 0 ? sk : sv);
@@ -992,23 +1000,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                         const int32_t left = pre ? p.n_prefix - tile * kBN : p.n_tokens - (tile - a.n_pre) * kBN;
                         info[step & 3] = (uint32_t)tile | ((uint32_t)min(left, kBN) << 16) | (list && (word & 0x8000u) ? kMixed : 0u);
                     }
+                    uint4 q[8];
+#pragma unroll
+                    for (uint32_t c = 0; c < 8; ++c) q[c] = lds128(src + ((c ^ x) << 4));
+                    if (in >= kTiles && !wwait(bar(kEmpty + ts), (in / kTiles - 1) & 1)) { ok = false; break; }
 #pragma unroll
                     for (uint32_t c = 0; c < 8; ++c) {
-                        const uint4 q = lds128(src + ((c ^ x) << 4));
                         uint4 lo, hi;
-                        q8::decode16<T, F>(q, s2, lo, hi);
+                        q8::decode16<T, F>(q[c], s2, lo, hi);
+                        if (c == 7) {            // the codes are in registers: their buffer is free
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(bar(kRawEmpty + rs));
+                        }
                         const uint32_t d = dst + (c >> 2) * kSpan;
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d + (((2 * (c & 3)) ^ x) << 4)), "r"(lo.x),
-                                     "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(d + (((2 * (c & 3) + 1) ^ x) << 4)), "r"(hi.x),
-                                     "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+                        sts128(d + (((2 * (c & 3)) ^ x) << 4), lo);
+                        sts128(d + (((2 * (c & 3) + 1) ^ x) << 4), hi);
                     }
-                    fence_proxy_async();     // the tensor core reads the tile through the async proxy
+                    fence_async_smem();      // the tensor core reads the tile through the async proxy
                     __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(bar(kFull + ts));
-                        mbar_arrive(bar(kRawEmpty + rs));
-                    }
+                    if (lane == 0) mbar_arrive(bar(kFull + ts));
                 }
             }
             __syncwarp();
