@@ -993,7 +993,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                     if (!wwait(bar(kRawFull + rs), (in / kRaws) & 1)) { ok = false; break; }
                     const uint32_t src = base + kSmRaw + rs * kSpan + r * 128;
                     const uint32_t dst = base + kSmTiles + ts * kTile + r * 128;
-                    const uint32_t s2 = q8::scale_pair<T, F>(kv == 0 ? sk : sv);
+                    const float f = kv == 0 ? sk : sv;
+                    q8::Decoder<T, F> dec;
+                    dec.scale(StoreT<T>::pack2(f, f));
                     if (kv == 0 && r == 0) {
                         const int32_t tile = (int32_t)(list ? word & 0x7fffu : word);
                         const bool pre = tile < a.n_pre;
@@ -1007,7 +1009,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
 #pragma unroll
                     for (uint32_t c = 0; c < 8; ++c) {
                         uint4 lo, hi;
-                        q8::decode16<T, F>(q[c], s2, lo, hi);
+                        q8::decode16<T, F>(q[c], dec, lo, hi);
                         if (c == 7) {            // the codes are in registers: their buffer is free
                             __syncwarp();
                             if (lane == 0) mbar_arrive(bar(kRawEmpty + rs));

@@ -43,19 +43,18 @@ template <> __device__ __forceinline__ float scale_up<__nv_bfloat16>(float t) {
 }
 template <> __device__ __forceinline__ float scale_up<__half>(float t) { return __half2float(__float2half_ru(t)); }
 
+// (largest T) / 128 or / 448, rounded down to T.
+template <typename T, int F> __device__ __forceinline__ constexpr float scale_cap() {
+    constexpr bool bf16 = StoreT<T>::kUmmaFormat == 1;
+    return F == kInt8 ? (bf16 ? 0x1.fep+120f : 511.75f) : (bf16 ? 0x1.22p+119f : 146.125f);
+}
+
 // Scale of a head vector whose largest magnitude has the bits `amax` (NaN and infinities compare
 // above every finite value).
 template <typename T, int F>
 __device__ __forceinline__ float scale_of(uint32_t amax) {
     if (amax >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-    const float t = __fdiv_rn(__uint_as_float(amax), top_code<F>());
-    float s = scale_up<T>(t);
-    if (sizeof(T) == 2 && StoreT<T>::kUmmaFormat == 0) {   // f16
-        if (s > 65504.f) return __uint_as_float(0x7fc00000u);   // no f16 scale holds this vector
-        if (s * top_code<F>() > 65504.f && __uint_as_float(amax) <= 65504.f)
-            s = __half2float(__float2half_rd(t));
-    }
-    return s;
+    return fminf(scale_up<T>(__fdiv_rn(__uint_as_float(amax), top_code<F>())), scale_cap<T, F>());
 }
 
 // Codes of 8 values as 8 bytes. s = 0 or NaN: codes 0.
@@ -84,15 +83,76 @@ __device__ __forceinline__ uint2 encode8(const float* x, float s) {
     return make_uint2(w[0], w[1]);
 }
 
-// Byte a of wa and byte b of wb as a packed pair of T, exact up to the factor 1 / code_scale():
-//   int8 -> bf16: 0x4300 | low 7 bits is 128 + low7, 0x4300 | sign bit is 128 or 256; the difference
-//                 is the two's complement value (bf16 holds 8 significant bits, so both are exact)
-//   int8 -> f16:  0x6400 | (x ^ 0x80) is 1024 + 128 + x
-//   e4m3 -> f16:  sign, exponent and mantissa fields moved into place: the value times 2^-8,
-//                 subnormals included
-//   e4m3 -> bf16: the same gives the value times 2^-120, multiplied back (bf16 products keep
-//                 subnormal operands)
+__device__ __forceinline__ __nv_bfloat162 as_bf(uint32_t u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); }
+__device__ __forceinline__ __half2 as_h(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+__device__ __forceinline__ uint32_t bits(const __nv_bfloat162& x) { return *reinterpret_cast<const uint32_t*>(&x); }
+__device__ __forceinline__ uint32_t bits(const __half2& x) { return *reinterpret_cast<const uint32_t*>(&x); }
+template <typename T> __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t mul2<__nv_bfloat16>(uint32_t a, uint32_t b) { return bits(__hmul2(as_bf(a), as_bf(b))); }
+template <> __device__ __forceinline__ uint32_t mul2<__half>(uint32_t a, uint32_t b) { return bits(__hmul2(as_h(a), as_h(b))); }
+
+// Codes -> T(code * s), pairs of T at a time. What bounds a decoder is the integer pipe, which runs at
+// half the rate of the FMA pipe (the attention's converters share both with the softmax warps), so as
+// much as can be is left to packed 16-bit arithmetic:
+//   int8 -> bf16: a permute puts byte x ^ 0x80 under the constant 0x42, the bf16 number a = 64 + x / 2
+//     for x >= 0 and 64 + x / 4 for x < 0. Then t = 2 s a - 128 s (one fma, one rounding) is s x for
+//     x >= 0 and s x / 2 otherwise, and t - max(0, -t) is s x for both: rounding commutes with the
+//     factor 2, so the result is the one rounding of s x.
+//   int8 -> f16:  0x6400 | (x ^ 0x80) is 1024 + 128 + x, exactly: subtract, multiply.
+//   e4m3 -> f16:  sign, exponent and mantissa fields moved into place give the value times 2^-8 (also
+//     where it is subnormal); the scale's multiplier holds the 2^8.
+//   e4m3 -> bf16: the same gives the value times 2^-120; products of bf16 keep subnormal operands, so
+//     a multiplication by 2^120 restores it.
 // The e4m3 NaN codes, which the write never produces, are not told apart from +-480.
+template <typename T, int F> struct Decoder;
+
+// word(): prepares four codes, once; pair(): two of them as values.
+template <> struct Decoder<__nv_bfloat16, kInt8> {
+    __nv_bfloat162 two, up, mtwo, down;      // 2 s, -128 s, -2 s, 128 s
+    __device__ __forceinline__ void scale(uint32_t s2) {
+        const __nv_bfloat162 s = as_bf(s2);
+        two = __hmul2(s, as_bf(0x40004000u));
+        mtwo = __hmul2(s, as_bf(0xc000c000u));
+        down = __hmul2(s, as_bf(0x43004300u));
+        up = __hmul2(s, as_bf(0xc300c300u));
+    }
+    static __device__ __forceinline__ uint32_t word(uint32_t w) { return w ^ 0x80808080u; }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int a, int b) const {
+        const uint32_t u = __byte_perm(w, 0x42424242u, (uint32_t)(a | 0x40 | (b << 8) | 0x4000));
+        const __nv_bfloat162 t = __hfma2(as_bf(u), two, up), n = __hfma2_relu(as_bf(u), mtwo, down);
+        return bits(__hsub2(t, n));
+    }
+};
+template <> struct Decoder<__half, kInt8> {
+    __half2 s;
+    __device__ __forceinline__ void scale(uint32_t s2) { s = as_h(s2); }
+    static __device__ __forceinline__ uint32_t word(uint32_t w) { return w ^ 0x80808080u; }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int a, int b) const {
+        const uint32_t u = __byte_perm(w, 0x64646464u, (uint32_t)(a | 0x40 | (b << 8) | 0x4000));
+        return bits(__hmul2(__hsub2(as_h(u), as_h(0x64806480u)), s));
+    }
+};
+template <> struct Decoder<__half, kE4m3> {
+    __half2 s;
+    __device__ __forceinline__ void scale(uint32_t s2) { s = __hmul2(as_h(s2), as_h(0x5c005c00u)); }   // * 2^8: s <= 146.125
+    static __device__ __forceinline__ uint32_t word(uint32_t w) { return w; }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int a, int b) const {
+        const uint32_t u = __byte_perm(w, 0u, (uint32_t)(4 | (a << 4) | 0x400 | (b << 12)));
+        return bits(__hmul2(as_h(((u >> 1) & 0x3f803f80u) | (u & 0x80008000u)), s));
+    }
+};
+template <> struct Decoder<__nv_bfloat16, kE4m3> {
+    __nv_bfloat162 s;
+    __device__ __forceinline__ void scale(uint32_t s2) { s = as_bf(s2); }
+    static __device__ __forceinline__ uint32_t word(uint32_t w) { return w; }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int a, int b) const {
+        const uint32_t u = __byte_perm(w, 0u, (uint32_t)(4 | (a << 4) | 0x400 | (b << 12)));
+        const uint32_t v = ((u >> 4) & 0x07f007f0u) | (u & 0x80008000u);
+        return bits(__hmul2(__hmul2(as_bf(v), as_bf(0x7b807b80u)), s));
+    }
+};
+
+// Byte a of wa and byte b of wb, codes alone: exact up to the factor 1 / code_scale().
 template <typename T, int F> __device__ __forceinline__ constexpr float code_scale() {
     return (F == kE4m3 && StoreT<T>::kUmmaFormat == 0) ? 256.f : 1.f;
 }
@@ -100,54 +160,27 @@ template <typename T, int F>
 __device__ __forceinline__ uint32_t decode2(uint32_t wa, uint32_t wb, int a, int b) {
     if constexpr (F == kInt8) {
         const uint32_t u = __byte_perm(wa, wb, (uint32_t)(a | ((4 + b) << 8)));
-        if constexpr (StoreT<T>::kUmmaFormat == 1) {
-            const uint32_t p = (u & 0x007f007fu) | 0x43004300u, n = (u & 0x00800080u) | 0x43004300u;
-            const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&p),
-                                             *reinterpret_cast<const __nv_bfloat162*>(&n));
-            return *reinterpret_cast<const uint32_t*>(&r);
-        } else {
-            const uint32_t p = (u & 0x00ff00ffu) ^ 0x64806480u, n = 0x64806480u;
-            const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&p), *reinterpret_cast<const __half2*>(&n));
-            return *reinterpret_cast<const uint32_t*>(&r);
-        }
+        if constexpr (StoreT<T>::kUmmaFormat == 1)
+            // 0x4300 | low 7 bits is 128 + low7, 0x4300 | sign bit is 128 or 256
+            return bits(__hsub2(as_bf((u & 0x007f007fu) | 0x43004300u), as_bf((u & 0x00800080u) | 0x43004300u)));
+        else
+            return bits(__hsub2(as_h((u & 0x00ff00ffu) ^ 0x64806480u), as_h(0x64806480u)));
     } else {
         const uint32_t u = __byte_perm(wa, wb, (uint32_t)((a << 4) | ((4 + b) << 12)));
-        if constexpr (StoreT<T>::kUmmaFormat == 1) {
-            const uint32_t p = ((u >> 4) & 0x07f007f0u) | (u & 0x80008000u), c = 0x7b807b80u;
-            const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&p),
-                                             *reinterpret_cast<const __nv_bfloat162*>(&c));
-            return *reinterpret_cast<const uint32_t*>(&r);
-        } else {
+        if constexpr (StoreT<T>::kUmmaFormat == 1)
+            return mul2<T>(((u >> 4) & 0x07f007f0u) | (u & 0x80008000u), 0x7b807b80u);
+        else
             return ((u >> 1) & 0x3f803f80u) | (u & 0x80008000u);
-        }
     }
-}
-
-template <typename T> __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b);
-template <> __device__ __forceinline__ uint32_t mul2<__nv_bfloat16>(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-template <> __device__ __forceinline__ uint32_t mul2<__half>(uint32_t a, uint32_t b) {
-    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// The scale as the multiplier of decode2's pairs, twice in a register. Exact: a code_scale of 256
-// belongs to f16 scales of at most 146.25.
-template <typename T, int F>
-__device__ __forceinline__ uint32_t scale_pair(float s) {
-    s *= code_scale<T, F>();
-    return StoreT<T>::pack2(s, s);
 }
 
 // 16 codes -> 16 values of T in two 16-byte vectors (lo: codes 0-7, hi: 8-15).
 template <typename T, int F>
-__device__ __forceinline__ void decode16(const uint4& c, uint32_t s2, uint4& lo, uint4& hi) {
-    lo = make_uint4(mul2<T>(decode2<T, F>(c.x, c.x, 0, 1), s2), mul2<T>(decode2<T, F>(c.x, c.x, 2, 3), s2),
-                    mul2<T>(decode2<T, F>(c.y, c.y, 0, 1), s2), mul2<T>(decode2<T, F>(c.y, c.y, 2, 3), s2));
-    hi = make_uint4(mul2<T>(decode2<T, F>(c.z, c.z, 0, 1), s2), mul2<T>(decode2<T, F>(c.z, c.z, 2, 3), s2),
-                    mul2<T>(decode2<T, F>(c.w, c.w, 0, 1), s2), mul2<T>(decode2<T, F>(c.w, c.w, 2, 3), s2));
+__device__ __forceinline__ void decode16(const uint4& c, const Decoder<T, F>& d, uint4& lo, uint4& hi) {
+    using De = Decoder<T, F>;
+    const uint32_t x = De::word(c.x), y = De::word(c.y), z = De::word(c.z), w = De::word(c.w);
+    lo = make_uint4(d.pair(x, 0, 1), d.pair(x, 2, 3), d.pair(y, 0, 1), d.pair(y, 2, 3));
+    hi = make_uint4(d.pair(z, 0, 1), d.pair(z, 2, 3), d.pair(w, 0, 1), d.pair(w, 2, 3));
 }
 
 // ---- write --------------------------------------------------------------------------------------
@@ -367,14 +400,15 @@ __global__ void __launch_bounds__(kReadThreads) q8_read_kernel(const __grid_cons
         const int64_t dst = (int64_t)m * a.ld + c * 16;
         const uint4 ck = __ldcs(reinterpret_cast<const uint4*>(a.c.k + src));
         const uint4 cv = __ldcs(reinterpret_cast<const uint4*>(a.c.v + src));
-        const uint32_t sk = scale_pair<T, F>(StoreT<T>::to_f(static_cast<const T*>(a.c.ks)[at]));
-        const uint32_t sv = scale_pair<T, F>(StoreT<T>::to_f(static_cast<const T*>(a.c.vs)[at]));
+        Decoder<T, F> dk, dv;
+        dk.scale(0x10001u * static_cast<const uint16_t*>(a.c.ks)[at]);
+        dv.scale(0x10001u * static_cast<const uint16_t*>(a.c.vs)[at]);
         uint4 lo, hi;
-        decode16<T, F>(ck, sk, lo, hi);
+        decode16<T, F>(ck, dk, lo, hi);
         uint4* ko = reinterpret_cast<uint4*>(static_cast<T*>(a.k) + dst);
         __stcs(ko, lo);
         __stcs(ko + 1, hi);
-        decode16<T, F>(cv, sv, lo, hi);
+        decode16<T, F>(cv, dv, lo, hi);
         uint4* vo = reinterpret_cast<uint4*>(static_cast<T*>(a.v) + dst);
         __stcs(vo, lo);
         __stcs(vo + 1, hi);

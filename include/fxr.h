@@ -630,10 +630,10 @@ int32_t fxr_frame_forward_heads_nccl(const fxr_frame_desc* desc, const fxr_head_
  *   scale = max|x| / Q rounded up to T, Q = 127 (FXR_Q8_INT8) or 448 (FXR_Q8_E4M3)
  *   code  = x / scale rounded to nearest even: a whole number in [-127, 127], or e4m3 (saturating)
  *   read  = code * scale, rounded once to T
- * A vector of zeros has scale 0. One that holds an infinity or NaN (or whose scale T cannot hold) has
+ * A vector of zeros has scale 0. One that holds an infinity or NaN has
  * scale NaN and codes 0: it reads back as NaN, and an attention row that sees it is NaN. K' is
- * quantised from its 32-bit value. (f16: the scale is rounded down where Q * scale would pass the
- * largest f16 value, so that every finite vector reads back finite.) */
+ * quantised from its 32-bit value. A scale is at most (largest T) / 128 for int8 and (largest T) / 448
+ * for e4m3, so that every finite vector reads back finite; codes saturate there. */
 typedef enum fxr_q8_format { FXR_Q8_INT8 = 0, FXR_Q8_E4M3 = 1 } fxr_q8_format;
 
 typedef struct fxr_q8_cache {

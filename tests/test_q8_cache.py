@@ -42,9 +42,10 @@ def quantise(x, fmt, dtype):
     x = torch.where(bad[..., None], torch.zeros_like(x), x)
     t = x.abs().amax(-1) / TOP[fmt]
     s = up_to(t, dtype)
-    if dtype == torch.float16:
-        over = s * TOP[fmt] > 65504
-        s = torch.where(over, torch.floor(t / 2.0 ** -3) * 2.0 ** -3 if fmt == "e4m3" else torch.floor(t * 2) / 2, s)
+    cap = torch.finfo(dtype).max / (128 if fmt == "int8" else 448)      # of the type itself for int8
+    if fmt == "e4m3":
+        cap = 146.125 if dtype == torch.float16 else math.floor(cap / 2.0 ** 112) * 2.0 ** 112
+    s = torch.clamp(s, max=cap)
     y = x / torch.where(s > 0, s, torch.ones_like(s))[..., None]
     if fmt == "int8":
         y = torch.clamp(torch.round(y), -127, 127)
