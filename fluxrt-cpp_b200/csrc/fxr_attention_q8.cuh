@@ -950,6 +950,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
         // ---------------- converters: one row of the tile per thread ----------------
         auto wwait = [&](uint32_t b_, uint32_t par_) -> bool { return __all_sync(0xffffffffu, mbar_wait(b_, par_, abort)); };
         const uint32_t r = (uint32_t)(warp - kConvWarp) * 32 + lane, x = r & 7;
+        constexpr uint32_t fmt16 = StoreT<T>::kUmmaFormat;
         uint32_t in = 0, step = 0;     // tiles converted, steps
         bool ok = true;
         for (uint32_t k = 0; ok; ++k) {
@@ -994,8 +995,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                     const uint32_t src = base + kSmRaw + rs * kSpan + r * 128;
                     const uint32_t dst = base + kSmTiles + ts * kTile + r * 128;
                     const float f = kv == 0 ? sk : sv;
-                    q8::Decoder<T, F> dec;
-                    dec.scale(StoreT<T>::pack2(f, f));
                     if (kv == 0 && r == 0) {
                         const int32_t tile = (int32_t)(list ? word & 0x7fffu : word);
                         const bool pre = tile < a.n_pre;
@@ -1006,17 +1005,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
 #pragma unroll
                     for (uint32_t c = 0; c < 8; ++c) q[c] = lds128(src + ((c ^ x) << 4));
                     if (in >= kTiles && !wwait(bar(kEmpty + ts), (in / kTiles - 1) & 1)) { ok = false; break; }
+                    auto convert = [&](auto dec) {
+                        dec.scale(StoreT<T>::pack2(f, f));
 #pragma unroll
-                    for (uint32_t c = 0; c < 8; ++c) {
-                        uint4 lo, hi;
-                        q8::decode16<T, F>(q[c], dec, lo, hi);
-                        if (c == 7) {            // the codes are in registers: their buffer is free
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(bar(kRawEmpty + rs));
+                        for (uint32_t c = 0; c < 8; ++c) {
+                            uint4 lo, hi;
+                            q8::decode16(q[c], dec, lo, hi);
+                            if (c == 7) {        // the codes are in registers: their buffer is free
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(bar(kRawEmpty + rs));
+                            }
+                            const uint32_t d = dst + (c >> 2) * kSpan;
+                            sts128(d + (((2 * (c & 3)) ^ x) << 4), lo);
+                            sts128(d + (((2 * (c & 3) + 1) ^ x) << 4), hi);
                         }
-                        const uint32_t d = dst + (c >> 2) * kSpan;
-                        sts128(d + (((2 * (c & 3)) ^ x) << 4), lo);
-                        sts128(d + (((2 * (c & 3) + 1) ^ x) << 4), hi);
+                    };
+                    if constexpr (F == q8::kE4m3 && fmt16 == 1) {
+                        if (__all_sync(0xffffffffu, !(f >= q8::kSmallScale))) convert(q8::SmallScaleDecoder{});
+                        else convert(q8::Decoder<T, F>{});
+                    } else {
+                        convert(q8::Decoder<T, F>{});
                     }
                     fence_async_smem();      // the tensor core reads the tile through the async proxy
                     __syncwarp();

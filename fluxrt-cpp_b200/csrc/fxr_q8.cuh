@@ -100,9 +100,11 @@ template <> __device__ __forceinline__ uint32_t mul2<__half>(uint32_t a, uint32_
 //     factor 2, so the result is the one rounding of s x.
 //   int8 -> f16:  0x6400 | (x ^ 0x80) is 1024 + 128 + x, exactly: subtract, multiply.
 //   e4m3 -> f16:  sign, exponent and mantissa fields moved into place give the value times 2^-8 (also
-//     where it is subnormal); the scale's multiplier holds the 2^8.
+//     where it is subnormal); the scale's multiplier holds the 2^8. The permute doubles the byte, so
+//     that the sign is in place already and the rest a left shift away, which the FMA pipe does.
 //   e4m3 -> bf16: the same gives the value times 2^-120; products of bf16 keep subnormal operands, so
-//     a multiplication by 2^120 restores it.
+//     a multiplication by 2^120 restores it. Where s < 2^7, as for every vector of magnitude below
+//     57344, the scale's multiplier holds the 2^120 (SmallScaleDecoder).
 // The e4m3 NaN codes, which the write never produces, are not told apart from +-480.
 template <typename T, int F> struct Decoder;
 
@@ -137,21 +139,32 @@ template <> struct Decoder<__half, kE4m3> {
     __device__ __forceinline__ void scale(uint32_t s2) { s = __hmul2(as_h(s2), as_h(0x5c005c00u)); }   // * 2^8: s <= 146.125
     static __device__ __forceinline__ uint32_t word(uint32_t w) { return w; }
     __device__ __forceinline__ uint32_t pair(uint32_t w, int a, int b) const {
-        const uint32_t u = __byte_perm(w, 0u, (uint32_t)(4 | (a << 4) | 0x400 | (b << 12)));
-        return bits(__hmul2(as_h(((u >> 1) & 0x3f803f80u) | (u & 0x80008000u)), s));
+        const uint32_t u = __byte_perm(w, 0u, (uint32_t)(a | (a << 4) | (b << 8) | (b << 12)));
+        return bits(__hmul2(as_h(((u << 7) & 0x3f803f80u) | (u & 0x80008000u)), s));
     }
 };
 template <> struct Decoder<__nv_bfloat16, kE4m3> {
     __nv_bfloat162 s;
     __device__ __forceinline__ void scale(uint32_t s2) { s = as_bf(s2); }
     static __device__ __forceinline__ uint32_t word(uint32_t w) { return w; }
+    static __device__ __forceinline__ uint32_t fields(uint32_t w, int a, int b) {
+        const uint32_t u = __byte_perm(w, 0u, (uint32_t)(a | (a << 4) | (b << 8) | (b << 12)));
+        return ((u << 4) & 0x07f007f0u) | (u & 0x80008000u);
+    }
     __device__ __forceinline__ uint32_t pair(uint32_t w, int a, int b) const {
-        const uint32_t u = __byte_perm(w, 0u, (uint32_t)(4 | (a << 4) | 0x400 | (b << 12)));
-        const uint32_t v = ((u >> 4) & 0x07f007f0u) | (u & 0x80008000u);
-        return bits(__hmul2(__hmul2(as_bf(v), as_bf(0x7b807b80u)), s));
+        return bits(__hmul2(__hmul2(as_bf(fields(w, a, b)), as_bf(0x7b807b80u)), s));
     }
 };
-
+// e4m3 -> bf16 for scales below kSmallScale (or NaN): one multiplication.
+constexpr float kSmallScale = 128.f;
+struct SmallScaleDecoder {
+    __nv_bfloat162 s;
+    __device__ __forceinline__ void scale(uint32_t s2) { s = __hmul2(as_bf(s2), as_bf(0x7b807b80u)); }
+    static __device__ __forceinline__ uint32_t word(uint32_t w) { return w; }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int a, int b) const {
+        return bits(__hmul2(as_bf(Decoder<__nv_bfloat16, kE4m3>::fields(w, a, b)), s));
+    }
+};
 // Byte a of wa and byte b of wb, codes alone: exact up to the factor 1 / code_scale().
 template <typename T, int F> __device__ __forceinline__ constexpr float code_scale() {
     return (F == kE4m3 && StoreT<T>::kUmmaFormat == 0) ? 256.f : 1.f;
@@ -175,9 +188,8 @@ __device__ __forceinline__ uint32_t decode2(uint32_t wa, uint32_t wb, int a, int
 }
 
 // 16 codes -> 16 values of T in two 16-byte vectors (lo: codes 0-7, hi: 8-15).
-template <typename T, int F>
-__device__ __forceinline__ void decode16(const uint4& c, const Decoder<T, F>& d, uint4& lo, uint4& hi) {
-    using De = Decoder<T, F>;
+template <typename De>
+__device__ __forceinline__ void decode16(const uint4& c, const De& d, uint4& lo, uint4& hi) {
     const uint32_t x = De::word(c.x), y = De::word(c.y), z = De::word(c.z), w = De::word(c.w);
     lo = make_uint4(d.pair(x, 0, 1), d.pair(x, 2, 3), d.pair(y, 0, 1), d.pair(y, 2, 3));
     hi = make_uint4(d.pair(z, 0, 1), d.pair(z, 2, 3), d.pair(w, 0, 1), d.pair(w, 2, 3));
@@ -404,11 +416,11 @@ __global__ void __launch_bounds__(kReadThreads) q8_read_kernel(const __grid_cons
         dk.scale(0x10001u * static_cast<const uint16_t*>(a.c.ks)[at]);
         dv.scale(0x10001u * static_cast<const uint16_t*>(a.c.vs)[at]);
         uint4 lo, hi;
-        decode16<T, F>(ck, dk, lo, hi);
+        decode16(ck, dk, lo, hi);
         uint4* ko = reinterpret_cast<uint4*>(static_cast<T*>(a.k) + dst);
         __stcs(ko, lo);
         __stcs(ko + 1, hi);
-        decode16<T, F>(cv, dv, lo, hi);
+        decode16(cv, dv, lo, hi);
         uint4* vo = reinterpret_cast<uint4*>(static_cast<T*>(a.v) + dst);
         __stcs(vo, lo);
         __stcs(vo + 1, hi);
