@@ -4,7 +4,7 @@
 // over the rows of a prefix that every stream of the launch shares and then the stream's own rows;
 // allow(m, j) = (q_groups[idx[m]] & k_groups[j]) != 0. A row that sees no key gives zeros.
 //
-// A key whose K or V scale is not finite (its 16-bit row held an infinity or NaN) makes the rows that
+// A key whose K or V scale is not valid (its 16-bit row held an infinity or NaN) makes the rows that
 // see it NaN and no others: its score is set to NaN before the mask and its V codes count as zeros.
 #pragma once
 
@@ -40,52 +40,55 @@ struct Params {
 };
 
 // ---------------------------------------------------------------------------------------------
-// Few rows per stream: bound by reading the cache once. One CTA per SM takes items of (16 rows, head,
-// key range); its 8 warps walk the range in blocks of 32 keys, each with its own running maximum,
-// sum and O, so that no warp waits for another inside the loop. A warp streams its blocks through a
-// ring of 3 in shared memory with 16-byte asynchronous copies (8 KB of codes per block: ~190 KB in
-// flight per SM). The codes become 16-bit operands in registers, on their way from shared memory to
-// mma.m16n8k16 (tcgen05 reads operands from memory and wants 128 rows; these calls have a few):
-//   S = Q K^T: a lane's B operand of a 16-dim step is 4 codes of one key. The order of the 128 dims
-//     inside a dot product is free, so the lane takes 16 consecutive bytes for four steps, and Q's
-//     fragments are loaded in the same order.
-//   O += P V: the operand pairs two keys of one dim: one byte permute takes both codes. A lane's 16
-//     column tiles are 16 consecutive dims (dim = 16 * column + tile).
+// Few rows per stream: bound by reading the cache once. Work is laid on a line of columns, each the
+// keys of one source for one head and one group of 8 or 16 rows: first (head, group of the packed rows
+// of all streams) against the prefix, so that the prefix is read once for every 16 rows of all
+// streams, then (stream, head, group) against the stream's own rows. The line is cut into one range
+// per CTA in units of 64 keys; a range covers one to a few items (parts of columns).
+// A CTA's 16 warps walk an item in blocks of 16 keys, each warp with its own running maximum, sum and
+// O, so that none waits for another. A warp streams its blocks through a ring of 3 in shared memory
+// by TMA (4 KB of codes per block: ~130 KB in flight per SM; one lane issues a block's copies, where
+// 16-byte asynchronous copies cost every lane eight addresses). The codes
+// become 16-bit operands in registers, between shared memory and mma.m16n8k16 with keys, then dims,
+// as its 16 rows and queries as its 8 columns (tcgen05 reads its operands from memory and wants 128
+// rows; these calls have a few):
+//   S^T = K Q^T: a lane holds codes of keys g and g + 8. The order of the 128 dims inside a dot
+//     product is free, so it takes 16 consecutive bytes for four steps of 16 dims, and reads Q's
+//     fragments in the same order.
+//   O^T += V^T P^T: an operand pairs two keys of one dim; one byte permute takes both codes. A lane's
+//     rows in the 8 row tiles are 16 consecutive dims. P^T changes from the accumulators' to the
+//     operand's layout by an 8 x 8 transpose (movmatrix).
 // K scales multiply the scores in 32 bits. A V scale is split into 2^e * f, f in [1, 2): f multiplies
 // P before its one rounding to T, 2^e the codes, exactly (all of the scale on P would push it into
 // f16's subnormals; all of it on V would cost a second rounding). bf16 P holds the whole product.
-// Rows of several streams share an MMA tile against the prefix (its codes are read once for every 16
-// of all streams' rows); own rows are per stream. The key range of an item is the shortest multiple
-// of 128 that gives every item a CTA at once, or whole sources when there are more (row, head)
-// groups than CTAs. Partial results (O, maximum, sum) meet in L2: the last item of a head to arrive
-// combines that head's rows in key order, so the result does not depend on the order of arrival.
+// Partial results (O, maximum, sum) meet in L2: the last of a row group's parts to arrive combines
+// them in key order, so the result does not depend on the order of arrival.
 // ---------------------------------------------------------------------------------------------
-constexpr int kRowsWarps = 8;
+constexpr int kRowsWarps = 16;
 constexpr int kRowsThreads = 32 * kRowsWarps;
-constexpr int kRowsTile = 16;
-constexpr int kBlk = 32;                       // keys per block
+constexpr int kRowsMax = 16;                   // rows of a group, at most
+constexpr int kBlk = 16;                       // keys per block
 constexpr int kDepth = 3;                      // ring
-constexpr int kChunkUnit = 128;                // key ranges are multiples of this
-constexpr uint32_t kBlkBytes = kBlk * 128;     // codes of one of K, V
-constexpr uint32_t kOffScale = 2 * kBlkBytes;  // K scales, V scales (kBlk x 2 bytes each), groups
-constexpr uint32_t kOffGroup = kOffScale + 2 * kBlk * 2;
-constexpr uint32_t kRingSlot = kOffGroup + kBlk * 4;
+constexpr int kUnitKeys = 64;                  // the line is cut at multiples of this
+constexpr int kMaxRowsPerStream = 64;          // what the launch accepts
+constexpr int kGroupsPerStream = kMaxRowsPerStream / 8;
+constexpr uint32_t kBlkBytes = kBlk * 128;     // codes of one of K, V (128-byte swizzle)
+constexpr uint32_t kRingSlot = 2 * kBlkBytes;
 constexpr uint32_t kRingWarp = kDepth * kRingSlot;
+constexpr uint32_t kScaleSlot = 2 * kBlk * 2;  // a block's K scales, V scales
 constexpr int kPadRow = 132;                   // floats per O row in the warps' exchange
-constexpr uint32_t kRowsSmem = kRowsWarps * kRingWarp + 2 * kRowsWarps * kRowsTile * 4;
-constexpr int kRowsSlotFloats = kRowsTile * kHeadDim + 2 * kRowsTile;
-static_assert(kRowsWarps * kRowsTile * kPadRow * 4 <= kRowsWarps * kRingWarp, "exchange fits the ring");
+constexpr uint32_t kQPad = 272;                // bytes per query row
+constexpr uint32_t kRowsSmemScale = kRowsWarps * kRingWarp;
+constexpr uint32_t kRowsSmemQ = kRowsSmemScale + kRowsWarps * kDepth * kScaleSlot;
+constexpr uint32_t kRowsSmemM = kRowsSmemQ + kRowsMax * kQPad;             // maxima, then sums: [16 rows][warps]
+constexpr uint32_t kRowsSmemBar = kRowsSmemM + 2 * kRowsWarps * kRowsMax * 4;
+constexpr uint32_t kRowsSmem = kRowsSmemBar + kRowsWarps * kDepth * 8 + 1024;   // + alignment slack
+constexpr int kRowsSlotFloats = kRowsMax * kHeadDim + 2 * kRowsMax;
+static_assert(kRowsWarps * kRowsMax * kPadRow * 4 <= kRowsWarps * kRingWarp, "exchange fits the ring");
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+// Orders this thread's shared-memory accesses before later ones of the asynchronous proxy.
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
@@ -94,452 +97,648 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
 __device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-    return v;
-}
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma16816<__nv_bfloat16>(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                         uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 template <>
 __device__ __forceinline__ void mma16816<__half>(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                                  uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8 x 8 matrix of 16-bit values over a warp, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
-__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+// Row g of an MMA's 8-row half holds key key_of(g) of the block, and a lane's 16 dims of V are chunk
+// key_of(g): in the 128-byte swizzle, neighbouring rows of the fragments then touch different banks.
+__device__ __forceinline__ int key_of(int g) { return ((g & 1) << 2) | (g >> 1); }
 
-// The launch's division into items, the same on every thread: a function of the counts.
-struct RowsPlan {
-    int32_t rows[kMaxBatch];     // of each stream
-    int32_t total;               // of all streams
-    int32_t gp;                  // 16-row groups of the packed rows (prefix items), 0 without a prefix
-    int32_t go;                  // of the streams' own items, all streams
-    int32_t len;                 // keys of an item
-    int32_t np, no;              // items per group: prefix, own
-    int32_t items;
+struct RowsMaps {
+    CUtensorMap k[kMaxBatch], v[kMaxBatch], pk, pv;
 };
 
-__device__ __forceinline__ RowsPlan rows_plan(const Params& p) {
-    RowsPlan r{};
+// The launch's division, a function of the counts; each CTA computes it into shared memory.
+struct RowsPlan {
+    int32_t rows[kMaxBatch];     // of each stream
+    int32_t first[kMaxBatch];    // its first packed row
+    int32_t group0[kMaxBatch];   // its first own group
+    int32_t total;               // rows of all streams
+    int32_t gp, go;              // groups: packed rows (0 without a prefix), own
+    int32_t up, uo;              // units of a prefix column, of an own column
+    int32_t per;                 // units per CTA
+    int32_t line;                // units in all (the host refuses calls of 2^31 or more)
+};
+
+// Column c of the line: its head, group and units; prefix columns first.
+struct Column {
+    int32_t head, group, stream, units, start;
+};
+
+template <int R>
+__device__ __forceinline__ Column column_at(const RowsPlan& r, int32_t n_heads, int32_t unit, int32_t& index) {
+    Column c;
+    const int32_t pre = n_heads * r.gp * r.up;
+    if (unit < pre) {
+        index = unit / r.up;
+        c.head = index / r.gp;
+        c.group = index - c.head * r.gp;
+        c.stream = -1;
+        c.units = r.up;
+        c.start = index * r.up;
+        return c;
+    }
+    int32_t e = (unit - pre) / r.uo;
+    index = n_heads * r.gp + e;
+    c.start = pre + e * r.uo;
+    c.units = r.uo;
+    c.stream = 0;
 #pragma unroll
-    for (int b = 0; b < kMaxBatch; ++b) {
-        r.rows[b] = 0;
-        if (b < p.n_streams) {
-            const int32_t c = *p.s[b].count;
-            r.rows[b] = max(0, min(c, p.max_rows));
-            if (c > p.max_rows && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(&g_error_word, kErrBounds);
+    for (int b = 0; b < kMaxBatch - 1; ++b) {
+        const int32_t n = n_heads * ((r.rows[b] + R - 1) / R);
+        if (c.stream == b && e >= n) {
+            e -= n;
+            c.stream = b + 1;
         }
-        r.total += r.rows[b];
-        r.go += (r.rows[b] + kRowsTile - 1) / kRowsTile;
     }
-    if (r.total == 0) return r;
-    r.gp = p.n_prefix > 0 ? (r.total + kRowsTile - 1) / kRowsTile : 0;
-    const int32_t groups = p.n_heads * (r.gp + r.go), grid = (int32_t)gridDim.x;
-    const int32_t target = (groups + grid - 1) / grid * grid;
-    const int32_t longest = max(p.n_prefix, p.n_tokens);
-    const int64_t keys = (int64_t)p.n_heads * ((int64_t)r.gp * p.n_prefix + (int64_t)r.go * p.n_tokens);
-    r.len = max(1, (int32_t)(keys / ((int64_t)target * kChunkUnit))) * kChunkUnit;
-    for (;;) {
-        r.np = (p.n_prefix + r.len - 1) / r.len;
-        r.no = (p.n_tokens + r.len - 1) / r.len;
-        r.items = p.n_heads * (r.gp * r.np + r.go * r.no);
-        if (r.items <= target || r.len >= longest) break;
-        r.len += kChunkUnit;
-    }
-    return r;
+    const int32_t groups = (r.rows[c.stream] + R - 1) / R;
+    c.head = e / groups;
+    c.group = e - c.head * groups;
+    return c;
 }
 
-// Packed row pr -> stream and compact row.
-__device__ __forceinline__ void unpack_row(const Params& p, const RowsPlan& r, int32_t pr, int32_t& b, int32_t& m) {
-    b = -1;
-    m = pr;
-#pragma unroll
-    for (int k = 0; k < kMaxBatch; ++k) {
-        if (b < 0 && k < p.n_streams) {
-            if (m < r.rows[k]) b = k;
-            else m -= r.rows[k];
-        }
-    }
+// CTAs [first, last] that hold the parts of a column.
+__device__ __forceinline__ void parts_of(const RowsPlan& r, int32_t start, int32_t units, int32_t& first, int32_t& last) {
+    first = start / r.per;
+    last = (start + units - 1) / r.per;
 }
 
-// Rows of head h from the partial results of every item, a warp per row, 4 dims per lane.
-template <typename T>
-__device__ __noinline__ void rows_combine(const Params& p, const RowsPlan& r, int32_t h) {
+// Own group (stream b, group g) of head h: every part of its rows, in key order, a row per warp.
+template <typename T, int R>
+__device__ __noinline__ void rows_combine(const Params& p, const RowsPlan& r, int32_t h, int32_t b, int32_t g) {
     const int lane = threadIdx.x & 31;
-    for (int32_t pr = threadIdx.x >> 5; pr < r.total; pr += kRowsWarps) {
-        int32_t b, m;
-        unpack_row(p, r, pr, b, m);
-        int32_t base = p.n_heads * r.gp * r.np, groups = 0;
-        const Stream* st = &p.s[0];
+    const int32_t m = g * R + (threadIdx.x >> 5);
+    if ((threadIdx.x >> 5) >= R || m >= r.rows[b]) return;
+    const int32_t* idx = nullptr;
+    void* out_base = nullptr;
 #pragma unroll
-        for (int k = 0; k < kMaxBatch; ++k) {
-            const int32_t g = (r.rows[k] + kRowsTile - 1) / kRowsTile;
-            if (k < b) base += p.n_heads * g * r.no;
-            if (k == b) {
-                groups = g;
-                st = &p.s[k];
+    for (int k = 0; k < kMaxBatch; ++k)
+        if (k == b) {
+            idx = p.s[k].idx;
+            out_base = p.s[k].out;
+        }
+    const int32_t i = idx[m];
+    // parts: the packed row's prefix column, then the own column; part c of column x is slot x + c
+    int32_t p0 = 0, n_pre = 0, pre_slot = 0;
+    const int32_t pr = r.first[b] + m;
+    if (r.gp > 0) {
+        const int32_t col = h * r.gp + pr / R;
+        int32_t last;
+        parts_of(r, col * r.up, r.up, p0, last);
+        n_pre = last - p0 + 1;
+        pre_slot = col + p0;
+    }
+    const int32_t groups = (r.rows[b] + R - 1) / R;
+    const int32_t own = p.n_heads * r.group0[b] + h * groups + g;
+    int32_t o0, o1;
+    parts_of(r, p.n_heads * r.gp * r.up + own * r.uo, r.uo, o0, o1);
+    const int32_t own_slot = p.n_heads * r.gp + own + o0, n = n_pre + o1 - o0 + 1;
+    auto slot = [&](int32_t c) {
+        return p.part + (int64_t)(c < n_pre ? pre_slot + c : own_slot + c - n_pre) * kRowsSlotFloats;
+    };
+    auto row_of = [&](int32_t c) { return c < n_pre ? pr % R : m % R; };
+    // 32 parts at a time: lane c holds part c's maximum and sum, all lanes 8 parts' positions, every load
+    // of a round in flight together (one round trip to L2 for up to 8 parts)
+    float top = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int32_t c0 = 0; c0 < n; c0 += 32) {
+        float m_c = -INFINITY, l_c = 0.f;
+        if (c0 + lane < n) {
+            const float* q = slot(c0 + lane) + kRowsMax * kHeadDim + row_of(c0 + lane);
+            m_c = __ldcg(q);
+            l_c = __ldcg(q + kRowsMax);
+        }
+        float w = 0.f;
+        for (int32_t c1 = c0; c1 < min(n, c0 + 32); c1 += 8) {
+            float4 x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                x[k] = c1 + k < n ? __ldcg(reinterpret_cast<const float4*>(slot(c1 + k) + row_of(c1 + k) * kHeadDim) + lane)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c1 == c0) {
+                float t = m_c;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+                t = fmaxf(t, top);
+                const float base = t == -INFINITY ? 0.f : t, al = ex2_approx(top - base);
+                l *= al;
+                acc = make_float4(acc.x * al, acc.y * al, acc.z * al, acc.w * al);
+                top = t;
+                w = ex2_approx(m_c - base);
+                l += w * l_c;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float wc = __shfl_sync(0xffffffffu, w, c1 + k - c0);
+                acc.x += wc * x[k].x;
+                acc.y += wc * x[k].y;
+                acc.z += wc * x[k].z;
+                acc.w += wc * x[k].w;
             }
         }
-        const int32_t n_pre = r.gp > 0 ? r.np : 0, n = n_pre + r.no;
-        const int32_t pre0 = (h * r.gp + pr / kRowsTile) * r.np, own0 = base + (h * groups + m / kRowsTile) * r.no;
-        auto slot = [&](int32_t c) { return p.part + (int64_t)(c < n_pre ? pre0 + c : own0 + c - n_pre) * kRowsSlotFloats; };
-        auto row_of = [&](int32_t c) { return c < n_pre ? pr % kRowsTile : m % kRowsTile; };
-        float top = -INFINITY;
-        for (int32_t c = lane; c < n; c += 32) top = fmaxf(top, __ldcg(slot(c) + kRowsTile * kHeadDim + row_of(c)));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (top == -INFINITY) top = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
-#pragma unroll 4
-        for (int32_t c = 0; c < n; ++c) {
-            const float* q = slot(c);
-            const int32_t rr = row_of(c);
-            const float w = ex2_approx(__ldcg(q + kRowsTile * kHeadDim + rr) - top);
-            l += w * __ldcg(q + kRowsTile * kHeadDim + kRowsTile + rr);
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(q + rr * kHeadDim) + lane);
-            acc.x += w * x.x;
-            acc.y += w * x.y;
-            acc.z += w * x.z;
-            acc.w += w * x.w;
-        }
-        const int32_t i = st->idx[m];
-        if (i < 0 || i >= p.n_tokens) {
-            if (lane == 0) atomicOr(&g_error_word, kErrBounds);
-            continue;
-        }
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-        T* out = static_cast<T*>(st->out) + (int64_t)i * p.ld_out + (int64_t)h * kHeadDim;
-        *reinterpret_cast<uint2*>(out + 4 * lane) =
-            make_uint2(StoreT<T>::pack2(acc.x * inv, acc.y * inv), StoreT<T>::pack2(acc.z * inv, acc.w * inv));
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (i < 0 || i >= p.n_tokens) {
+        if (lane == 0) atomicOr(&g_error_word, kErrBounds);
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    // position 8 d + e of a stored row is dim 16 key_of(e) + d: this lane's e = 4 (lane & 1) + 0..3
+    uint16_t* out = reinterpret_cast<uint16_t*>(static_cast<T*>(out_base) + (int64_t)i * p.ld_out + (int64_t)h * kHeadDim) +
+                    (lane >> 1);
+    const uint32_t lo = StoreT<T>::pack2(acc.x * inv, acc.y * inv), hi = StoreT<T>::pack2(acc.z * inv, acc.w * inv);
+    const int e = 4 * (lane & 1);
+    out[16 * key_of(e)] = (uint16_t)lo;
+    out[16 * key_of(e + 1)] = (uint16_t)(lo >> 16);
+    out[16 * key_of(e + 2)] = (uint16_t)hi;
+    out[16 * key_of(e + 3)] = (uint16_t)(hi >> 16);
 }
 
-template <typename T, int F>
-__global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_constant__ Params p) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int32_t last;
+// NQ: 8-row tiles of a group.
+template <typename T, int F, int NQ>
+__global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_constant__ RowsMaps maps, const __grid_constant__ Params p) {
+    constexpr int R = 8 * NQ;
+    constexpr bool kF16 = StoreT<T>::kUmmaFormat == 0;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    __shared__ RowsPlan r;
+    __shared__ int abort;
+    __shared__ uint32_t ready;                 // own groups whose last part this CTA delivered
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
-    const uint32_t ring = smem_u32(smem) + warp * kRingWarp;
-    float* xo = reinterpret_cast<float*>(smem);                                     // [warp][16][kPadRow]
-    float* xm = reinterpret_cast<float*>(smem + kRowsWarps * kRingWarp);            // [warp][16] maxima, then sums
+    const uint32_t base = smem_u32(smem), ring = base + warp * kRingWarp, q_at = base + kRowsSmemQ;
+    const uint32_t bars = base + kRowsSmemBar + warp * kDepth * 8;
+    uint32_t it = 0;                           // blocks of this warp so far
+    if (threadIdx.x == 0) abort = 0;
+    if (lane == 0) {
+        for (int d = 0; d < kDepth; ++d) mbar_init(bars + 8 * d, 1);
+        fence_mbar_init();
+    }
+    float* xo = reinterpret_cast<float*>(smem);                                     // [warp][R][kPadRow]
+    float* xm = reinterpret_cast<float*>(smem + kRowsSmemM);                        // [R][warp] maxima, then sums
     pdl_launch_dependents();
     pdl_wait();
-    const RowsPlan r = rows_plan(p);
-    const int32_t pre_items = p.n_heads * r.gp * r.np;
-
-    for (int32_t item = blockIdx.x; item < r.items; item += gridDim.x) {
-        // ---- the item: 16 rows of head h against keys [k0, k0 + n) of one source
-        const bool pre = item < pre_items;
-        int32_t h, grp, chunk, b_own = 0, n_src;
-        Cache c = p.prefix;
-        const uint32_t* kg = p.pg;
-        if (pre) {
-            chunk = item % r.np;
-            const int32_t e = item / r.np;
-            h = e / r.gp;
-            grp = e - h * r.gp;
-            n_src = p.n_prefix;
-        } else {
-            int32_t e = item - pre_items, groups = 1;
-            b_own = -1;
+    if (warp == 0) {
+        int32_t m = 0, c = 0;
 #pragma unroll
-            for (int k = 0; k < kMaxBatch; ++k) {
-                const int32_t gk = (r.rows[k] + kRowsTile - 1) / kRowsTile, n_k = p.n_heads * gk * r.no;
-                if (b_own < 0 && k < p.n_streams) {
-                    if (e < n_k) {
-                        b_own = k;
-                        groups = gk;
-                        c = p.s[k].c;
-                        kg = p.s[k].kg;
-                    } else {
-                        e -= n_k;
-                    }
-                }
+        for (int b = 0; b < kMaxBatch; ++b)
+            if (b == lane && b < p.n_streams) c = *p.s[b].count;
+        m = max(0, min(c, p.max_rows));
+        if (c > p.max_rows && blockIdx.x == 0) atomicOr(&g_error_word, kErrBounds);
+        const int32_t groups = (m + R - 1) / R;
+        int32_t rows_to = m, groups_to = groups;      // inclusive sums over the streams
+#pragma unroll
+        for (int o = 1; o < kMaxBatch; o <<= 1) {
+            const int32_t x = __shfl_up_sync(0xffffffffu, rows_to, o), y = __shfl_up_sync(0xffffffffu, groups_to, o);
+            if (lane >= o) {
+                rows_to += x;
+                groups_to += y;
             }
-            chunk = e % r.no;
-            e /= r.no;
-            h = e / groups;
-            grp = e - h * groups;
-            n_src = p.n_tokens;
         }
-        const int32_t k0 = chunk * r.len;
-        const int32_t n_keys = min(r.len, n_src - k0), n_blk = (n_keys + kBlk - 1) / kBlk;
+        if (lane < kMaxBatch) {
+            r.rows[lane] = m;
+            r.first[lane] = rows_to - m;
+            r.group0[lane] = groups_to - groups;
+        }
+        if (lane == kMaxBatch - 1) {
+            r.total = rows_to;
+            r.go = groups_to;
+            r.gp = p.n_prefix > 0 ? (rows_to + R - 1) / R : 0;
+            r.up = (p.n_prefix + kUnitKeys - 1) / kUnitKeys;
+            r.uo = (p.n_tokens + kUnitKeys - 1) / kUnitKeys;
+            r.line = p.n_heads * (r.gp * r.up + r.go * r.uo);
+            r.per = (r.line + (int32_t)gridDim.x - 1) / (int32_t)gridDim.x;
+        }
+    }
+    __syncthreads();
 
-        const uint8_t* ck = c.k + (int64_t)h * kHeadDim;
-        const uint8_t* cv = c.v + (int64_t)h * kHeadDim;
-        const T* ks = static_cast<const T*>(c.ks) + (int64_t)h * c.ld_scale;
-        const T* vs = static_cast<const T*>(c.vs) + (int64_t)h * c.ld_scale;
-        // ---- asynchronous copies of block b of this warp's walk into ring slot `slot`. Keys past the
-        // source are filled with zeros (scales in groups of 8, whose rows are padded to 8).
-        auto fetch = [&](int32_t b, int slot) {
-            const uint32_t dst = ring + slot * kRingSlot;
-            const int32_t key0 = k0 + b * kBlk;
-            const int32_t row = lane >> 3, ch = lane & 7;
+    int32_t at = min((int64_t)r.line, (int64_t)blockIdx.x * r.per);
+    const int32_t end = min((int64_t)r.line, (int64_t)at + r.per);
+    while (at < end) {
+        // ---- the item: the part [u0, u0 + n) of a column
+        int32_t col;
+        const Column cl = column_at<R>(r, p.n_heads, at, col);
+        const int32_t u0 = at - cl.start, n_units = min(cl.units - u0, end - at);
+        at += n_units;
+        const bool pre = cl.stream < 0;
+        const int32_t h = cl.head, n_src = pre ? p.n_prefix : p.n_tokens;
+        const void *ks0 = p.prefix.ks, *vs0 = p.prefix.vs;
+        int64_t ld_scale = p.prefix.ld_scale;
+        const uint32_t* kg = p.pg;
+        const CUtensorMap *tk = &maps.pk, *tv = &maps.pv;
 #pragma unroll
-            for (int i = 0; i < kBlk / 4; ++i) {
-                const int32_t rr = i * 4 + row, key = key0 + rr;
-                const bool in = key < n_src;
-                const int64_t off = (int64_t)(in ? key : 0) * c.ld + ch * 16;
-                cp_async16(dst + rr * 128 + ((ch ^ ((rr & 1) << 2)) << 4), ck + off, in ? 16u : 0u);
-                cp_async16(dst + kBlkBytes + rr * 128 + ((ch ^ (rr & 7)) << 4), cv + off, in ? 16u : 0u);
+        for (int k = 0; k < kMaxBatch; ++k)
+            if (k == cl.stream) {
+                ks0 = p.s[k].c.ks;
+                vs0 = p.s[k].c.vs;
+                ld_scale = p.s[k].c.ld_scale;
+                kg = p.s[k].kg;
+                tk = &maps.k[k];
+                tv = &maps.v[k];
             }
-            if (lane < 8) {
-                const int32_t key = key0 + (lane & 3) * 8;
-                const bool in = key < n_src;
-                cp_async16(dst + kOffScale + lane * 16, (lane < 4 ? ks : vs) + (in ? key : 0), in ? 16u : 0u);
+        const int32_t k0 = u0 * kUnitKeys, n_keys = min(n_units * kUnitKeys, n_src - k0), n_blk = (n_keys + kBlk - 1) / kBlk;
+        const uint16_t* ks = static_cast<const uint16_t*>(ks0) + (int64_t)h * ld_scale + k0;
+        const uint16_t* vs = static_cast<const uint16_t*>(vs0) + (int64_t)h * ld_scale + k0;
+        if (kg != nullptr) kg += k0;
+        // ---- copies of block b of this warp's walk, the `at`-th it takes. Codes past the source are
+        // zeros; scales come in groups of 8, to which their rows are padded.
+        auto fetch = [&](int32_t b, uint32_t nth) {
+            if (lane == 0) {
+                const uint32_t slot = nth % kDepth, bar = bars + 8 * slot, dst = ring + slot * kRingSlot;
+                const uint32_t sdst = base + kRowsSmemScale + (warp * kDepth + slot) * kScaleSlot;
+                const uint32_t sbytes = n_keys - b * kBlk > 8 ? 32u : 16u;
+                mbar_arrive_expect_tx(bar, kRingSlot + 2 * sbytes);
+                tma_load_2d(dst, tk, bar, h * kHeadDim, k0 + b * kBlk);
+                tma_load_2d(dst + kBlkBytes, tv, bar, h * kHeadDim, k0 + b * kBlk);
+                bulk_load(sdst, ks + b * kBlk, sbytes, bar);
+                bulk_load(sdst + kBlk * 2, vs + b * kBlk, sbytes, bar);
             }
+        };
+        uint32_t g_next[2] = {0xffffffffu, 0xffffffffu};     // groups of this lane's keys, a block ahead
+        auto groups_of = [&](int32_t b) {
             if (kg != nullptr) {
-                const bool in = key0 + lane < n_src;
-                cp_async4(dst + kOffGroup + lane * 4, kg + (in ? key0 + lane : 0), in ? 4u : 0u);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int32_t key = b * kBlk + key_of(g) + 8 * e;
+                    g_next[e] = key < n_keys ? __ldg(kg + key) : 0u;
+                }
             }
         };
 #pragma unroll
         for (int d = 0; d < kDepth - 1; ++d) {
             const int32_t b = warp + d * kRowsWarps;
-            if (b < n_blk) fetch(b, d);
-            cp_async_commit();
+            if (b < n_blk) fetch(b, it + d);
         }
+        groups_of(warp);
 
-        // ---- the queries: rows g and g + 8 of the group, fragments in the order of the codes
-        uint32_t qa[2][16];
-        uint32_t qg[2];
+        // ---- queries into shared memory (a 16-byte piece per thread), this lane's rows' groups
+        auto row_at = [&](int32_t e, int32_t& b, int32_t& m) -> bool {      // row e of the group
+            m = cl.group * R + e;
+            b = cl.stream;
+            if (!pre) return m < r.rows[b];
+            if (m >= r.total) return false;
+            b = 0;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            int32_t b = b_own, m = grp * kRowsTile + g + 8 * e;
-            bool live = true;
-            if (pre) {
-                const int32_t pr = m;
-                live = pr < r.total;
-                unpack_row(p, r, live ? pr : 0, b, m);
-            }
+            for (int k = 1; k < kMaxBatch; ++k)
+                if (k < p.n_streams && m >= r.first[k]) b = k;
+            m -= r.first[b];
+            return true;
+        };
+        auto stream_of = [&](int32_t b) {
             const Stream* st = &p.s[0];
 #pragma unroll
-            for (int k = 0; k < kMaxBatch; ++k)
-                if (k == b) {
-                    st = &p.s[k];
-                    live = live && m < r.rows[k];
-                }
-            const T* q = static_cast<const T*>(st->qc) + (int64_t)m * st->ld_qc + (int64_t)h * kHeadDim + t * 16;
+            for (int k = 1; k < kMaxBatch; ++k)
+                if (k == b) st = &p.s[k];
+            return st;
+        };
+        if (threadIdx.x < R * 16) {
+            int32_t b, m;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (row_at(threadIdx.x >> 4, b, m)) {
+                const Stream* st = stream_of(b);
+                x = *reinterpret_cast<const uint4*>(static_cast<const T*>(st->qc) + (int64_t)m * st->ld_qc + (int64_t)h * kHeadDim +
+                                                    (threadIdx.x & 15) * 8);
+            }
+            sts128(q_at + (threadIdx.x >> 4) * kQPad + (threadIdx.x & 15) * 16, x);
+        }
+        uint32_t qg[NQ][2];
 #pragma unroll
-            for (int cc = 0; cc < 2; ++cc)
+        for (int q = 0; q < NQ; ++q)
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const uint4 x = live ? *reinterpret_cast<const uint4*>(q + cc * 64 + w * 8) : make_uint4(0, 0, 0, 0);
-                    qa[e][cc * 8 + w * 4 + 0] = x.x;
-                    qa[e][cc * 8 + w * 4 + 1] = x.y;
-                    qa[e][cc * 8 + w * 4 + 2] = x.z;
-                    qa[e][cc * 8 + w * 4 + 3] = x.w;
+            for (int e = 0; e < 2; ++e) {
+                int32_t b, m;
+                qg[q][e] = 0xffffffffu;
+                if (row_at(8 * q + 2 * t + e, b, m)) {
+                    const Stream* st = stream_of(b);
+                    if (st->qg != nullptr) {
+                        const int32_t i = st->idx[m];
+                        qg[q][e] = (i >= 0 && i < p.n_tokens) ? st->qg[i] : 0u;
+                    }
                 }
-            qg[e] = 0xffffffffu;
-            if (live && st->qg != nullptr) {
-                const int32_t i = st->idx[m];
-                qg[e] = (i >= 0 && i < p.n_tokens) ? st->qg[i] : 0u;
+            }
+        bool any_empty = false;      // a row that sees nothing needs its mask where the keys have none
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) any_empty = any_empty || qg[q][0] == 0 || qg[q][1] == 0;
+        any_empty = __any_sync(0xffffffffu, any_empty);
+        if (threadIdx.x == 0) ready = 0;
+        __syncthreads();
+
+        float o[NQ][8][4], m_run[NQ][2], l_run[NQ][2];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[q][j][e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                m_run[q][e] = -INFINITY;
+                l_run[q][e] = 0.f;
             }
         }
-
-        float o[16][4];
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-        float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
         const float sc = p.scale_log2 * q8::code_scale<T, F>();
 
-        int slot = 0;
-        for (int32_t b = warp; b < n_blk; b += kRowsWarps) {
-            {
-                const int32_t nb = b + (kDepth - 1) * kRowsWarps;
-                int ns = slot + kDepth - 1;
-                if (ns >= kDepth) ns -= kDepth;
-                if (nb < n_blk) fetch(nb, ns);
-                cp_async_commit();
-                cp_async_wait<kDepth - 1>();
-                __syncwarp();
+        uint32_t issued = it + min(kDepth - 1, (n_blk - warp + kRowsWarps - 1) / kRowsWarps);
+        for (int32_t b = warp; b < n_blk; b += kRowsWarps, ++it) {
+            if (b + (kDepth - 1) * kRowsWarps < n_blk) {
+                fetch(b + (kDepth - 1) * kRowsWarps, it + kDepth - 1);
+                ++issued;
             }
-            const uint32_t at = ring + slot * kRingSlot;
-            // S = Q K^T, four tiles of 8 keys
-            float s[4][4];
+            const uint32_t seen[2] = {g_next[0], g_next[1]};
+            groups_of(b + kRowsWarps);
+            const uint32_t slot = it % kDepth;
+            if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * slot, (it / kDepth) & 1, &abort))) break;
+            const uint8_t* blk_p = smem + warp * kRingWarp + slot * kRingSlot;
+            const uint16_t* sc_p = reinterpret_cast<const uint16_t*>(smem + kRowsSmemScale + (warp * kDepth + slot) * kScaleSlot);
+            // S^T = K Q^T
+            float s[NQ][4];
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) {
-                s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-                const uint32_t row = at + (nt * 8 + g) * 128, x4 = (uint32_t)(g & 1) << 2;
+            for (int q = 0; q < NQ; ++q) s[q][0] = s[q][1] = s[q][2] = s[q][3] = 0.f;
 #pragma unroll
-                for (int cc = 0; cc < 2; ++cc) {
-                    const uint4 k4 = lds128(row + (((uint32_t)(cc * 4 + t) ^ x4) << 4));
-                    const uint32_t w[4] = {k4.x, k4.y, k4.z, k4.w};
+            for (int cc = 0; cc < 2; ++cc) {
+                const uint32_t off = key_of(g) * 128 + ((uint32_t)((cc * 4 + t) ^ key_of(g)) << 4);
+                const uint4 ka = *reinterpret_cast<const uint4*>(blk_p + off), kb = *reinterpret_cast<const uint4*>(blk_p + off + 8 * 128);
+                const uint32_t wa[4] = {q8::code_word<F>(ka.x), q8::code_word<F>(ka.y), q8::code_word<F>(ka.z), q8::code_word<F>(ka.w)};
+                const uint32_t wb[4] = {q8::code_word<F>(kb.x), q8::code_word<F>(kb.y), q8::code_word<F>(kb.z), q8::code_word<F>(kb.w)};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        mma16816<T>(s[nt], qa[0][cc * 8 + 2 * j], qa[1][cc * 8 + 2 * j], qa[0][cc * 8 + 2 * j + 1],
-                                    qa[1][cc * 8 + 2 * j + 1], q8::decode2<T, F>(w[j], w[j], 0, 1),
-                                    q8::decode2<T, F>(w[j], w[j], 2, 3));
+                for (int jp = 0; jp < 2; ++jp) {
+                    uint4 q4[NQ];
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+                        q4[q] = *reinterpret_cast<const uint4*>(smem + kRowsSmemQ + (g + 8 * q) * kQPad + (cc * 64 + t * 16 + jp * 8) * 2);
+#pragma unroll
+                    for (int jj = 0; jj < 2; ++jj) {
+                        const int j = 2 * jp + jj;
+                        const uint32_t a0 = q8::code_pair<T, F>(wa[j], 0, 1), a1 = q8::code_pair<T, F>(wb[j], 0, 1);
+                        const uint32_t a2 = q8::code_pair<T, F>(wa[j], 2, 3), a3 = q8::code_pair<T, F>(wb[j], 2, 3);
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q)
+                            mma16816<T>(s[q], a0, a1, a2, a3, jj ? q4[q].z : q4[q].x, jj ? q4[q].w : q4[q].y);
+                    }
                 }
             }
-            // scales, masks
-            float v_sc[4][2];            // what P is multiplied with
-            uint32_t v_pow[4];           // f16: the pairs' powers of two
+            // scales and masks: this lane's keys, key_of(g) and 8 behind it
+            float v_sc[2];               // what P is multiplied with
             const int32_t left = n_keys - b * kBlk;
-            float bm[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int nt = 0; nt < 4; ++nt) {
-                const float2 k2 = StoreT<T>::unpack2(lds32(at + kOffScale + (nt * 8 + 2 * t) * 2));
-                const float2 v2 = StoreT<T>::unpack2(lds32(at + kOffScale + kBlk * 2 + (nt * 8 + 2 * t) * 2));
-                const float kk[2] = {k2.x, k2.y};
-                float vv[2] = {v2.x, v2.y};
-                uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-                if (kg != nullptr) {
-                    const uint2 g2 = lds64(at + kOffGroup + (nt * 8 + 2 * t) * 4);
-                    seen[0] = g2.x;
-                    seen[1] = g2.y;
-                }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const bool v_ok = finite(vv[e]);
-                    const float f = v_ok && finite(kk[e]) ? kk[e] * sc : __uint_as_float(0x7fc00000u);
-                    v_sc[nt][e] = v_ok ? vv[e] : 0.f;
-                    if constexpr (StoreT<T>::kUmmaFormat == 0) {
-                        vv[e] = v_sc[nt][e];
-                        v_sc[nt][e] = __uint_as_float((__float_as_uint(vv[e]) & 0x007fffffu) | 0x3f800000u);
-                        vv[e] = __uint_as_float(__float_as_uint(vv[e]) & 0x7f800000u) * q8::code_scale<T, F>();
-                    }
-                    const bool in = nt * 8 + 2 * t + e < left;
-                    s[nt][e] = in && (seen[e] & qg[0]) ? s[nt][e] * f : -INFINITY;
-                    s[nt][2 + e] = in && (seen[e] & qg[1]) ? s[nt][2 + e] * f : -INFINITY;
-                    bm[0] = fmaxf(bm[0], s[nt][e]);
-                    bm[1] = fmaxf(bm[1], s[nt][2 + e]);
-                }
-                if constexpr (StoreT<T>::kUmmaFormat == 0) v_pow[nt] = StoreT<T>::pack2(vv[0], vv[1]);
-            }
+            bool grow = false;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                bm[e] = fmaxf(bm[e], __shfl_xor_sync(0xffffffffu, bm[e], 1));
-                bm[e] = fmaxf(bm[e], __shfl_xor_sync(0xffffffffu, bm[e], 2));
+                const int key = key_of(g) + 8 * e;
+                const float kk = StoreT<T>::unpack2(sc_p[key]).x, vv = StoreT<T>::unpack2(sc_p[kBlk + key]).x;
+                const bool v_ok = q8::valid_scale<T, F>(vv);
+                const float f = v_ok && q8::valid_scale<T, F>(kk) ? kk * sc : __uint_as_float(0x7fc00000u);
+                v_sc[e] = v_ok ? vv : 0.f;
+                if (kF16) v_sc[e] = __uint_as_float((__float_as_uint(v_sc[e]) & 0x007fffffu) | 0x3f800000u);
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) s[q][2 * e + d] *= f;
             }
-            // the running maxima move only where one grows by more than 2^8 (P stays below that)
-            if (__any_sync(0xffffffffu, bm[0] > m_run[0] + 8.f || bm[1] > m_run[1] + 8.f)) {
-                float al[2];
+            if (kg != nullptr || left < kBlk) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float mn = fmaxf(m_run[e], bm[e]);
-                    al[e] = mn == m_run[e] ? 1.f : ex2_approx(m_run[e] - mn);
-                    m_run[e] = mn;
-                    l_run[e] *= al[e];
-                }
+                    const bool in = key_of(g) + 8 * e < left;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    o[j][0] *= al[0];
-                    o[j][1] *= al[0];
-                    o[j][2] *= al[1];
-                    o[j][3] *= al[1];
+                    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                        for (int d = 0; d < 2; ++d)
+                            if (!in || (seen[e] & qg[q][d]) == 0) s[q][2 * e + d] = -INFINITY;
                 }
+            } else if (any_empty) {
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int d = 0; d < 2; ++d)
+                        if (qg[q][d] == 0) s[q][d] = s[q][2 + d] = -INFINITY;
             }
-            uint32_t pa[4][2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float mu = m_run[e] == -INFINITY ? 0.f : m_run[e];
+            for (int q = 0; q < NQ; ++q)
 #pragma unroll
-                for (int nt = 0; nt < 4; ++nt) {
-                    const float p0 = ex2_approx(s[nt][2 * e] - mu), p1 = ex2_approx(s[nt][2 * e + 1] - mu);
-                    l_run[e] += p0 + p1;
-                    pa[nt][e] = StoreT<T>::pack2(p0 * v_sc[nt][0], p1 * v_sc[nt][1]);
-                }
-            }
-            // O += P V, two steps of 16 keys
+                for (int d = 0; d < 2; ++d) grow = grow || fmaxf(s[q][d], s[q][2 + d]) > m_run[q][d] + 8.f;
+            // the running maxima move only where a score passes one by more than 2^8 (P stays below that)
+            if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                uint32_t w[4][4];
+                for (int q = 0; q < NQ; ++q)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t row = kt * 16 + 2 * t + (e & 1) + (e >> 1) * 8;
-                    const uint4 v4 = lds128(at + kBlkBytes + row * 128 + (((uint32_t)g ^ (row & 7)) << 4));
-                    w[e][0] = v4.x;
-                    w[e][1] = v4.y;
-                    w[e][2] = v4.z;
-                    w[e][3] = v4.w;
-                }
+                    for (int d = 0; d < 2; ++d) {
+                        float x = fmaxf(s[q][d], s[q][2 + d]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        const float mn = fmaxf(m_run[q][d], x);
+                        const float al = mn == m_run[q][d] ? 1.f : ex2_approx(m_run[q][d] - mn);
+                        m_run[q][d] = mn;
+                        l_run[q][d] *= al;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    uint32_t b0 = q8::decode2<T, F>(w[0][j >> 2], w[1][j >> 2], j & 3, j & 3);
-                    uint32_t b1 = q8::decode2<T, F>(w[2][j >> 2], w[3][j >> 2], j & 3, j & 3);
-                    if constexpr (StoreT<T>::kUmmaFormat == 0) {
-                        b0 = q8::mul2<T>(b0, v_pow[2 * kt]);
-                        b1 = q8::mul2<T>(b1, v_pow[2 * kt + 1]);
+                        for (int j = 0; j < 8; ++j) {
+                            o[q][j][d] *= al;
+                            o[q][j][2 + d] *= al;
+                        }
                     }
-                    mma16816<T>(o[j], pa[2 * kt][0], pa[2 * kt][1], pa[2 * kt + 1][0], pa[2 * kt + 1][1], b0, b1);
+            }
+            uint32_t pb[NQ][2];
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) {
+                float e_[4];
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    const float mu = m_run[q][d] == -INFINITY ? 0.f : m_run[q][d];
+                    e_[d] = ex2_approx(s[q][d] - mu);
+                    e_[2 + d] = ex2_approx(s[q][2 + d] - mu);
+                    l_run[q][d] += e_[d] + e_[2 + d];
                 }
+                pb[q][0] = transpose8(StoreT<T>::pack2(e_[0] * v_sc[0], e_[1] * v_sc[0]));
+                pb[q][1] = transpose8(StoreT<T>::pack2(e_[2] * v_sc[1], e_[3] * v_sc[1]));
+            }
+            // O^T += V^T P^T
+            // (operand row index 2 t + x of a half is key key_of(2 t + x) = t + 4 x)
+            uint32_t w[4][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t row = t + 4 * (e & 1) + 8 * (e >> 1);
+                const uint4 v4 = *reinterpret_cast<const uint4*>(blk_p + kBlkBytes + row * 128 + (((uint32_t)key_of(g) ^ (row & 7)) << 4));
+                w[e][0] = q8::code_word<F>(v4.x);
+                w[e][1] = q8::code_word<F>(v4.y);
+                w[e][2] = q8::code_word<F>(v4.z);
+                w[e][3] = q8::code_word<F>(v4.w);
+            }
+            uint32_t pow2[2] = {0, 0};
+            if constexpr (kF16) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float2 v2 = make_float2(StoreT<T>::unpack2(sc_p[kBlk + 8 * e + t]).x, StoreT<T>::unpack2(sc_p[kBlk + 8 * e + t + 4]).x);
+                    v2.x = q8::valid_scale<T, F>(v2.x) ? __uint_as_float(__float_as_uint(v2.x) & 0x7f800000u) * q8::code_scale<T, F>() : 0.f;
+                    v2.y = q8::valid_scale<T, F>(v2.y) ? __uint_as_float(__float_as_uint(v2.y) & 0x7f800000u) * q8::code_scale<T, F>() : 0.f;
+                    pow2[e] = StoreT<T>::pack2(v2.x, v2.y);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                // dims 2 j and 2 j + 1 of the lane's 16: the two keys' bytes side by side
+                const uint32_t lo = __byte_perm(w[0][j >> 1], w[1][j >> 1], (j & 1) ? 0x7362 : 0x5140);
+                const uint32_t hi = __byte_perm(w[2][j >> 1], w[3][j >> 1], (j & 1) ? 0x7362 : 0x5140);
+                uint32_t a0 = q8::code_pair<T, F>(lo, 0, 1), a1 = q8::code_pair<T, F>(lo, 2, 3);
+                uint32_t a2 = q8::code_pair<T, F>(hi, 0, 1), a3 = q8::code_pair<T, F>(hi, 2, 3);
+                if constexpr (kF16) {
+                    a0 = q8::mul2<T>(a0, pow2[0]);
+                    a1 = q8::mul2<T>(a1, pow2[0]);
+                    a2 = q8::mul2<T>(a2, pow2[1]);
+                    a3 = q8::mul2<T>(a3, pow2[1]);
+                }
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) mma16816<T>(o[q][j], a0, a1, a2, a3, pb[q][0], pb[q][1]);
             }
             __syncwarp();
-            if (++slot == kDepth) slot = 0;
         }
-        cp_async_wait<0>();
+        // after a timeout only: nothing may land in shared memory any more
+        for (; it < issued; ++it) mbar_wait_drain_bounded(bars + 8 * (it % kDepth), (it / kDepth) & 1);
         __syncthreads();
-        // ---- the warps' results meet: O[row][8 * tile + column], then each thread 8 dims of one row
+        if (abort) return;
+        // ---- the warps' results meet: position 8 d + g of a row is d of lane g's 16 dims (tile j holds
+        // d = 2 j and 2 j + 1), then a row per warp, four positions per lane
+        const int live = pre ? min(R, r.total - cl.group * R) : min(R, r.rows[cl.stream] - cl.group * R);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
-            l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
-            float* dst = xo + (warp * kRowsTile + g + 8 * e) * kPadRow + 2 * t;
+        for (int q = 0; q < NQ; ++q)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) *reinterpret_cast<float2*>(dst + 8 * j) = make_float2(o[j][2 * e], o[j][2 * e + 1]);
-            if (t == 0) {
-                xm[warp * kRowsTile + g + 8 * e] = m_run[e];
-                xm[(kRowsWarps + warp) * kRowsTile + g + 8 * e] = l_run[e];
+            for (int d = 0; d < 2; ++d) {
+                const int row = 8 * q + 2 * t + d;
+                float* dst = xo + (warp * R + row) * kPadRow + g;
+                if (row < live) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        dst[16 * j] = o[q][j][d];
+                        dst[16 * j + 8] = o[q][j][2 + d];
+                    }
+                }
+                float l = l_run[q][d];
+                l += __shfl_xor_sync(0xffffffffu, l, 4);
+                l += __shfl_xor_sync(0xffffffffu, l, 8);
+                l += __shfl_xor_sync(0xffffffffu, l, 16);
+                if (g == 0) {
+                    xm[row * kRowsWarps + warp] = m_run[q][d];
+                    xm[(R + row) * kRowsWarps + warp] = l;
+                }
+            }
+        __syncthreads();
+        if (warp < live) {
+            const int row = warp;
+            const float m_w = lane < kRowsWarps ? xm[row * kRowsWarps + lane] : -INFINITY;
+            float top = m_w;
+#pragma unroll
+            for (int e = 8; e > 0; e >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
+            top = __shfl_sync(0xffffffffu, top, 0);
+            const float f = ex2_approx(m_w - (top == -INFINITY ? 0.f : top));
+            float l = lane < kRowsWarps ? f * xm[(R + row) * kRowsWarps + lane] : 0.f;
+#pragma unroll
+            for (int e = 8; e > 0; e >>= 1) l += __shfl_xor_sync(0xffffffffu, l, e);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < kRowsWarps; ++k) {
+                const float fk = __shfl_sync(0xffffffffu, f, k);
+                const float4 x = *reinterpret_cast<const float4*>(xo + (k * R + row) * kPadRow + 4 * lane);
+                acc.x += fk * x.x;
+                acc.y += fk * x.y;
+                acc.z += fk * x.z;
+                acc.w += fk * x.w;
+            }
+            float* dst = p.part + (int64_t)(col + (int32_t)blockIdx.x) * kRowsSlotFloats;
+            *reinterpret_cast<float4*>(dst + row * kHeadDim + 4 * lane) = acc;
+            if (lane == 0) {
+                dst[kRowsMax * kHeadDim + row] = top;
+                dst[kRowsMax * kHeadDim + kRowsMax + row] = l;
             }
         }
-        __syncthreads();
-        {
-            const int row = threadIdx.x >> 4, cc = threadIdx.x & 15;
-            float top = -INFINITY;
+        __syncthreads();     // the arrivals below release what every thread stored
+        // ---- arrivals: thread e for the e-th own group that the item's rows belong to
+        if (threadIdx.x < 32) {
+            int32_t b = -1, grp = 0, found = 0;
+            if (!pre) {
+                if (lane == 0) {
+                    b = cl.stream;
+                    grp = cl.group;
+                }
+            } else {
+                const int32_t r0 = cl.group * R, r1 = min(r0 + R, r.total);     // packed rows
 #pragma unroll
-            for (int w = 0; w < kRowsWarps; ++w) top = fmaxf(top, xm[w * kRowsTile + row]);
-            const float mu = top == -INFINITY ? 0.f : top;
-            float acc[8], l = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-#pragma unroll
-            for (int w = 0; w < kRowsWarps; ++w) {
-                const float f = ex2_approx(xm[w * kRowsTile + row] - mu);
-                l += f * xm[(kRowsWarps + w) * kRowsTile + row];
-                const float* src = xo + (w * kRowsTile + row) * kPadRow + (cc >> 1) + (cc & 1) * 64;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) acc[e] += f * src[8 * e];   // dim 16 * (cc / 2) + 8 * (cc % 2) + e
+                for (int k = 0; k < kMaxBatch; ++k)
+                    if (k < p.n_streams && r.rows[k] > 0) {
+                        const int32_t a0 = max(r0, r.first[k]) - r.first[k], a1 = min(r1, r.first[k] + r.rows[k]) - r.first[k];
+                        if (a1 > a0) {
+                            const int32_t g0 = a0 / R, g1 = (a1 - 1) / R;
+                            if (lane >= found && lane <= found + g1 - g0) {
+                                b = k;
+                                grp = g0 + lane - found;
+                            }
+                            found += g1 - g0 + 1;
+                        }
+                    }
             }
-            float* dst = p.part + (int64_t)item * kRowsSlotFloats;
-            float4* d4 = reinterpret_cast<float4*>(dst + row * kHeadDim + cc * 8);
-            d4[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-            d4[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-            if (cc == 0) {
-                dst[kRowsTile * kHeadDim + row] = top;
-                dst[kRowsTile * kHeadDim + kRowsTile + row] = l;
+            bool done = false;
+            if (b >= 0) {
+                const int32_t groups = (r.rows[b] + R - 1) / R, own = p.n_heads * r.group0[b] + h * groups + grp;
+                int32_t c0, c1;
+                parts_of(r, p.n_heads * r.gp * r.up + own * r.uo, r.uo, c0, c1);
+                int32_t all = c1 - c0 + 1;
+                if (r.gp > 0) {
+                    const int32_t x0 = r.first[b] + grp * R, x1 = min(x0 + R, r.first[b] + r.rows[b]);
+                    for (int32_t x = x0 / R; x <= (x1 - 1) / R; ++x) {
+                        parts_of(r, (h * r.gp + x) * r.up, r.up, c0, c1);
+                        all += c1 - c0 + 1;
+                    }
+                }
+                int32_t* cnt = p.cnt + (r.group0[b] + grp) * p.n_heads + h;
+                done = atom_add_acq_rel_gpu(cnt, 1) == all - 1;
+                if (done) *cnt = 0;      // for the next launch
             }
-        }
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const int32_t all = r.gp * r.np + r.go * r.no;
-            const int32_t before = atom_add_acq_rel_gpu(p.cnt + h, 1);
-            last = before == all - 1;
-            if (last) p.cnt[h] = 0;      // for the next launch
+            const uint32_t vote = __ballot_sync(0xffffffffu, done);
+            if (lane == 0) ready = vote;
         }
         __syncthreads();
-        if (last) rows_combine<T>(p, r, h);
+        for (uint32_t left = ready; left != 0; left &= left - 1) {
+            const int e = __ffs(left) - 1;
+            int32_t b = cl.stream, grp = cl.group;
+            if (pre) {                   // the e-th own group again
+                const int32_t r0 = cl.group * R, r1 = min(r0 + R, r.total);
+                int32_t found = 0;
+#pragma unroll
+                for (int k = 0; k < kMaxBatch; ++k)
+                    if (k < p.n_streams && r.rows[k] > 0) {
+                        const int32_t a0 = max(r0, r.first[k]) - r.first[k], a1 = min(r1, r.first[k] + r.rows[k]) - r.first[k];
+                        if (a1 > a0) {
+                            const int32_t g0 = a0 / R, g1 = (a1 - 1) / R;
+                            if (e >= found && e <= found + g1 - g0) {
+                                b = k;
+                                grp = g0 + e - found;
+                            }
+                            found += g1 - g0 + 1;
+                        }
+                    }
+            }
+            rows_combine<T, R>(p, r, h, b, grp);
+        }
+        fence_async_smem();          // the next item's copies overwrite the exchange
         __syncthreads();
     }
 }
@@ -671,8 +870,9 @@ __global__ void __launch_bounds__(kVisThreads) visible_steps_kernel(const __grid
     }
     const uint32_t w_any = __reduce_or_sync(0xffffffffu, live ? mine : 0u);
     if (lane == 0) atomicOr(&any_row, w_any);
-    const uint32_t same = __match_any_sync(0xffffffffu, mine) & __ballot_sync(0xffffffffu, live);
-    if (live && lane == __ffs(same) - 1) row_word[atomicAdd(&n_words, 1)] = mine;
+    // (rows whose set is empty are left out: their result is zeros whatever their scores)
+    const uint32_t same = __match_any_sync(0xffffffffu, mine) & __ballot_sync(0xffffffffu, live && mine != 0);
+    if (live && mine != 0 && lane == __ffs(same) - 1) row_word[atomicAdd(&n_words, 1)] = mine;
     __syncthreads();
     const uint32_t seen_by = any_row;
     const int32_t tiles = a.n_pre + a.n_own;
@@ -768,9 +968,6 @@ __global__ void __launch_bounds__(kVisThreads) visible_steps_kernel(const __grid
         : "r"(taddr), "r"((taddr) + 32u), "r"((taddr) + 64u), "r"((taddr) + 96u)                                      \
         : "memory")
 
-// Orders this thread's shared-memory writes before the asynchronous proxy's reads of them.
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
 // ---- pieces of the tile kernel --------------------------------------------------------------------
 // Maximum that is NaN where an operand is (a NaN score must reach its row).
 __device__ __forceinline__ float max3n(float a, float b, float c) {
@@ -795,30 +992,51 @@ __device__ __forceinline__ int64_t part_at(int32_t i0, int32_t per, int32_t c, i
 template <typename T>
 __device__ __forceinline__ void combine_parts(const float* part, int32_t i0, int32_t per, int32_t c0, int32_t c1, int t, int r,
                                               T* out_row) {
-    float top = -INFINITY;
-    for (int32_t c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(part + part_at(i0, per, c, t) + kBM * kD + r));
-    if (top == -INFINITY) top = 0.f;
-    float l = 0.f;
-    for (int32_t c = c0; c <= c1; ++c) {
-        const float* q = part + part_at(i0, per, c, t) + kBM * kD + r;
-        l += ex2_approx(__ldcg(q) - top) * __ldcg(q + kBM);
+    float top = -INFINITY, l = 0.f;
+    for (int32_t c = c0; c <= c1; c += 4) {              // four parts' maxima and sums in flight together
+        float m4[4], l4[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float* q = part + part_at(i0, per, min(c + e, c1), t) + kBM * kD + r;
+            m4[e] = c + e <= c1 ? __ldcg(q) : -INFINITY;
+            l4[e] = c + e <= c1 ? __ldcg(q + kBM) : 0.f;
+        }
+        const float next = fmaxf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), top);
+        const float base = next == -INFINITY ? 0.f : next;
+        l *= ex2_approx(top - base);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) l += ex2_approx(m4[e] - base) * l4[e];
+        top = next;
     }
+    if (top == -INFINITY) top = 0.f;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll 1
     for (int h = 0; h < 4; ++h) {
         float acc[32];
 #pragma unroll
         for (int k = 0; k < 32; ++k) acc[k] = 0.f;
-        for (int32_t c = c0; c <= c1; ++c) {
-            const float* q = part + part_at(i0, per, c, t);
-            const float w = ex2_approx(__ldcg(q + kBM * kD + r) - top);
+#pragma unroll 1
+        for (int32_t c = c0; c <= c1; c += 2) {          // two parts' loads in flight together
+            float4 x[2][8];
+            float w[2];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(q) + (h * 8 + k) * kBM + r);
-                acc[4 * k] += w * x.x;
-                acc[4 * k + 1] += w * x.y;
-                acc[4 * k + 2] += w * x.z;
-                acc[4 * k + 3] += w * x.w;
+            for (int e = 0; e < 2; ++e) {
+                const bool in = c + e <= c1;
+                const float* q = part + part_at(i0, per, in ? c + e : c, t);
+                w[e] = in ? __ldcg(q + kBM * kD + r) : -INFINITY;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[e][k] = __ldcg(reinterpret_cast<const float4*>(q) + (h * 8 + k) * kBM + r);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float f = ex2_approx(w[e] - top);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    acc[4 * k] += f * x[e][k].x;
+                    acc[4 * k + 1] += f * x[e][k].y;
+                    acc[4 * k + 2] += f * x[e][k].z;
+                    acc[4 * k + 3] += f * x[e][k].w;
+                }
             }
         }
         if (out_row != nullptr) {
@@ -838,7 +1056,7 @@ __device__ __forceinline__ void combine_parts(const float* part, int32_t i0, int
 // kernel, so that the step loop around it keeps its code.
 template <typename T>
 __device__ __noinline__ void cut_epilogue(float* part, int32_t* counters, int32_t per, const Item* it, int t, int r, int warp,
-                                          uint32_t tO, float m_run, float l_run, uint32_t ofree, T* out_row) {
+                                          uint32_t tO, float m_run, float l_run, bool blind, uint32_t ofree, T* out_row) {
     const int32_t c = (int32_t)blockIdx.x, i0 = it->i0, c_first = it->c_first, c_last = it->c_last;
     float* slot = part + part_at(i0, per, c, t);
 #pragma unroll 1
@@ -848,8 +1066,9 @@ __device__ __noinline__ void cut_epilogue(float* part, int32_t* counters, int32_
 #pragma unroll
         for (int k = 0; k < 8; ++k)
             reinterpret_cast<float4*>(slot)[(h * 8 + k) * kBM + r] =
-                make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]),
-                            __uint_as_float(o[4 * k + 3]));
+                blind ? make_float4(0.f, 0.f, 0.f, 0.f)
+                      : make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]),
+                                    __uint_as_float(o[4 * k + 3]));
     }
     slot[kBM * kD + r] = m_run;
     slot[kBM * kD + kBM + r] = l_run;
@@ -985,9 +1204,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                     next_word = list ? list[s0 + j + 1] : (uint32_t)(s0 + j + 1);
                     scales(next_word, next_k, next_v);
                 }
-                // a row that is not finite: its scores are NaN, its V counts as zeros
-                if (!finite(sv) || !finite(sk)) sk = __uint_as_float(0x7fc00000u);
-                if (!finite(sv)) sv = 0.f;
+                // a row without a valid scale: its scores are NaN, its V counts as zeros
+                const bool v_ok = q8::valid_scale<T, F>(sv);
+                if (!v_ok || !q8::valid_scale<T, F>(sk)) sk = __uint_as_float(0x7fc00000u);
+                if (!v_ok) sv = 0.f;
 #pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv, ++in) {
                     const uint32_t rs = in % kRaws, ts = in % kTiles;
@@ -1402,9 +1622,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                 else
                     atomicOr(&g_error_word, kErrBounds);
             }
+            const bool blind = it->list != nullptr && *my_groups == 0;   // the row's set is empty
+            if (blind) m_run = -INFINITY;
             if (m_run == -INFINITY) l_run = 0.f;      // the row saw nothing
             if (it->cut) {
-                cut_epilogue<T>(a.part, a.cnt, per, it, t, r, warp, tO, m_run, l_run, bar(kOFree + t), out_row);
+                cut_epilogue<T>(a.part, a.cnt, per, it, t, r, warp, tO, m_run, l_run, blind, bar(kOFree + t), out_row);
             } else {
                 const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
 #pragma unroll 1
@@ -1415,7 +1637,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                         uint4* dst = reinterpret_cast<uint4*>(out_row + 32 * h);
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
-                            dst[q] = make_uint4(
+                            dst[q] = blind ? make_uint4(0, 0, 0, 0) : make_uint4(
                                 StoreT<T>::pack2(__uint_as_float(o[8 * q]) * inv, __uint_as_float(o[8 * q + 1]) * inv),
                                 StoreT<T>::pack2(__uint_as_float(o[8 * q + 2]) * inv, __uint_as_float(o[8 * q + 3]) * inv),
                                 StoreT<T>::pack2(__uint_as_float(o[8 * q + 4]) * inv, __uint_as_float(o[8 * q + 5]) * inv),

@@ -49,6 +49,9 @@ template <typename T, int F> __device__ __forceinline__ constexpr float scale_ca
     return F == kInt8 ? (bf16 ? 0x1.fep+120f : 511.75f) : (bf16 ? 0x1.22p+119f : 146.125f);
 }
 
+// Whether s is a scale that the write stores for a finite vector (every code times it is finite).
+template <typename T, int F> __device__ __forceinline__ bool valid_scale(float s) { return fabsf(s) <= scale_cap<T, F>(); }
+
 // Scale of a head vector whose largest magnitude has the bits `amax` (NaN and infinities compare
 // above every finite value).
 template <typename T, int F>
@@ -57,24 +60,38 @@ __device__ __forceinline__ float scale_of(uint32_t amax) {
     return fminf(scale_up<T>(__fdiv_rn(__uint_as_float(amax), top_code<F>())), scale_cap<T, F>());
 }
 
-// Codes of 8 values as 8 bytes. s = 0 or NaN: codes 0.
-template <int F>
-__device__ __forceinline__ uint2 encode8(const float* x, float s) {
-    const bool zero = !(s > 0.f);
+// Codes of 8 values as 8 bytes. s = 0 or NaN: codes 0. x / s is taken as x times the rounded 1 / s, off
+// by at most 2^-22 relative (1.5e-5 of a code). kExact (x of T): such a quotient of two numbers of T
+// that is not half way between two codes is farther from there than 2.4e-4 of a code (int8; the
+// numerator of the difference is a whole multiple of the smaller unit) or 2^-16 relative (e4m3), so
+// rounding it first to a multiple of 2^-13, or to 18 bits, puts the half-way cases, and only those,
+// exactly half way, and the nearest-even rounding that follows is that of the true quotient. Divisions
+// took half of this kernel's instructions.
+template <int F, bool kExact>
+__device__ __forceinline__ uint2 encode8(const float* x, float s, bool capped) {
+    const float r = s > 0.f ? __frcp_rn(s) : 0.f;
     float y[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = zero ? 0.f : __fdiv_rn(x[e], s);
+    for (int e = 0; e < 8; ++e) y[e] = s > 0.f ? x[e] * r : 0.f;
     uint32_t w[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if (F == kInt8) {
-            int32_t c[4];
+            // in 1.5 * 2^23 + y the low byte of the bits is y's whole number, two's complement
+            uint32_t c[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) c[e] = min(127, max(-127, __float2int_rn(y[4 * h + e])));
-            const uint32_t lo = __byte_perm((uint32_t)c[0], (uint32_t)c[1], 0x0040);
-            const uint32_t hi = __byte_perm((uint32_t)c[2], (uint32_t)c[3], 0x0040);
-            w[h] = __byte_perm(lo, hi, 0x5410);
+            for (int e = 0; e < 4; ++e) {
+                float v = y[4 * h + e];
+                if (capped) v = fminf(fmaxf(v, -127.f), 127.f);
+                if (kExact) v = __fadd_rn(__fadd_rn(v, 1536.f), -1536.f);
+                c[e] = __float_as_uint(__fadd_rn(v, 12582912.f));
+            }
+            w[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
         } else {
+            if (kExact) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[4 * h + e] = __uint_as_float((__float_as_uint(y[4 * h + e]) + 0x20u) & ~0x3fu);
+            }
             const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h], y[4 * h + 1]), __NV_SATFINITE, __NV_E4M3);
             const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h + 2], y[4 * h + 3]), __NV_SATFINITE, __NV_E4M3);
             w[h] = lo | (hi << 16);
@@ -165,25 +182,25 @@ struct SmallScaleDecoder {
         return bits(__hmul2(as_bf(Decoder<__nv_bfloat16, kE4m3>::fields(w, a, b)), s));
     }
 };
-// Byte a of wa and byte b of wb, codes alone: exact up to the factor 1 / code_scale().
+// Codes alone, exact up to the factor 1 / code_scale(): as Decoder with s = 1.
 template <typename T, int F> __device__ __forceinline__ constexpr float code_scale() {
     return (F == kE4m3 && StoreT<T>::kUmmaFormat == 0) ? 256.f : 1.f;
 }
-template <typename T, int F>
-__device__ __forceinline__ uint32_t decode2(uint32_t wa, uint32_t wb, int a, int b) {
+template <int F> __device__ __forceinline__ uint32_t code_word(uint32_t w) { return F == kInt8 ? w ^ 0x80808080u : w; }
+template <typename T, int F> __device__ __forceinline__ uint32_t code_pair(uint32_t w, int a, int b) {
+    constexpr bool bf16 = StoreT<T>::kUmmaFormat == 1;
     if constexpr (F == kInt8) {
-        const uint32_t u = __byte_perm(wa, wb, (uint32_t)(a | ((4 + b) << 8)));
-        if constexpr (StoreT<T>::kUmmaFormat == 1)
-            // 0x4300 | low 7 bits is 128 + low7, 0x4300 | sign bit is 128 or 256
-            return bits(__hsub2(as_bf((u & 0x007f007fu) | 0x43004300u), as_bf((u & 0x00800080u) | 0x43004300u)));
-        else
-            return bits(__hsub2(as_h((u & 0x00ff00ffu) ^ 0x64806480u), as_h(0x64806480u)));
+        const uint32_t u = __byte_perm(w, bf16 ? 0x42424242u : 0x64646464u, (uint32_t)(a | 0x40 | (b << 8) | 0x4000));
+        if constexpr (bf16) {
+            const __nv_bfloat162 t = __hfma2(as_bf(u), as_bf(0x40004000u), as_bf(0xc300c300u));
+            return bits(__hsub2(t, __hfma2_relu(as_bf(u), as_bf(0xc000c000u), as_bf(0x43004300u))));
+        } else {
+            return bits(__hsub2(as_h(u), as_h(0x64806480u)));
+        }
     } else {
-        const uint32_t u = __byte_perm(wa, wb, (uint32_t)((a << 4) | ((4 + b) << 12)));
-        if constexpr (StoreT<T>::kUmmaFormat == 1)
-            return mul2<T>(((u >> 4) & 0x07f007f0u) | (u & 0x80008000u), 0x7b807b80u);
-        else
-            return ((u >> 1) & 0x3f803f80u) | (u & 0x80008000u);
+        const uint32_t u = __byte_perm(w, 0u, (uint32_t)(a | (a << 4) | (b << 8) | (b << 12)));
+        if constexpr (bf16) return mul2<T>(((u << 4) & 0x07f007f0u) | (u & 0x80008000u), 0x7b807b80u);
+        else return ((u << 7) & 0x3f803f80u) | (u & 0x80008000u);
     }
 }
 
@@ -254,7 +271,7 @@ __device__ __forceinline__ void norm_rope8(const uint4& x, const float2* w2, flo
 }
 
 // Quantises a half-warp's head vector (8 values per lane) and stores its codes and scale.
-template <typename T, int F>
+template <typename T, int F, bool kExact>
 __device__ __forceinline__ void quantise_store(const float* y, uint8_t* codes, T* scale, int sub, bool active) {
     uint32_t amax = 0;
 #pragma unroll
@@ -262,7 +279,18 @@ __device__ __forceinline__ void quantise_store(const float* y, uint8_t* codes, T
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     const float s = scale_of<T, F>(amax);
-    const uint2 w = encode8<F>(y, s);
+    // (__frcp_rn overflows below 2^-126: such scales, and capped ones, are brought into range exactly)
+    const bool capped = s >= scale_cap<T, F>(), tiny = s < 0x1p-100f;
+    uint2 w;
+    if (__any_sync(0xffffffffu, capped || tiny)) {
+        const float up = tiny ? 0x1p+100f : 1.f;
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = y[e] * up;
+        w = encode8<F, kExact>(z, s * up, true);
+    } else {
+        w = encode8<F, kExact>(y, s, false);
+    }
     if (active) {
         *reinterpret_cast<uint2*>(codes + 8 * sub) = w;
         if (sub == 0) {
@@ -281,7 +309,7 @@ constexpr int kWriteWarps = kWriteThreads / 32;
 // warps, as many as give every warp of the grid work (a few rows: one head pair per warp).
 // Bound by memory: 3 rows of T read, one of T and two of bytes written, per token.
 template <typename T, int F, bool kRaw>
-__global__ void __launch_bounds__(kWriteThreads) q8_write_kernel(const __grid_constant__ WriteArgs a) {
+__global__ void __launch_bounds__(kWriteThreads, 3) q8_write_kernel(const __grid_constant__ WriteArgs a) {
     const int lane = threadIdx.x & 31, sub = lane & 15, half = lane >> 4;
     const int32_t warp = blockIdx.x * kWriteWarps + (threadIdx.x >> 5), warps = gridDim.x * kWriteWarps;
     float2 turns[4];
@@ -324,15 +352,21 @@ __global__ void __launch_bounds__(kWriteThreads) q8_write_kernel(const __grid_co
                 rope_turn(at, turns[t], &sn[t], &cs[t]);
             }
         }
+        uint4 nq, nk, nv;      // the next head pair's vectors are on their way while one is worked on
+        auto load = [&](int32_t pr) {
+            const int32_t h = 2 * pr + half;
+            const int64_t at = (int64_t)i * a.ld_qkv + (int64_t)(h < a.n_heads ? h : 0) * kHeadDim + 8 * sub;
+            if (!kRaw) nq = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at));
+            nk = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.k) + at));
+            nv = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + at));
+        };
+        load(part);
         for (int32_t pr = part; pr < pairs; pr += parts) {
             const int32_t h = 2 * pr + half;
             const bool active = h < a.n_heads;
             const int64_t col = (int64_t)(active ? h : 0) * kHeadDim + 8 * sub;
-            const int64_t at = (int64_t)i * a.ld_qkv + col;
-            uint4 xq;
-            if (!kRaw) xq = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at));
-            const uint4 xk = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.k) + at));
-            const uint4 xv = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + at));
+            const uint4 xq = nq, xk = nk, xv = nv;
+            if (pr + parts < pairs) load(pr + parts);
             uint8_t* ck = a.c.k + (int64_t)i * a.c.ld + (col - 8 * sub);
             uint8_t* cv = a.c.v + (int64_t)i * a.c.ld + (col - 8 * sub);
             T* ks = static_cast<T*>(a.c.ks) + (int64_t)(active ? h : 0) * a.c.ld_scale + i;
@@ -366,7 +400,7 @@ __global__ void __launch_bounds__(kWriteThreads) q8_write_kernel(const __grid_co
                     y[2 * t + 1] = p.y;
                 }
             }
-            quantise_store<T, F>(y, ck, ks, sub, active);
+            quantise_store<T, F, kRaw>(y, ck, ks, sub, active);
             const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
@@ -374,7 +408,7 @@ __global__ void __launch_bounds__(kWriteThreads) q8_write_kernel(const __grid_co
                 y[2 * t] = p.x;
                 y[2 * t + 1] = p.y;
             }
-            quantise_store<T, F>(y, cv, vs, sub, active);
+            quantise_store<T, F, true>(y, cv, vs, sub, active);
         }
     }
 }
@@ -399,10 +433,12 @@ __global__ void __launch_bounds__(kReadThreads) q8_read_kernel(const __grid_cons
     pdl_launch_dependents();
     pdl_wait();
     const int32_t m_all = min(a.count ? *a.count : a.host_count, a.n_rows);
-    const int32_t per_row = a.n_heads * (kHeadDim / 16);   // 16-code chunks of a row
+    const uint32_t per_row = (uint32_t)a.n_heads * (kHeadDim / 16);   // 16-code chunks of a row
     const int64_t total = (int64_t)m_all * per_row;
+    const bool small = total <= 0xffffffffll;         // 32-bit divisions
     for (int64_t e = (int64_t)blockIdx.x * kReadThreads + threadIdx.x; e < total; e += (int64_t)gridDim.x * kReadThreads) {
-        const int32_t m = (int32_t)(e / per_row), c = (int32_t)(e - (int64_t)m * per_row);
+        const int32_t m = small ? (int32_t)((uint32_t)e / per_row) : (int32_t)(e / per_row);
+        const int32_t c = (int32_t)(e - (int64_t)m * per_row);
         const int32_t i = a.idx ? a.idx[m] : m;
         if (i < 0 || i >= a.n_rows) {
             if (c == 0) atomicOr(&g_error_word, kErrBounds);

@@ -37,6 +37,38 @@ int64_t q8_save_bytes(const fxr_frame_desc* d) {
     return (int64_t)align_up((size_t)d->n_heads * ((size_t)d->head_dim * 2 + 4), 16);
 }
 
+// Revolutions per position of each rotary pair. 64 powers cost as much as a launch, so a thread keeps
+// the table of the last axes and theta it was asked for.
+void fill_turns(const fxr_frame_desc* d, fxr::q8::WriteArgs* a) {
+    struct Table {
+        int32_t n_axes = -1;
+        int32_t dims[4];
+        float theta;
+        float2 turns[fxr::kPairs];
+        int8_t axis[fxr::kPairs];
+    };
+    static thread_local Table t;
+    bool same = t.n_axes == d->rope_n_axes && t.theta == d->rope_theta;
+    for (int x = 0; same && x < d->rope_n_axes; ++x) same = t.dims[x] == d->rope_axes_dim[x];
+    if (!same) {
+        std::memset(t.turns, 0, sizeof(t.turns));
+        std::memset(t.axis, 0, sizeof(t.axis));
+        for (int x = 0, j = 0; x < d->rope_n_axes; ++x) {
+            t.dims[x] = d->rope_axes_dim[x];
+            for (int jj = 0; jj < d->rope_axes_dim[x] / 2; ++jj, ++j) {
+                const double w = std::pow((double)d->rope_theta, -2.0 * jj / d->rope_axes_dim[x]) / 6.283185307179586;
+                const float hi = (float)w;
+                t.turns[j] = make_float2(hi, (float)(w - (double)hi));
+                t.axis[j] = (int8_t)x;
+            }
+        }
+        t.n_axes = d->rope_n_axes;
+        t.theta = d->rope_theta;
+    }
+    std::memcpy(a->turns, t.turns, sizeof(t.turns));
+    std::memcpy(a->axis, t.axis, sizeof(t.axis));
+}
+
 int32_t launch_q8_write(const fxr_frame_desc* d, const fxr_q8_cache* cache, fxr::q8::WriteArgs a, bool raw, int64_t max_rows,
                         cudaStream_t s) {
     NvtxRange nvtx_("fxr:q8_write");
@@ -46,18 +78,10 @@ int32_t launch_q8_write(const fxr_frame_desc* d, const fxr_q8_cache* cache, fxr:
     a.n_axes = d->rope_n_axes;
     a.eps = d->eps;
     a.ld_save = q8_save_bytes(d);
-    for (int j = 0; j < fxr::kPairs; ++j) a.turns[j] = make_float2(0.f, 0.f);
-    for (int x = 0, j = 0; x < d->rope_n_axes; ++x) {
-        for (int jj = 0; jj < d->rope_axes_dim[x] / 2; ++jj, ++j) {
-            const double w = std::pow((double)d->rope_theta, -2.0 * jj / d->rope_axes_dim[x]) / 6.283185307179586;
-            const float hi = (float)w;
-            a.turns[j] = make_float2(hi, (float)(w - (double)hi));
-            a.axis[j] = (int8_t)x;
-        }
-    }
+    fill_turns(d, &a);
     const int64_t units = max_rows * ((d->n_heads + 1) / 2);
     const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((units + fxr::q8::kWriteWarps - 1) / fxr::q8::kWriteWarps,
-                                                                (int64_t)sm_count() * 4));
+                                                                (int64_t)sm_count() * 3));
     return q8_dispatch(d->dtype, cache->format, [&](auto t, auto f) -> int32_t {
         using T = decltype(t);
         constexpr int F = decltype(f)::value;
@@ -68,7 +92,7 @@ int32_t launch_q8_write(const fxr_frame_desc* d, const fxr_q8_cache* cache, fxr:
 }
 
 // Streams of at most this many rows take the kernel for few rows.
-constexpr int32_t kQ8RowsLimit = 64;
+constexpr int32_t kQ8RowsLimit = fxr::attn8::kMaxRowsPerStream;
 
 // Workspace of the attention: arrivals (zero before and after a call), then partial results, then the
 // visible steps of the kernel for many rows.
@@ -80,7 +104,9 @@ struct Q8Work {
     uint32_t* groups;
     int32_t rows;         // bound of a stream's rows
     bool few;             // the kernel for few rows
-    int32_t slots;        // its partial results
+    bool one_tile;        // it takes groups of 8 rows, not of 16
+    int64_t line;         // bound of its work line
+    int32_t slots;        // its partial results: one per column and CTA boundary
     int32_t units;        // 256-row units of a stream, key tiles: the kernel for many
     int32_t n_pre, n_own;
     size_t zero_bytes;    // from the start: what has to be zero before a launch
@@ -101,12 +127,15 @@ Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, in
     };
     // one place and size for the arrivals of either kernel: calls with other bounds may share a workspace
     const size_t ctas = (size_t)sm_count();
-    w.cnt = reinterpret_cast<int32_t*>(take(std::max(ctas * fxr::attn8::kPartWarps, (size_t)d->n_heads) * sizeof(int32_t)));
+    w.cnt = reinterpret_cast<int32_t*>(take(std::max(ctas * fxr::attn8::kPartWarps,
+                                                     (size_t)d->n_heads * FXR_MAX_BATCH * fxr::attn8::kGroupsPerStream) * sizeof(int32_t)));
     w.zero_bytes = off;
     if (w.few) {
-        const int64_t tile = fxr::attn8::kRowsTile;
+        const int64_t tile = S * R <= 8 ? 8 : 16;    // rows of a group
+        w.one_tile = tile == 8;
         const int64_t groups = (n_prefix > 0 ? (S * R + tile - 1) / tile : 0) + S * ((R + tile - 1) / tile);
         w.slots = (int32_t)std::min<int64_t>(INT32_MAX, sm_count() + groups * d->n_heads);
+        w.line = groups * d->n_heads * ((std::max(n_prefix, d->n_tokens) + fxr::attn8::kUnitKeys - 1) / fxr::attn8::kUnitKeys);
         w.part = reinterpret_cast<float*>(take((size_t)w.slots * fxr::attn8::kRowsSlotFloats * sizeof(float)));
     } else {
         w.units = (w.rows + fxr::attn8::kUnitRows - 1) / fxr::attn8::kUnitRows;
@@ -121,36 +150,48 @@ Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, in
     return w;
 }
 
-template <typename T, int F>
-int32_t launch_q8_rows(const fxr::attn8::Params& p, cudaStream_t s) {
-    static bool configured[kMaxDevices] = {false};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= kMaxDevices) return fail(FXR_ERR_CUDA, "device %d", dev);
-    if (!configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(fxr::attn8::rows_kernel<T, F>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (int)fxr::attn8::kRowsSmem);
-        if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(rows_kernel)");
-        configured[dev] = true;
-    }
-    return cuda_status(launch_pdl(fxr::attn8::rows_kernel<T, F>, dim3(sm_count()), dim3(fxr::attn8::kRowsThreads),
-                                  fxr::attn8::kRowsSmem, s, p),
-                       "rows_kernel launch");
-}
-
-// 2-D map over rows of 8-bit codes: boxes of 128 rows x 128 bytes (a head), 128-byte swizzle.
-int32_t make_code_tmap(CUtensorMap* map, const void* ptr, int64_t cols, int64_t rows, int64_t ld) {
+// 2-D map over rows of 8-bit codes: boxes of `box_rows` rows x 128 bytes (a head), 128-byte swizzle.
+int32_t make_code_tmap(CUtensorMap* map, const void* ptr, int64_t cols, int64_t rows, int64_t ld, uint32_t box_rows) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return fail(FXR_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)ld};
-    const cuuint32_t box[2] = {(cuuint32_t)fxr::attn8::kD, (cuuint32_t)fxr::attn8::kBN};
+    const cuuint32_t box[2] = {(cuuint32_t)fxr::attn8::kD, box_rows};
     const cuuint32_t estr[2] = {1, 1};
     const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(FXR_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return FXR_OK;
+}
+
+template <typename T, int F, int NQ>
+int32_t launch_q8_rows(const fxr_frame_desc* d, const fxr::attn8::Params& p, cudaStream_t s) {
+    static bool configured[kMaxDevices] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= kMaxDevices) return fail(FXR_ERR_CUDA, "device %d", dev);
+    if (!configured[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(fxr::attn8::rows_kernel<T, F, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)fxr::attn8::kRowsSmem);
+        if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(rows_kernel)");
+        configured[dev] = true;
+    }
+    const int64_t C = (int64_t)d->n_heads * d->head_dim;
+    fxr::attn8::RowsMaps maps;
+    std::memset(&maps, 0, sizeof(maps));
+    int32_t rc;
+    for (int32_t b = 0; b < p.n_streams; ++b) {
+        if ((rc = make_code_tmap(&maps.k[b], p.s[b].c.k, C, p.n_tokens, p.s[b].c.ld, fxr::attn8::kBlk)) != FXR_OK) return rc;
+        if ((rc = make_code_tmap(&maps.v[b], p.s[b].c.v, C, p.n_tokens, p.s[b].c.ld, fxr::attn8::kBlk)) != FXR_OK) return rc;
+    }
+    if (p.n_prefix > 0) {
+        if ((rc = make_code_tmap(&maps.pk, p.prefix.k, C, p.n_prefix, p.prefix.ld, fxr::attn8::kBlk)) != FXR_OK) return rc;
+        if ((rc = make_code_tmap(&maps.pv, p.prefix.v, C, p.n_prefix, p.prefix.ld, fxr::attn8::kBlk)) != FXR_OK) return rc;
+    }
+    return cuda_status(launch_pdl(fxr::attn8::rows_kernel<T, F, NQ>, dim3(sm_count()), dim3(fxr::attn8::kRowsThreads),
+                                  fxr::attn8::kRowsSmem, s, maps, p),
+                       "rows_kernel launch");
 }
 
 template <typename T, int F>
@@ -177,13 +218,13 @@ int32_t launch_q8_tiles(const fxr_frame_desc* d, const fxr::attn8::Params& p, co
     bool groups = p.pg != nullptr && p.n_prefix > 0;
     for (int32_t b = 0; b < p.n_streams; ++b) {
         if ((rc = make_tmap(&maps.q[b], p.s[b].qc, d->dtype, C, p.max_rows, p.s[b].ld_qc)) != FXR_OK) return rc;
-        if ((rc = make_code_tmap(&maps.k[b], p.s[b].c.k, C, p.n_tokens, p.s[b].c.ld)) != FXR_OK) return rc;
-        if ((rc = make_code_tmap(&maps.v[b], p.s[b].c.v, C, p.n_tokens, p.s[b].c.ld)) != FXR_OK) return rc;
+        if ((rc = make_code_tmap(&maps.k[b], p.s[b].c.k, C, p.n_tokens, p.s[b].c.ld, fxr::attn8::kBN)) != FXR_OK) return rc;
+        if ((rc = make_code_tmap(&maps.v[b], p.s[b].c.v, C, p.n_tokens, p.s[b].c.ld, fxr::attn8::kBN)) != FXR_OK) return rc;
         groups = groups || p.s[b].qg != nullptr || p.s[b].kg != nullptr;
     }
     if (p.n_prefix > 0) {
-        if ((rc = make_code_tmap(&maps.pk, p.prefix.k, C, p.n_prefix, p.prefix.ld)) != FXR_OK) return rc;
-        if ((rc = make_code_tmap(&maps.pv, p.prefix.v, C, p.n_prefix, p.prefix.ld)) != FXR_OK) return rc;
+        if ((rc = make_code_tmap(&maps.pk, p.prefix.k, C, p.n_prefix, p.prefix.ld, fxr::attn8::kBN)) != FXR_OK) return rc;
+        if ((rc = make_code_tmap(&maps.pv, p.prefix.v, C, p.n_prefix, p.prefix.ld, fxr::attn8::kBN)) != FXR_OK) return rc;
     }
     fxr::attn8::TileParams a{};
     a.p = p;
@@ -343,6 +384,7 @@ int32_t fxr_attention_q8(const fxr_frame_desc* desc, int32_t n_streams, const fx
     if (!workspace) return fail(FXR_ERR_INVALID, "null workspace");
     if (!aligned16(workspace)) return fail(FXR_ERR_INVALID, "workspace must be 16-byte aligned");
     if (workspace_bytes < w.total) return fail(FXR_ERR_WORKSPACE, "workspace %zu < required %zu", workspace_bytes, w.total);
+    if (w.few && w.line >= INT32_MAX) return fail(FXR_ERR_UNSUPPORTED, "too many keys x heads x row groups for one call (%lld)", (long long)w.line);
     if (!w.few && w.n_pre + w.n_own > 0x7fff)
         return fail(FXR_ERR_UNSUPPORTED, "%d key rows: more than 32767 tiles of 128", n_prefix + desc->n_tokens);
     for (int32_t b0 = 0; b0 < n_streams; b0 += FXR_MAX_BATCH) {
@@ -365,8 +407,9 @@ int32_t fxr_attention_q8(const fxr_frame_desc* desc, int32_t n_streams, const fx
         st = q8_dispatch(desc->dtype, streams[0].cache.format, [&](auto t, auto f) -> int32_t {
             using T = decltype(t);
             constexpr int F = decltype(f)::value;
-            return w.few ? launch_q8_rows<T, F>(p, static_cast<cudaStream_t>(stream))
-                         : launch_q8_tiles<T, F>(desc, p, w, static_cast<cudaStream_t>(stream));
+            const cudaStream_t cs = static_cast<cudaStream_t>(stream);
+            if (!w.few) return launch_q8_tiles<T, F>(desc, p, w, cs);
+            return w.one_tile ? launch_q8_rows<T, F, 1>(desc, p, cs) : launch_q8_rows<T, F, 2>(desc, p, cs);
         });
         if (st != FXR_OK) return st;
     }

@@ -342,6 +342,16 @@ class FrameConfig:
     ld_cache: int = 0
     ld_out: int = 0
 
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_ref", None)
+
+    def ref(self):
+        """A ctypes reference to desc(), built once until a field changes (for calls of a few microseconds)."""
+        if self._ref is None:
+            object.__setattr__(self, "_ref", ctypes.byref(self.desc()))
+        return self._ref
+
     def desc(self) -> FrameDesc:
         d = FrameDesc()
         C = self.n_heads * self.head_dim
@@ -761,13 +771,21 @@ def _refuse(msg: str):
     raise FxrError(FXR_ERR_INVALID, msg)
 
 
-def _here(*tensors):
-    """Refuses tensors of another device than the current one, whose stream the call would use."""
+def _raw_stream(device: int, stream=None) -> int:
+    """The cudaStream_t of `stream` or of the current stream of `device`, the current device. These
+    calls take a few microseconds on the GPU, so the handle is asked for without a Stream object."""
     import torch
-    at = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != at:
-            _refuse(f"tensor on {t.device}, the current device is cuda:{at}")
+    if torch._C._cuda_getDevice() != device:
+        _refuse(f"tensor on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
+
+
+def _device_of(*tensors):
+    """The one device of the tensors (None entries apart)."""
+    at = {t.device for t in tensors if t is not None}
+    if len(at) != 1 or next(iter(at)).type != "cuda":
+        _refuse(f"tensors on one CUDA device: got {sorted(map(str, at))}")
+    return next(iter(at)).index
 
 
 def _groups(t, rows: int, what: str):
@@ -796,12 +814,14 @@ class CacheQ8:
         if len({t.device for t in (k, v, k_scale, v_scale)}) > 1:
             _refuse("codes and scales on one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device, self.dtype = k.device.index, {torch.bfloat16: "bf16", torch.float16: "f16"}[k_scale.dtype]
         self.n_rows, self.n_heads = k.shape[0], k_scale.shape[0]
         # a single row or head has no stride of its own
         ld = k.stride(0) if k.shape[0] > 1 else max(k.stride(0), k.shape[1])
         ld_scale = k_scale.stride(0) if k_scale.shape[0] > 1 else k_scale.shape[1] // 8 * 8
         self.struct = Q8CacheStruct(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), ld, ld_scale, k.shape[0],
                                     formats[k.dtype])
+        self.ref = ctypes.byref(self.struct)
 
     @classmethod
     def empty(cls, cfg: FrameConfig, n_rows: int | None = None, fmt: str = "int8", device="cuda") -> "CacheQ8":
@@ -815,57 +835,51 @@ class CacheQ8:
         return cls(*kv, *sc)
 
     def check(self, cfg: FrameConfig, rows: int, what: str = "cache"):
-        import torch
-        if self.n_heads < cfg.n_heads or self.n_rows < rows or \
-                self.k_scale.dtype != {"bf16": torch.bfloat16, "f16": torch.float16}.get(cfg.dtype):
-            _refuse(f"{what}: {self.n_rows} rows, {self.n_heads} heads, {self.k_scale.dtype} scales for a frame of "
-                    f"{rows} rows, {cfg.n_heads} heads, {cfg.dtype}")
-        _here(self.k)
+        if self.n_heads < cfg.n_heads or self.n_rows < rows or self.dtype != cfg.dtype:
+            _refuse(f"{what}: {self.n_rows} rows, {self.n_heads} heads, {self.dtype} scales for a frame of {rows} rows, "
+                    f"{cfg.n_heads} heads, {cfg.dtype}")
 
 
 def q8_save_row_bytes(cfg: FrameConfig) -> int:
-    return int(load().fxr_q8_save_row_bytes(ctypes.byref(cfg.desc())))
+    return int(load().fxr_q8_save_row_bytes(cfg.ref()))
 
 
 def gather_norm_rope_q8(cfg: FrameConfig, q, k, v, mask, idx, count, pos, norm_q, norm_k, qc, cache: CacheQ8,
                         save=None, stream=None):
     """gather_norm_rope into an 8-bit cache (fxr_gather_norm_rope_q8). save: uint8 [N, q8_save_row_bytes(cfg)]."""
-    d = cfg.desc()
     cache.check(cfg, cfg.n_tokens)
-    _check(load().fxr_gather_norm_rope_q8(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(mask), _ptr(idx),
-                                          _ptr(count), _ptr(pos), _ptr(norm_q), _ptr(norm_k), _ptr(qc), qc.stride(0),
-                                          ctypes.byref(cache.struct), _ptr(save), _stream(stream)))
+    _check(load().fxr_gather_norm_rope_q8(cfg.ref(), q.data_ptr(), k.data_ptr(), v.data_ptr(), mask.data_ptr(),
+                                          idx.data_ptr(), count.data_ptr(), _ptr(pos), norm_q.data_ptr(),
+                                          norm_k.data_ptr(), qc.data_ptr(), qc.stride(0), cache.ref, _ptr(save),
+                                          _raw_stream(cache.device, stream)))
 
 
 def cache_write_q8(cfg: FrameConfig, cache_k, cache_v, cache: CacheQ8, idx=None, count=None, host_count: int = -1,
                    stream=None):
     """Rows of a 16-bit cache (row stride cfg.ld_cache) into an 8-bit one, listed by idx / count or, by
     default, all of the frame's tokens."""
-    d = cfg.desc()
     cache.check(cfg, cfg.n_tokens)
     if idx is None and count is None and host_count < 0:
         host_count = cfg.n_tokens
-    _check(load().fxr_cache_write_q8(ctypes.byref(d), _ptr(cache_k), _ptr(cache_v), _ptr(idx), _ptr(count), host_count,
-                                     ctypes.byref(cache.struct), _stream(stream)))
+    _check(load().fxr_cache_write_q8(cfg.ref(), _ptr(cache_k), _ptr(cache_v), _ptr(idx), _ptr(count), host_count,
+                                     cache.ref, _raw_stream(cache.device, stream)))
 
 
 def cache_read_q8(cfg: FrameConfig, cache: CacheQ8, k, v, idx=None, count=None, host_count: int = -1, stream=None):
     """Cache rows back in the frame's type: k[m], v[m] = row idx[m], or by default every row of the cache."""
-    d = cfg.desc()
     cache.check(cfg, 0)
     if k.stride() != v.stride():
         _refuse("k and v: one row stride")
     if idx is None and count is None and host_count < 0:
         host_count = cache.n_rows
-    _check(load().fxr_cache_read_q8(ctypes.byref(d), ctypes.byref(cache.struct), _ptr(idx), _ptr(count), host_count,
-                                    _ptr(k), _ptr(v), k.stride(0), _stream(stream)))
+    _check(load().fxr_cache_read_q8(cfg.ref(), cache.ref, _ptr(idx), _ptr(count), host_count, k.data_ptr(),
+                                    v.data_ptr(), k.stride(0), _raw_stream(cache.device, stream)))
 
 
 def restore_rows_q8(cfg: FrameConfig, mask, idx, count, save, cache: CacheQ8, stream=None):
-    d = cfg.desc()
     cache.check(cfg, cfg.n_tokens)
-    _check(load().fxr_restore_rows_q8(ctypes.byref(d), _ptr(mask), _ptr(idx), _ptr(count), _ptr(save),
-                                      ctypes.byref(cache.struct), _stream(stream)))
+    _check(load().fxr_restore_rows_q8(cfg.ref(), _ptr(mask), _ptr(idx), _ptr(count), _ptr(save), cache.ref,
+                                      _raw_stream(cache.device, stream)))
 
 
 class Q8Streams:
@@ -875,33 +889,40 @@ class Q8Streams:
         self.streams = streams                  # keeps the tensors alive
         self.array = (Q8StreamStruct * max(len(streams), 1))()
         for b, f in enumerate(streams):
-            self.array[b] = Q8StreamStruct(_ptr(f["qc"]), f["qc"].stride(0) if f["qc"].shape[0] > 1 else f["qc"].shape[1],
-                                           _ptr(f["idx"]), _ptr(f["count"]), _ptr(f["out"]), _ptr(f.get("q_groups")),
-                                           _ptr(f.get("k_groups")), f["cache"].struct)
+            qc, out, cache = f["qc"], f["out"], f["cache"]
+            if qc.dtype != cache.k_scale.dtype or out.dtype != qc.dtype:
+                _refuse("qc, out and the scales are of one type")
+            self.array[b] = Q8StreamStruct(_ptr(qc), qc.stride(0) if qc.shape[0] > 1 else qc.shape[1], _ptr(f["idx"]),
+                                           _ptr(f["count"]), _ptr(out), _ptr(f.get("q_groups")),
+                                           _ptr(f.get("k_groups")), cache.struct)
+        self.rows = min((f["qc"].shape[0] for f in streams), default=0)
+        self.tokens = min((f["out"].shape[0] for f in streams), default=0)
 
     def check(self, cfg: FrameConfig, max_rows: int = 0):
         n = cfg.n_tokens
         rows = min(max_rows, n) if max_rows > 0 else n
+        if self.rows < rows:
+            _refuse(f"qc holds {self.rows} rows, the bound is {rows}")
+        if self.tokens < n:
+            _refuse(f"out holds {self.tokens} rows, the frame has {n} tokens")
         for f in self.streams:
-            if f["qc"].shape[0] < rows:
-                _refuse(f"qc holds {f['qc'].shape[0]} rows, the bound is {rows}")
             f["cache"].check(cfg, n, "stream cache")
             _groups(f.get("q_groups"), n, "q_groups")
             _groups(f.get("k_groups"), n, "k_groups")
-            if f["out"].dtype != f["cache"].k_scale.dtype or f["qc"].dtype != f["out"].dtype:
-                _refuse("qc, out and the scales are of one type")
-            _here(f["qc"], f["idx"], f["count"], f["out"], f.get("q_groups"), f.get("k_groups"))
 
 
 def q8_streams(streams) -> Q8Streams:
     """streams: list of dicts with qc, idx, count, out tensors, cache (CacheQ8) and, optionally, q_groups
     and k_groups (int32 or uint32 [N])."""
-    return Q8Streams(list(streams))
+    made = Q8Streams(list(streams))
+    if made.streams:
+        _device_of(*[f.get(n) for f in made.streams for n in ("qc", "idx", "count", "out", "q_groups", "k_groups")],
+                   *[f["cache"].k for f in made.streams])
+    return made
 
 
 def attention_q8_workspace_size(cfg: FrameConfig, n_streams: int = 1, n_prefix: int = 0, max_rows: int = 0) -> int:
-    d = cfg.desc()
-    return int(load().fxr_attention_q8_workspace_size(ctypes.byref(d), n_streams, n_prefix, max_rows))
+    return int(load().fxr_attention_q8_workspace_size(cfg.ref(), n_streams, n_prefix, max_rows))
 
 
 def attention_q8(cfg: FrameConfig, streams, workspace, prefix: CacheQ8 | None = None, prefix_groups=None,
@@ -909,41 +930,37 @@ def attention_q8(cfg: FrameConfig, streams, workspace, prefix: CacheQ8 | None = 
     """Attention of each stream's executed rows over the prefix and its own 8-bit cache
     (fxr_attention_q8). streams: a list of dicts as for q8_streams(), or what it returned. workspace: a
     zeroed uint8 tensor of attention_q8_workspace_size() bytes, reused as is."""
-    d = cfg.desc()
     if not isinstance(streams, Q8Streams):
         streams = q8_streams(streams)
     streams.check(cfg, max_rows)
     if prefix is not None:
         prefix.check(cfg, 0, "prefix")
         _groups(prefix_groups, prefix.n_rows, "prefix_groups")
-    _here(workspace)
-    _check(load().fxr_attention_q8(ctypes.byref(d), len(streams.streams), streams.array,
-                                   ctypes.byref(prefix.struct) if prefix is not None else None, _ptr(prefix_groups),
-                                   max_rows, _ptr(workspace), workspace.numel() * workspace.element_size(),
-                                   _stream(stream)))
+    _check(load().fxr_attention_q8(cfg.ref(), len(streams.streams), streams.array, prefix.ref if prefix is not None else None,
+                                   _ptr(prefix_groups), max_rows, workspace.data_ptr(),
+                                   workspace.numel() * workspace.element_size(),
+                                   _raw_stream(workspace.device.index, stream)))
 
 
 def frame_q8_workspace_size(cfg: FrameConfig, n_prefix: int = 0, max_rows: int = 0) -> int:
-    d = cfg.desc()
-    return int(load().fxr_frame_q8_workspace_size(ctypes.byref(d), n_prefix, max_rows))
+    return int(load().fxr_frame_q8_workspace_size(cfg.ref(), n_prefix, max_rows))
 
 
 def frame_forward_q8(cfg: FrameConfig, q, k, v, mask, valid, pos, norm_q, norm_k, cache: CacheQ8, out, workspace,
                      prefix: CacheQ8 | None = None, prefix_groups=None, q_groups=None, k_groups=None,
                      max_rows: int = 0, stream=None):
     """One frame over an 8-bit cache (fxr_frame_forward_q8)."""
-    d = cfg.desc()
     cache.check(cfg, cfg.n_tokens)
     _groups(q_groups, cfg.n_tokens, "q_groups")
     _groups(k_groups, cfg.n_tokens, "k_groups")
     if prefix is not None:
         prefix.check(cfg, 0, "prefix")
         _groups(prefix_groups, prefix.n_rows, "prefix_groups")
-    _check(load().fxr_frame_forward_q8(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(mask), _ptr(valid), _ptr(pos),
-                                       _ptr(norm_q), _ptr(norm_k), ctypes.byref(cache.struct), _ptr(q_groups),
-                                       _ptr(k_groups), ctypes.byref(prefix.struct) if prefix is not None else None,
-                                       _ptr(prefix_groups), max_rows, _ptr(out), _ptr(workspace),
-                                       workspace.numel() * workspace.element_size(), _stream(stream)))
+    _check(load().fxr_frame_forward_q8(cfg.ref(), _ptr(q), _ptr(k), _ptr(v), _ptr(mask), _ptr(valid), _ptr(pos),
+                                       _ptr(norm_q), _ptr(norm_k), cache.ref, _ptr(q_groups), _ptr(k_groups),
+                                       prefix.ref if prefix is not None else None, _ptr(prefix_groups), max_rows,
+                                       _ptr(out), _ptr(workspace), workspace.numel() * workspace.element_size(),
+                                       _raw_stream(cache.device, stream)))
 
 
 def qkv_project(cfg: FrameConfig, hidden, w_qkv, bias, idx, count, q, k, v, scratch=None,

@@ -271,6 +271,14 @@ def test_bad_arguments_are_refused(lib):
     assert lib.fxr_frame_forward_q8(d, *([4096] * 8), ctypes.byref(c), None, None, None, None, 0, 4096, 4096, 16, None) == fxr.FXR_ERR_WORKSPACE
 
 
+def test_a_configuration_s_reference_follows_its_fields():
+    cfg = cfg_of(8, 2, "bf16")
+    first = cfg.ref()
+    assert cfg.ref() is first and first._obj.n_tokens == 8
+    cfg.n_tokens = 9
+    assert cfg.ref()._obj.n_tokens == 9 and cfg.desc().n_tokens == 9
+
+
 def test_structs_match_the_header():
     assert ctypes.sizeof(fxr.Q8CacheStruct) == 4 * 8 + 2 * 8 + 2 * 4
     assert ctypes.sizeof(fxr.Q8StreamStruct) == 7 * 8 + 56 and fxr.Q8StreamStruct.cache.offset == 56
@@ -289,10 +297,20 @@ def test_binding_refuses_other_types():
     k = torch.zeros(16, 256, dtype=torch.int8)
     s = torch.zeros(2, 16, dtype=torch.bfloat16)
     fxr.CacheQ8(k, k.clone(), s, s.clone())
-    few = fxr.q8_streams([{"qc": torch.zeros(3, 256, dtype=torch.bfloat16), "idx": k, "count": k, "out": k,
-                           "cache": fxr.CacheQ8(k, k, s, s)}])
+    st = {"qc": torch.zeros(3, 256, dtype=torch.bfloat16), "idx": k, "count": k, "out": torch.zeros(16, 256, dtype=torch.bfloat16),
+          "cache": fxr.CacheQ8(k, k, s, s)}
     with pytest.raises(fxr.FxrError, match="qc holds 3 rows"):
-        few.check(cfg_of(16, 2, "bf16"), 4)
+        fxr.Q8Streams([st]).check(cfg_of(16, 2, "bf16"), 4)
+    with pytest.raises(fxr.FxrError, match="out holds 16 rows"):
+        fxr.Q8Streams([st]).check(cfg_of(17, 2, "bf16"), 3)
+    with pytest.raises(fxr.FxrError, match="16 rows, 2 heads"):
+        fxr.Q8Streams([st]).check(cfg_of(16, 3, "bf16"), 3)
+    with pytest.raises(fxr.FxrError, match="CUDA device"):
+        fxr.q8_streams([st])
+    with pytest.raises(fxr.FxrError, match="q_groups"):
+        fxr.Q8Streams([dict(st, q_groups=torch.zeros(15, dtype=torch.int32))]).check(cfg_of(16, 2, "bf16"), 3)
+    with pytest.raises(fxr.FxrError, match="one type"):
+        fxr.Q8Streams([dict(st, out=k)])
     for bad in ((k.float(), k, s, s), (k, k.view(torch.float8_e4m3fn), s, s), (k, k, s.float(), s.float()), (k, k, s, s.half()),
                 (k, k[:8], s, s), (k, k, s[:, :8], s[:, :8]), (k[:, :128], k[:, :128], s, s), (k.t(), k.t(), s, s)):
         with pytest.raises(fxr.FxrError):
