@@ -43,8 +43,12 @@ struct Params {
 // Few rows per stream: bound by reading the cache once. Work is laid on a line of columns, each the
 // keys of one source for one head and one group of 8 or 16 rows: first (head, group of the packed rows
 // of all streams) against the prefix, so that the prefix is read once for every 16 rows of all
-// streams, then (stream, head, group) against the stream's own rows. The line is cut into one range
-// per CTA in units of 64 keys; a range covers one to a few items (parts of columns).
+// streams, then (stream, head, group) against the stream's own rows. Where there are at least as many
+// CTAs as columns, every column is cut into parts of one length, the shortest (in units of 64 keys)
+// that gives every part a CTA of its own. Otherwise the line is cut into one range per CTA, and a range
+// covers a few items (parts of columns). An item costs its CTA about 6 us besides its keys (queries,
+// first copies, exchange, arrival: as long as 700 keys), so ranges that straddle columns are avoided
+// where they can be.
 // A CTA's 16 warps walk an item in blocks of 16 keys, each warp with its own running maximum, sum and
 // O, so that none waits for another. A warp streams its blocks through a ring of 3 in shared memory
 // by TMA (4 KB of codes per block: ~130 KB in flight per SM; one lane issues a block's copies, where
@@ -137,21 +141,22 @@ struct RowsPlan {
     int32_t total;               // rows of all streams
     int32_t gp, go;              // groups: packed rows (0 without a prefix), own
     int32_t up, uo;              // units of a prefix column, of an own column
-    int32_t per;                 // units per CTA
+    int32_t len;                 // units of a part, 0: the line is cut into ranges
+    int32_t np, no;              // parts of a prefix column, of an own column
+    int32_t per;                 // units of a CTA's range
     int32_t line;                // units in all (the host refuses calls of 2^31 or more)
 };
 
-// Column c of the line: its head, group and units; prefix columns first.
+// A column of the line, prefix columns first: its head, group and units.
 struct Column {
     int32_t head, group, stream, units, start;
 };
 
 template <int R>
-__device__ __forceinline__ Column column_at(const RowsPlan& r, int32_t n_heads, int32_t unit, int32_t& index) {
+__device__ __forceinline__ Column column(const RowsPlan& r, int32_t n_heads, int32_t index) {
     Column c;
-    const int32_t pre = n_heads * r.gp * r.up;
-    if (unit < pre) {
-        index = unit / r.up;
+    const int32_t pre = n_heads * r.gp;
+    if (index < pre) {
         c.head = index / r.gp;
         c.group = index - c.head * r.gp;
         c.stream = -1;
@@ -159,9 +164,8 @@ __device__ __forceinline__ Column column_at(const RowsPlan& r, int32_t n_heads, 
         c.start = index * r.up;
         return c;
     }
-    int32_t e = (unit - pre) / r.uo;
-    index = n_heads * r.gp + e;
-    c.start = pre + e * r.uo;
+    int32_t e = index - pre;
+    c.start = pre * r.up + e * r.uo;
     c.units = r.uo;
     c.stream = 0;
 #pragma unroll
@@ -178,10 +182,28 @@ __device__ __forceinline__ Column column_at(const RowsPlan& r, int32_t n_heads, 
     return c;
 }
 
-// CTAs [first, last] that hold the parts of a column.
-__device__ __forceinline__ void parts_of(const RowsPlan& r, int32_t start, int32_t units, int32_t& first, int32_t& last) {
-    first = start / r.per;
-    last = (start + units - 1) / r.per;
+// One item: keys [k0, k0 + n_keys) of a column. Kept in shared memory: across the step loop the warps
+// have no registers to spare.
+struct RowsItem {
+    int32_t head, group, stream, live;
+    int32_t k0, n_keys, slot;
+    int32_t at;                  // ranges: the next unit of the line
+};
+
+// The parts of column `index` are `n` consecutive scratch slots from `slot`. (Ranges: part c of column x,
+// the one that CTA c holds, is slot x + c, which grows along the line with every cut.)
+__device__ __forceinline__ void parts_of(const RowsPlan& r, int32_t n_heads, int32_t index, int32_t& slot, int32_t& n) {
+    const int32_t pre = n_heads * r.gp;
+    const bool is_pre = index < pre;
+    if (r.len > 0) {
+        slot = is_pre ? index * r.np : pre * r.np + (index - pre) * r.no;
+        n = is_pre ? r.np : r.no;
+    } else {
+        const int32_t start = is_pre ? index * r.up : pre * r.up + (index - pre) * r.uo;
+        const int32_t first = start / r.per;
+        slot = index + first;
+        n = (start + (is_pre ? r.up : r.uo) - 1) / r.per - first + 1;
+    }
 }
 
 // Own group (stream b, group g) of head h: every part of its rows, in key order, a row per warp.
@@ -199,21 +221,13 @@ __device__ __noinline__ void rows_combine(const Params& p, const RowsPlan& r, in
             out_base = p.s[k].out;
         }
     const int32_t i = idx[m];
-    // parts: the packed row's prefix column, then the own column; part c of column x is slot x + c
-    int32_t p0 = 0, n_pre = 0, pre_slot = 0;
+    // parts: the packed row's prefix column's, then the own column's
+    int32_t n_pre = 0, pre_slot = 0, own_slot, n;
     const int32_t pr = r.first[b] + m;
-    if (r.gp > 0) {
-        const int32_t col = h * r.gp + pr / R;
-        int32_t last;
-        parts_of(r, col * r.up, r.up, p0, last);
-        n_pre = last - p0 + 1;
-        pre_slot = col + p0;
-    }
+    if (r.gp > 0) parts_of(r, p.n_heads, h * r.gp + pr / R, pre_slot, n_pre);
     const int32_t groups = (r.rows[b] + R - 1) / R;
-    const int32_t own = p.n_heads * r.group0[b] + h * groups + g;
-    int32_t o0, o1;
-    parts_of(r, p.n_heads * r.gp * r.up + own * r.uo, r.uo, o0, o1);
-    const int32_t own_slot = p.n_heads * r.gp + own + o0, n = n_pre + o1 - o0 + 1;
+    parts_of(r, p.n_heads, p.n_heads * (r.gp + r.group0[b]) + h * groups + g, own_slot, n);
+    n += n_pre;
     auto slot = [&](int32_t c) {
         return p.part + (int64_t)(c < n_pre ? pre_slot + c : own_slot + c - n_pre) * kRowsSlotFloats;
     };
@@ -284,6 +298,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ RowsPlan r;
+    __shared__ RowsItem item;
     __shared__ int abort;
     __shared__ uint32_t ready;                 // own groups whose last part this CTA delivered
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -329,28 +344,70 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
             r.up = (p.n_prefix + kUnitKeys - 1) / kUnitKeys;
             r.uo = (p.n_tokens + kUnitKeys - 1) / kUnitKeys;
             r.line = p.n_heads * (r.gp * r.up + r.go * r.uo);
-            r.per = (r.line + (int32_t)gridDim.x - 1) / (int32_t)gridDim.x;
+            const int32_t grid = (int32_t)gridDim.x;
+            r.per = (r.line + grid - 1) / grid;
+            r.len = r.np = r.no = 0;
+            if (rows_to > 0 && p.n_heads * (r.gp + r.go) <= grid) {
+                r.len = r.per;       // from the length that would do without remainders
+                for (;; ++r.len) {
+                    r.np = (r.up + r.len - 1) / r.len;
+                    r.no = (r.uo + r.len - 1) / r.len;
+                    if (p.n_heads * (r.gp * r.np + r.go * r.no) <= grid) break;
+                }
+            }
         }
     }
     __syncthreads();
 
-    int32_t at = min((int64_t)r.line, (int64_t)blockIdx.x * r.per);
-    const int32_t end = min((int64_t)r.line, (int64_t)at + r.per);
-    while (at < end) {
-        // ---- the item: the part [u0, u0 + n) of a column
-        int32_t col;
-        const Column cl = column_at<R>(r, p.n_heads, at, col);
-        const int32_t u0 = at - cl.start, n_units = min(cl.units - u0, end - at);
-        at += n_units;
-        const bool pre = cl.stream < 0;
-        const int32_t h = cl.head, n_src = pre ? p.n_prefix : p.n_tokens;
+    for (bool first = true;; first = false) {
+        if (threadIdx.x == 0) {
+            // ---- the item: units [u0, u0 + n) of a column
+            int32_t col = -1, u0 = 0, n = 0;
+            if (r.len > 0) {
+                const int32_t pre_items = p.n_heads * r.gp * r.np, e = (int32_t)blockIdx.x;
+                if (first && e < pre_items + p.n_heads * r.go * r.no) {
+                    col = e < pre_items ? e / r.np : p.n_heads * r.gp + (e - pre_items) / r.no;
+                    u0 = (e < pre_items ? e % r.np : (e - pre_items) % r.no) * r.len;
+                    n = r.len;
+                    item.slot = e;
+                }
+            } else {
+                const int32_t pre_units = p.n_heads * r.gp * r.up;
+                const int32_t begin = (int32_t)min((int64_t)r.line, (int64_t)blockIdx.x * r.per);
+                const int32_t end = (int32_t)min((int64_t)r.line, (int64_t)begin + r.per), at = first ? begin : item.at;
+                if (at < end) {
+                    col = at < pre_units ? at / r.up : p.n_heads * r.gp + (at - pre_units) / r.uo;
+                    u0 = at - (at < pre_units ? col * r.up : pre_units + (col - p.n_heads * r.gp) * r.uo);
+                    n = end - at;
+                    item.slot = col + (int32_t)blockIdx.x;
+                }
+                item.at = at;
+            }
+            item.n_keys = 0;
+            if (col >= 0) {
+                const Column cl = column<R>(r, p.n_heads, col);
+                n = min(n, cl.units - u0);
+                item.at += n;
+                item.head = cl.head;
+                item.group = cl.group;
+                item.stream = cl.stream;
+                item.live = min(R, (cl.stream < 0 ? r.total : r.rows[cl.stream]) - cl.group * R);
+                item.k0 = u0 * kUnitKeys;
+                item.n_keys = min(n * kUnitKeys, (cl.stream < 0 ? p.n_prefix : p.n_tokens) - item.k0);
+            }
+        }
+        __syncthreads();
+        const int32_t n_keys = item.n_keys, n_blk = (n_keys + kBlk - 1) / kBlk;
+        if (n_keys == 0) break;
+        const int32_t h = item.head, k0 = item.k0, stream = item.stream;
+        const bool pre = stream < 0;
         const void *ks0 = p.prefix.ks, *vs0 = p.prefix.vs;
         int64_t ld_scale = p.prefix.ld_scale;
         const uint32_t* kg = p.pg;
         const CUtensorMap *tk = &maps.pk, *tv = &maps.pv;
 #pragma unroll
         for (int k = 0; k < kMaxBatch; ++k)
-            if (k == cl.stream) {
+            if (k == stream) {
                 ks0 = p.s[k].c.ks;
                 vs0 = p.s[k].c.vs;
                 ld_scale = p.s[k].c.ld_scale;
@@ -358,7 +415,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                 tk = &maps.k[k];
                 tv = &maps.v[k];
             }
-        const int32_t k0 = u0 * kUnitKeys, n_keys = min(n_units * kUnitKeys, n_src - k0), n_blk = (n_keys + kBlk - 1) / kBlk;
         const uint16_t* ks = static_cast<const uint16_t*>(ks0) + (int64_t)h * ld_scale + k0;
         const uint16_t* vs = static_cast<const uint16_t*>(vs0) + (int64_t)h * ld_scale + k0;
         if (kg != nullptr) kg += k0;
@@ -395,8 +451,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
 
         // ---- queries into shared memory (a 16-byte piece per thread), this lane's rows' groups
         auto row_at = [&](int32_t e, int32_t& b, int32_t& m) -> bool {      // row e of the group
-            m = cl.group * R + e;
-            b = cl.stream;
+            m = item.group * R + e;
+            b = stream;
             if (!pre) return m < r.rows[b];
             if (m >= r.total) return false;
             b = 0;
@@ -618,7 +674,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
         if (abort) return;
         // ---- the warps' results meet: position 8 d + g of a row is d of lane g's 16 dims (tile j holds
         // d = 2 j and 2 j + 1), then a row per warp, four positions per lane
-        const int live = pre ? min(R, r.total - cl.group * R) : min(R, r.rows[cl.stream] - cl.group * R);
+        const int live = item.live;
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -663,7 +719,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                 acc.z += fk * x.z;
                 acc.w += fk * x.w;
             }
-            float* dst = p.part + (int64_t)(col + (int32_t)blockIdx.x) * kRowsSlotFloats;
+            float* dst = p.part + (int64_t)item.slot * kRowsSlotFloats;
             *reinterpret_cast<float4*>(dst + row * kHeadDim + 4 * lane) = acc;
             if (lane == 0) {
                 dst[kRowsMax * kHeadDim + row] = top;
@@ -674,13 +730,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
         // ---- arrivals: thread e for the e-th own group that the item's rows belong to
         if (threadIdx.x < 32) {
             int32_t b = -1, grp = 0, found = 0;
-            if (!pre) {
+            if (item.stream >= 0) {
                 if (lane == 0) {
-                    b = cl.stream;
-                    grp = cl.group;
+                    b = item.stream;
+                    grp = item.group;
                 }
             } else {
-                const int32_t r0 = cl.group * R, r1 = min(r0 + R, r.total);     // packed rows
+                const int32_t r0 = item.group * R, r1 = min(r0 + R, r.total);     // packed rows
 #pragma unroll
                 for (int k = 0; k < kMaxBatch; ++k)
                     if (k < p.n_streams && r.rows[k] > 0) {
@@ -697,18 +753,18 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
             }
             bool done = false;
             if (b >= 0) {
-                const int32_t groups = (r.rows[b] + R - 1) / R, own = p.n_heads * r.group0[b] + h * groups + grp;
-                int32_t c0, c1;
-                parts_of(r, p.n_heads * r.gp * r.up + own * r.uo, r.uo, c0, c1);
-                int32_t all = c1 - c0 + 1;
+                const int32_t groups = (r.rows[b] + R - 1) / R;
+                int32_t unused, all;
+                parts_of(r, p.n_heads, p.n_heads * (r.gp + r.group0[b]) + item.head * groups + grp, unused, all);
                 if (r.gp > 0) {
                     const int32_t x0 = r.first[b] + grp * R, x1 = min(x0 + R, r.first[b] + r.rows[b]);
                     for (int32_t x = x0 / R; x <= (x1 - 1) / R; ++x) {
-                        parts_of(r, (h * r.gp + x) * r.up, r.up, c0, c1);
-                        all += c1 - c0 + 1;
+                        int32_t more;
+                        parts_of(r, p.n_heads, item.head * r.gp + x, unused, more);
+                        all += more;
                     }
                 }
-                int32_t* cnt = p.cnt + (r.group0[b] + grp) * p.n_heads + h;
+                int32_t* cnt = p.cnt + (r.group0[b] + grp) * p.n_heads + item.head;
                 done = atom_add_acq_rel_gpu(cnt, 1) == all - 1;
                 if (done) *cnt = 0;      // for the next launch
             }
@@ -718,9 +774,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
         __syncthreads();
         for (uint32_t left = ready; left != 0; left &= left - 1) {
             const int e = __ffs(left) - 1;
-            int32_t b = cl.stream, grp = cl.group;
-            if (pre) {                   // the e-th own group again
-                const int32_t r0 = cl.group * R, r1 = min(r0 + R, r.total);
+            int32_t b = item.stream, grp = item.group;
+            if (b < 0) {                 // the e-th own group again
+                const int32_t r0 = item.group * R, r1 = min(r0 + R, r.total);
                 int32_t found = 0;
 #pragma unroll
                 for (int k = 0; k < kMaxBatch; ++k)
@@ -736,7 +792,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                         }
                     }
             }
-            rows_combine<T, R>(p, r, h, b, grp);
+            rows_combine<T, R>(p, r, item.head, b, grp);
         }
         fence_async_smem();          // the next item's copies overwrite the exchange
         __syncthreads();
@@ -770,7 +826,7 @@ constexpr uint32_t kRegsSoftmax = 176, kRegsOther = 80;
 constexpr uint32_t kTileRegPool = 256 * kRegsSoftmax + 256 * kRegsOther;
 static_assert(kTileRegPool == kTileThreads * 128, "the warpgroups' shares are the launch's registers");
 constexpr int kPolyPeriod = 4;
-constexpr float kItemSteps = 2.0f, kCutSteps = 4.5f;   // as the 16-bit kernel's schedule, in steps
+constexpr float kItemSteps = 2.0f, kCutSteps = 4.5f;   // an item's and the combine's cost, in steps (2.6 us each)
 constexpr int kPartSlots = 4;                    // partial tiles a CTA may write
 constexpr int kPartFloats = kBM * kD + 2 * kBM;
 constexpr int kPartWarps = 8;                    // arrival counters per cut unit
@@ -1097,6 +1153,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
     volatile int* abort = reinterpret_cast<volatile int*>(gbase + kSmAbort);
     auto item_at = [&](uint32_t k) { return reinterpret_cast<Item*>(gbase + kSmItem + (k & 1) * 160); };
     volatile uint32_t* info = reinterpret_cast<volatile uint32_t*>(gbase + kSmInfo);
+    __shared__ int32_t stream_rows[kMaxBatch];
     const int warp = threadIdx.x >> 5;
     const uint32_t lane = lane_id();
     const Params& p = a.p;
@@ -1137,31 +1194,44 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
     pdl_launch_dependents();
     pdl_wait();
 
-    // iterations per CTA when units are cut, 0 for whole units; the same on every thread
+    if (threadIdx.x < kMaxBatch) {
+        int32_t c = 0;
+#pragma unroll
+        for (int b = 0; b < kMaxBatch; ++b)
+            if (b == (int)threadIdx.x && b < p.n_streams) c = *p.s[b].count;
+        if (c > p.max_rows && blockIdx.x == 0) atomicOr(&g_error_word, kErrBounds);
+        stream_rows[threadIdx.x] = max(0, min(c, p.max_rows));
+    }
+    __syncthreads();
+    // The schedule, the same on every thread: whole units round-robin (per = parts = 0), units cut into
+    // `parts` equal parts with a CTA each (where there are at least twice as many CTAs as units), or
+    // the launch's iterations cut into ranges of `per` per CTA.
     const int32_t n_steps = a.n_pre + a.n_own;
-    int32_t per = 0;
-    int64_t total = 0;
-    int32_t n_units = 0;
+    int32_t per = 0, parts = 0, total = 0, n_units = 0;
     {
 #pragma unroll
         for (int b = 0; b < kMaxBatch; ++b)
             if (b < p.n_streams) {
-                const int32_t units = (max(0, min(*p.s[b].count, p.max_rows)) + kUnitRows - 1) / kUnitRows;
+                const int32_t units = (stream_rows[b] + kUnitRows - 1) / kUnitRows;
                 n_units += units * p.n_heads;
                 if (a.steps == nullptr) {
-                    total += (int64_t)units * p.n_heads * n_steps;
+                    total += units * p.n_heads * n_steps;
                 } else {
                     int32_t sum = 0;
                     for (int32_t u = (int32_t)lane; u < units; u += 32) sum += a.steps[b * a.units_cap + u];
-                    total += (int64_t)__reduce_add_sync(0xffffffffu, sum) * p.n_heads;
+                    total += __reduce_add_sync(0xffffffffu, sum) * p.n_heads;
                 }
             }
         const int32_t grid = (int32_t)gridDim.x;
-        const int64_t each = (total + grid - 1) / grid;
+        const int32_t each = (total + grid - 1) / grid, split = n_units > 0 ? grid / n_units : 0;
         const float avg = n_units > 0 ? (float)total / (float)n_units : 0.f;
         const float whole = (float)((n_units + grid - 1) / grid) * (avg + kItemSteps);
-        const float cut = (float)each + kItemSteps * ((float)each / fmaxf(avg, 1.f) + 1.f) + 2.f * kCutSteps;
-        if (cut < whole && each < (1 << 28) && total < (1ll << 31)) per = (int32_t)each;
+        const float cut = (float)each + kItemSteps * ((float)each / fmaxf(avg, 1.f) + 1.f) + kCutSteps;
+        const float even = split > 1 ? ceilf(avg / (float)split) + kItemSteps + kCutSteps : INFINITY;
+        if (fminf(cut, even) < whole) {
+            if (even <= cut) parts = split;
+            else per = each;
+        }
     }
 
     if (warp >= kConvWarp) {
@@ -1390,24 +1460,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
         } else if (warp == kSchedWarp) {
             // ---------------- scheduler ----------------
             const int32_t grid = (int32_t)gridDim.x, c = (int32_t)blockIdx.x;
-            int64_t cur = per > 0 ? (int64_t)c * per : c;
-            const int64_t end = per > 0 ? min(total, cur + per) : n_units;
+            int32_t cur = per > 0 ? (int32_t)min((int64_t)total, (int64_t)c * per) : parts > 0 ? c / parts : c;
+            const int32_t end = per > 0 ? (int32_t)min((int64_t)total, (int64_t)cur + per) : n_units;
             for (uint32_t k = 0;; ++k) {
-                const bool more = cur < end;
+                bool more = cur < end;
                 // the unit: stream, head, first row, steps, first iteration
-                int32_t b = -1, rows = 0, head = 0, unit = 0, cnt = n_steps;
-                int64_t rest = cur, i0 = cur;
+                int32_t b = -1, rows = 0, head = 0, unit = 0, cnt = n_steps, rest = cur, i0 = cur;
                 if (more) {
                     int32_t units = 1;
 #pragma unroll
                     for (int s = 0; s < kMaxBatch; ++s)
                         if (b < 0 && s < p.n_streams) {
-                            const int32_t m = max(0, min(*p.s[s].count, p.max_rows));
+                            const int32_t m = stream_rows[s];
                             const int32_t u = (m + kUnitRows - 1) / kUnitRows;
-                            int64_t span = u;             // per head, in units or iterations
+                            int32_t span = u;             // per head, in units or iterations
                             if (per > 0) {
                                 if (a.steps == nullptr) {
-                                    span = (int64_t)u * n_steps;
+                                    span = u * n_steps;
                                 } else {
                                     int32_t sum = 0;
                                     for (int32_t e = (int32_t)lane; e < u; e += 32) sum += a.steps[s * a.units_cap + e];
@@ -1418,20 +1487,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                                 b = s;
                                 rows = m;
                                 units = u;
-                                head = (int32_t)(rest / span);
+                                head = rest / span;
                                 rest -= head * span;
                             } else {
                                 rest -= span * p.n_heads;
                             }
                         }
                     if (per == 0) {
-                        unit = (int32_t)rest;
+                        unit = rest;
                         if (a.steps) cnt = a.steps[b * a.units_cap + unit];
                     } else if (a.steps == nullptr) {
-                        unit = (int32_t)(rest / n_steps);
-                        i0 = cur - (rest - (int64_t)unit * n_steps);
+                        unit = rest / n_steps;
+                        i0 = cur - (rest - unit * n_steps);
                     } else {
-                        int32_t left = (int32_t)rest;     // iterations into the head's units
+                        int32_t left = rest;              // iterations into the head's units
                         bool found = false;
                         for (int32_t e0 = 0; e0 < units && !found; e0 += 32) {
                             const int32_t mine = e0 + (int32_t)lane < units ? a.steps[b * a.units_cap + e0 + lane] : 0;
@@ -1454,10 +1523,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                         }
                     }
                 }
+                // the item's steps, and the CTAs that hold the unit's parts
+                int32_t s0 = 0, n = cnt, c_first = c, c_last = c;
+                if (per > 0) {
+                    s0 = cur - i0;
+                    n = min(cnt - s0, end - cur);
+                    c_first = i0 / per;
+                    c_last = (i0 + cnt - 1) / per;
+                } else if (parts > 0) {
+                    const int32_t e = c - cur * parts, of = min(parts, cnt);
+                    more = more && e < of;
+                    s0 = cnt * e / of;
+                    n = cnt * (e + 1) / of - s0;
+                    c_first = c - e;
+                    c_last = c_first + of - 1;
+                    i0 = 0;                               // the part is the CTA's first item
+                }
+                if (!more) n = 0;
                 if (k >= 2 && !__all_sync(0xffffffffu, mbar_wait(bar(kItemEmpty + (k & 1)), ((k >> 1) - 1) & 1, abort))) break;
                 Item* it = item_at(k);
-                const int32_t s0 = per > 0 ? (int32_t)(cur - i0) : 0;
-                const int32_t n = !more ? 0 : per > 0 ? min(cnt - s0, (int32_t)(end - cur)) : cnt;
                 if (lane == 0) {
                     it->n = n;
                     if (n > 0) {
@@ -1472,7 +1556,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                                 it->idx = p.s[s].idx;
                                 it->qg = p.s[s].qg;
                                 it->out = p.s[s].out;
-                                if (*p.s[s].count > p.max_rows && unit == 0 && head == 0) atomicOr(&g_error_word, kErrBounds);
                             }
                         it->s0 = s0;
                         it->head = head;
@@ -1480,16 +1563,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                         it->rows = rows;
                         it->list = a.steps ? a.list + ((int64_t)b * a.units_cap + unit) * n_steps : nullptr;
                         it->cut = n < cnt;
-                        it->i0 = (int32_t)i0;
-                        it->c_first = per > 0 ? (int32_t)(i0 / per) : 0;
-                        it->c_last = per > 0 ? (int32_t)((i0 + cnt - 1) / per) : 0;
+                        it->i0 = i0;
+                        it->c_first = c_first;
+                        it->c_last = c_last;
                         it->stream = b;
                     }
                     mbar_arrive(bar(kItemFull + (k & 1)));
                 }
                 __syncwarp();
                 if (n == 0) break;
-                cur += per > 0 ? n : grid;
+                cur = per > 0 ? cur + n : parts > 0 ? end : cur + grid;
             }
         }
     } else {

@@ -385,6 +385,8 @@ int32_t fxr_attention_q8(const fxr_frame_desc* desc, int32_t n_streams, const fx
     if (!aligned16(workspace)) return fail(FXR_ERR_INVALID, "workspace must be 16-byte aligned");
     if (workspace_bytes < w.total) return fail(FXR_ERR_WORKSPACE, "workspace %zu < required %zu", workspace_bytes, w.total);
     if (w.few && w.line >= INT32_MAX) return fail(FXR_ERR_UNSUPPORTED, "too many keys x heads x row groups for one call (%lld)", (long long)w.line);
+    if (!w.few && (int64_t)(w.n_pre + w.n_own) * w.units * desc->n_heads * std::min(n_streams, FXR_MAX_BATCH) >= INT32_MAX)
+        return fail(FXR_ERR_UNSUPPORTED, "too many rows x keys x heads for one call");
     if (!w.few && w.n_pre + w.n_own > 0x7fff)
         return fail(FXR_ERR_UNSUPPORTED, "%d key rows: more than 32767 tiles of 128", n_prefix + desc->n_tokens);
     for (int32_t b0 = 0; b0 < n_streams; b0 += FXR_MAX_BATCH) {
