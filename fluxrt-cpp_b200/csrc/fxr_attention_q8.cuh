@@ -62,9 +62,11 @@ struct Params {
 //   O^T += V^T P^T: an operand pairs two keys of one dim; one byte permute takes both codes. A lane's
 //     rows in the 8 row tiles are 16 consecutive dims. P^T changes from the accumulators' to the
 //     operand's layout by an 8 x 8 transpose (movmatrix).
-// K scales multiply the scores in 32 bits. A V scale is split into 2^e * f, f in [1, 2): f multiplies
-// P before its one rounding to T, 2^e the codes, exactly (all of the scale on P would push it into
-// f16's subnormals; all of it on V would cost a second rounding). bf16 P holds the whole product.
+// All operands are f16, whatever the frame's type: it holds the codes exactly, and the codes reach it in
+// fewer instructions than bf16. bf16 queries are brought to f16 by a power of two per row (exactly, but
+// for elements below 2^-24 of the row's largest). K scales multiply the scores in 32 bits. V scales
+// multiply P before its one rounding, relative to the largest that the warp has met, so that P stays in
+// f16's range whatever the scales are.
 // Partial results (O, maximum, sum) meet in L2: the last of a row group's parts to arrive combines
 // them in key order, so the result does not depend on the order of arrival.
 // ---------------------------------------------------------------------------------------------
@@ -85,7 +87,7 @@ constexpr uint32_t kQPad = 272;                // bytes per query row
 constexpr uint32_t kRowsSmemScale = kRowsWarps * kRingWarp;
 constexpr uint32_t kRowsSmemQ = kRowsSmemScale + kRowsWarps * kDepth * kScaleSlot;
 constexpr uint32_t kRowsSmemM = kRowsSmemQ + kRowsMax * kQPad;             // maxima, then sums: [16 rows][warps]
-constexpr uint32_t kRowsSmemBar = kRowsSmemM + 2 * kRowsWarps * kRowsMax * 4;
+constexpr uint32_t kRowsSmemBar = kRowsSmemM + (2 * kRowsWarps + 1) * kRowsMax * 4;   // (and the queries' factors)
 constexpr uint32_t kRowsSmem = kRowsSmemBar + kRowsWarps * kDepth * 8 + 1024;   // + alignment slack
 constexpr int kRowsSlotFloats = kRowsMax * kHeadDim + 2 * kRowsMax;
 static_assert(kRowsWarps * kRowsMax * kPadRow * 4 <= kRowsWarps * kRingWarp, "exchange fits the ring");
@@ -102,18 +104,7 @@ __device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                        uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16816<__half>(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                                 uint32_t b1) {
+__device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -294,7 +285,6 @@ __device__ __noinline__ void rows_combine(const Params& p, const RowsPlan& r, in
 template <typename T, int F, int NQ>
 __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_constant__ RowsMaps maps, const __grid_constant__ Params p) {
     constexpr int R = 8 * NQ;
-    constexpr bool kF16 = StoreT<T>::kUmmaFormat == 0;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ RowsPlan r;
@@ -469,7 +459,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                 if (k == b) st = &p.s[k];
             return st;
         };
-        if (threadIdx.x < R * 16) {
+        float* q_factor = xm + 2 * kRowsWarps * kRowsMax;      // what a row's queries were divided by
+        if (threadIdx.x < R * 16) {                            // whole warps: a row per half-warp
             int32_t b, m;
             uint4 x = make_uint4(0, 0, 0, 0);
             if (row_at(threadIdx.x >> 4, b, m)) {
@@ -477,6 +468,26 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(st->qc) + (int64_t)m * st->ld_qc + (int64_t)h * kHeadDim +
                                                     (threadIdx.x & 15) * 8);
             }
+            float factor = 1.f;
+            if constexpr (StoreT<T>::kUmmaFormat == 1) {
+                // the largest magnitude's exponent: bf16 bits, doubled to drop the sign
+                uint32_t top = 0;
+                uint32_t* w = &x.x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
+#pragma unroll
+                for (int e = 8; e > 0; e >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, e));
+                // to [2^10, 2^11); the exponent is kept where both the factor and its inverse are normal
+                const int e = min(max((int)(top >> 7), 20), 254) - 137;
+                factor = __int_as_float((127 + e) << 23);
+                const float inv = __int_as_float((127 - e) << 23);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 v = StoreT<T>::unpack2(w[k]);
+                    w[k] = StoreT<__half>::pack2(v.x * inv, v.y * inv);
+                }
+            }
+            if ((threadIdx.x & 15) == 0) q_factor[threadIdx.x >> 4] = factor;
             sts128(q_at + (threadIdx.x >> 4) * kQPad + (threadIdx.x & 15) * 16, x);
         }
         uint32_t qg[NQ][2];
@@ -514,8 +525,12 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                 l_run[q][e] = 0.f;
             }
         }
-        const float sc = p.scale_log2 * q8::code_scale<T, F>();
-
+        float v_top = 0.f, v_inv = 0.f;      // the largest V scale so far (of the warp), its inverse
+        float qs[NQ][2];                     // score factors of this lane's queries
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int d = 0; d < 2; ++d) qs[q][d] = p.scale_log2 * q_factor[8 * q + 2 * t + d];
         uint32_t issued = it + min(kDepth - 1, (n_blk - warp + kRowsWarps - 1) / kRowsWarps);
         for (int32_t b = warp; b < n_blk; b += kRowsWarps, ++it) {
             if (b + (kDepth - 1) * kRowsWarps < n_blk) {
@@ -547,31 +562,46 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
 #pragma unroll
                     for (int jj = 0; jj < 2; ++jj) {
                         const int j = 2 * jp + jj;
-                        const uint32_t a0 = q8::code_pair<T, F>(wa[j], 0, 1), a1 = q8::code_pair<T, F>(wb[j], 0, 1);
-                        const uint32_t a2 = q8::code_pair<T, F>(wa[j], 2, 3), a3 = q8::code_pair<T, F>(wb[j], 2, 3);
+                        const uint32_t a0 = q8::code_pair<F>(wa[j], false), a1 = q8::code_pair<F>(wb[j], false);
+                        const uint32_t a2 = q8::code_pair<F>(wa[j], true), a3 = q8::code_pair<F>(wb[j], true);
 #pragma unroll
                         for (int q = 0; q < NQ; ++q)
-                            mma16816<T>(s[q], a0, a1, a2, a3, jj ? q4[q].z : q4[q].x, jj ? q4[q].w : q4[q].y);
+                            mma16816(s[q], a0, a1, a2, a3, jj ? q4[q].z : q4[q].x, jj ? q4[q].w : q4[q].y);
                     }
                 }
             }
             // scales and masks: this lane's keys, key_of(g) and 8 behind it
-            float v_sc[2];               // what P is multiplied with
+            float v_sc[2];               // V scales, then relative to v_top: what P is multiplied with
             const int32_t left = n_keys - b * kBlk;
             bool grow = false;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int key = key_of(g) + 8 * e;
                 const float kk = StoreT<T>::unpack2(sc_p[key]).x, vv = StoreT<T>::unpack2(sc_p[kBlk + key]).x;
-                const bool v_ok = q8::valid_scale<T, F>(vv);
-                const float f = v_ok && q8::valid_scale<T, F>(kk) ? kk * sc : __uint_as_float(0x7fc00000u);
-                v_sc[e] = v_ok ? vv : 0.f;
-                if (kF16) v_sc[e] = __uint_as_float((__float_as_uint(v_sc[e]) & 0x007fffffu) | 0x3f800000u);
+                const bool in = key < left, v_ok = q8::valid_scale<T, F>(vv);
+                const float f = v_ok && q8::valid_scale<T, F>(kk) ? kk : __uint_as_float(0x7fc00000u);
+                v_sc[e] = v_ok && in ? vv : 0.f;
 #pragma unroll
                 for (int q = 0; q < NQ; ++q)
 #pragma unroll
-                    for (int d = 0; d < 2; ++d) s[q][2 * e + d] *= f;
+                    for (int d = 0; d < 2; ++d) s[q][2 * e + d] *= f * qs[q][d];
             }
+            if (__any_sync(0xffffffffu, fmaxf(v_sc[0], v_sc[1]) > v_top)) {
+                float x = fmaxf(v_sc[0], v_sc[1]);
+#pragma unroll
+                for (int e = 16; e > 0; e >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, e));
+                const float inv = 1.f / fmaxf(x, 0x1p-126f), al = v_inv > 0.f ? inv / v_inv : 0.f;
+                v_top = x;
+                v_inv = inv;
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[q][j][e] *= al;
+            }
+            v_sc[0] *= v_inv;
+            v_sc[1] *= v_inv;
             if (kg != nullptr || left < kBlk) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -625,8 +655,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                     e_[2 + d] = ex2_approx(s[q][2 + d] - mu);
                     l_run[q][d] += e_[d] + e_[2 + d];
                 }
-                pb[q][0] = transpose8(StoreT<T>::pack2(e_[0] * v_sc[0], e_[1] * v_sc[0]));
-                pb[q][1] = transpose8(StoreT<T>::pack2(e_[2] * v_sc[1], e_[3] * v_sc[1]));
+                pb[q][0] = transpose8(StoreT<__half>::pack2(e_[0] * v_sc[0], e_[1] * v_sc[0]));
+                pb[q][1] = transpose8(StoreT<__half>::pack2(e_[2] * v_sc[1], e_[3] * v_sc[1]));
             }
             // O^T += V^T P^T
             // (operand row index 2 t + x of a half is key key_of(2 t + x) = t + 4 x)
@@ -640,31 +670,15 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                 w[e][2] = q8::code_word<F>(v4.z);
                 w[e][3] = q8::code_word<F>(v4.w);
             }
-            uint32_t pow2[2] = {0, 0};
-            if constexpr (kF16) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float2 v2 = make_float2(StoreT<T>::unpack2(sc_p[kBlk + 8 * e + t]).x, StoreT<T>::unpack2(sc_p[kBlk + 8 * e + t + 4]).x);
-                    v2.x = q8::valid_scale<T, F>(v2.x) ? __uint_as_float(__float_as_uint(v2.x) & 0x7f800000u) * q8::code_scale<T, F>() : 0.f;
-                    v2.y = q8::valid_scale<T, F>(v2.y) ? __uint_as_float(__float_as_uint(v2.y) & 0x7f800000u) * q8::code_scale<T, F>() : 0.f;
-                    pow2[e] = StoreT<T>::pack2(v2.x, v2.y);
-                }
-            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 // dims 2 j and 2 j + 1 of the lane's 16: the two keys' bytes side by side
                 const uint32_t lo = __byte_perm(w[0][j >> 1], w[1][j >> 1], (j & 1) ? 0x7362 : 0x5140);
                 const uint32_t hi = __byte_perm(w[2][j >> 1], w[3][j >> 1], (j & 1) ? 0x7362 : 0x5140);
-                uint32_t a0 = q8::code_pair<T, F>(lo, 0, 1), a1 = q8::code_pair<T, F>(lo, 2, 3);
-                uint32_t a2 = q8::code_pair<T, F>(hi, 0, 1), a3 = q8::code_pair<T, F>(hi, 2, 3);
-                if constexpr (kF16) {
-                    a0 = q8::mul2<T>(a0, pow2[0]);
-                    a1 = q8::mul2<T>(a1, pow2[0]);
-                    a2 = q8::mul2<T>(a2, pow2[1]);
-                    a3 = q8::mul2<T>(a3, pow2[1]);
-                }
+                const uint32_t a0 = q8::code_pair<F>(lo, false), a1 = q8::code_pair<F>(lo, true);
+                const uint32_t a2 = q8::code_pair<F>(hi, false), a3 = q8::code_pair<F>(hi, true);
 #pragma unroll
-                for (int q = 0; q < NQ; ++q) mma16816<T>(o[q][j], a0, a1, a2, a3, pb[q][0], pb[q][1]);
+                for (int q = 0; q < NQ; ++q) mma16816(o[q][j], a0, a1, a2, a3, pb[q][0], pb[q][1]);
             }
             __syncwarp();
         }
@@ -675,6 +689,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
         // ---- the warps' results meet: position 8 d + g of a row is d of lane g's 16 dims (tile j holds
         // d = 2 j and 2 j + 1), then a row per warp, four positions per lane
         const int live = item.live;
+        const float v_unit = v_inv > 0.f ? 1.f / v_inv : 0.f;     // of P's V factors
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -684,8 +699,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                 if (row < live) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        dst[16 * j] = o[q][j][d];
-                        dst[16 * j + 8] = o[q][j][2 + d];
+                        dst[16 * j] = o[q][j][d] * v_unit;
+                        dst[16 * j + 8] = o[q][j][2 + d] * v_unit;
                     }
                 }
                 float l = l_run[q][d];

@@ -182,25 +182,16 @@ struct SmallScaleDecoder {
         return bits(__hmul2(as_bf(Decoder<__nv_bfloat16, kE4m3>::fields(w, a, b)), s));
     }
 };
-// Codes alone, exact up to the factor 1 / code_scale(): as Decoder with s = 1.
-template <typename T, int F> __device__ __forceinline__ constexpr float code_scale() {
-    return (F == kE4m3 && StoreT<T>::kUmmaFormat == 0) ? 256.f : 1.f;
-}
+// Codes alone as a pair of f16, which holds every code exactly. word: four codes prepared by code_word;
+// upper: its codes 2 and 3, not 0 and 1. e4m3 has an instruction for it.
 template <int F> __device__ __forceinline__ uint32_t code_word(uint32_t w) { return F == kInt8 ? w ^ 0x80808080u : w; }
-template <typename T, int F> __device__ __forceinline__ uint32_t code_pair(uint32_t w, int a, int b) {
-    constexpr bool bf16 = StoreT<T>::kUmmaFormat == 1;
+template <int F> __device__ __forceinline__ uint32_t code_pair(uint32_t w, bool upper) {
     if constexpr (F == kInt8) {
-        const uint32_t u = __byte_perm(w, bf16 ? 0x42424242u : 0x64646464u, (uint32_t)(a | 0x40 | (b << 8) | 0x4000));
-        if constexpr (bf16) {
-            const __nv_bfloat162 t = __hfma2(as_bf(u), as_bf(0x40004000u), as_bf(0xc300c300u));
-            return bits(__hsub2(t, __hfma2_relu(as_bf(u), as_bf(0xc000c000u), as_bf(0x43004300u))));
-        } else {
-            return bits(__hsub2(as_h(u), as_h(0x64806480u)));
-        }
+        return bits(__hsub2(as_h(__byte_perm(w, 0x64646464u, upper ? 0x4342 : 0x4140)), as_h(0x64806480u)));
     } else {
-        const uint32_t u = __byte_perm(w, 0u, (uint32_t)(a | (a << 4) | (b << 8) | (b << 12)));
-        if constexpr (bf16) return mul2<T>(((u << 4) & 0x07f007f0u) | (u & 0x80008000u), 0x7b807b80u);
-        else return ((u << 7) & 0x3f803f80u) | (u & 0x80008000u);
+        uint32_t r;
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(upper ? w >> 16 : w));
+        return r;
     }
 }
 
