@@ -1040,18 +1040,6 @@ __global__ void __launch_bounds__(kVisThreads) visible_steps_kernel(const __grid
         : "memory")
 
 // ---- pieces of the tile kernel --------------------------------------------------------------------
-// Maximum that is NaN where an operand is (a NaN score must reach its row).
-__device__ __forceinline__ float max3n(float a, float b, float c) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-__device__ __forceinline__ float max2n(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
 // Scratch slot of the part that CTA c holds of a unit whose iterations start at i0: its first item
 // unless the unit starts inside c's range behind others.
 __device__ __forceinline__ int64_t part_at(int32_t i0, int32_t per, int32_t c, int t) {
@@ -1651,13 +1639,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                 }
                 float mp[8];
 #pragma unroll
-                for (int q = 0; q < 8; ++q) mp[q] = max2n(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1]));
+                for (int q = 0; q < 8; ++q) mp[q] = q8::max2n(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1]));
 #pragma unroll
                 for (int i = 1; i < 8; ++i)
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
-                        mp[q] = max3n(mp[q], __uint_as_float(s[16 * i + 2 * q]), __uint_as_float(s[16 * i + 2 * q + 1]));
-                const float mx = max3n(max3n(mp[0], mp[1], mp[2]), max3n(mp[3], mp[4], mp[5]), max2n(mp[6], mp[7])) * c;
+                        mp[q] = q8::max3n(mp[q], __uint_as_float(s[16 * i + 2 * q]), __uint_as_float(s[16 * i + 2 * q + 1]));
+                const float mx = q8::max3n(q8::max3n(mp[0], mp[1], mp[2]), q8::max3n(mp[3], mp[4], mp[5]), q8::max2n(mp[6], mp[7])) * c;
                 if (mx != mx) l_run = mx;        // a NaN score: the row is NaN
                 if (j == 0) {
                     m_run = mx;

@@ -52,52 +52,62 @@ template <typename T, int F> __device__ __forceinline__ constexpr float scale_ca
 // Whether s is a scale that the write stores for a finite vector (every code times it is finite).
 template <typename T, int F> __device__ __forceinline__ bool valid_scale(float s) { return fabsf(s) <= scale_cap<T, F>(); }
 
-// Scale of a head vector whose largest magnitude has the bits `amax` (NaN and infinities compare
-// above every finite value).
+// Scale of a head vector whose largest magnitude is amax (infinite or NaN where an element is).
 template <typename T, int F>
-__device__ __forceinline__ float scale_of(uint32_t amax) {
-    if (amax >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
-    return fminf(scale_up<T>(__fdiv_rn(__uint_as_float(amax), top_code<F>())), scale_cap<T, F>());
+__device__ __forceinline__ float scale_of(float amax) {
+    if (!(amax < INFINITY)) return __uint_as_float(0x7fc00000u);
+    return fminf(scale_up<T>(__fdiv_rn(amax, top_code<F>())), scale_cap<T, F>());
 }
 
-// Codes of 8 values as 8 bytes. s = 0 or NaN: codes 0. x / s is taken as x times the rounded 1 / s, off
-// by at most 2^-22 relative (1.5e-5 of a code). kExact (x of T): such a quotient of two numbers of T
-// that is not half way between two codes is farther from there than 2.4e-4 of a code (int8; the
-// numerator of the difference is a whole multiple of the smaller unit) or 2^-16 relative (e4m3), so
-// rounding it first to a multiple of 2^-13, or to 18 bits, puts the half-way cases, and only those,
-// exactly half way, and the nearest-even rounding that follows is that of the true quotient. Divisions
-// took half of this kernel's instructions.
+// Maximum that is NaN where an operand is.
+__device__ __forceinline__ float max3n(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max2n(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 f2add(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d)
+        : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+
+// Codes of 4 values as 4 bytes. x / s is taken as x times the rounded 1 / s, off by at most 2^-22
+// relative (1.5e-5 of a code). kExact (x of T): such a quotient of two numbers of T that is not half way
+// between two codes is farther from there than 2.4e-4 of a code (int8; the numerator of the difference
+// is a whole multiple of the smaller unit) or 2^-16 relative (e4m3), so rounding it first to a multiple
+// of 2^-13, or to 18 bits, puts the half-way cases, and only those, exactly half way, and the
+// nearest-even rounding that follows is that of the true quotient. (Divisions took half of the write
+// kernel's instructions.)
 template <int F, bool kExact>
-__device__ __forceinline__ uint2 encode8(const float* x, float s, bool capped) {
-    const float r = s > 0.f ? __frcp_rn(s) : 0.f;
-    float y[8];
+__device__ __forceinline__ uint32_t encode4(float2 a, float2 b, float r, bool clamp) {
+    float2 y[2] = {f2mul(a, make_float2(r, r)), f2mul(b, make_float2(r, r))};
+    if (F == kInt8) {
+        // in 1.5 * 2^23 + y the low byte of the bits is y's whole number, two's complement
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = s > 0.f ? x[e] * r : 0.f;
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        if (F == kInt8) {
-            // in 1.5 * 2^23 + y the low byte of the bits is y's whole number, two's complement
-            uint32_t c[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float v = y[4 * h + e];
-                if (capped) v = fminf(fmaxf(v, -127.f), 127.f);
-                if (kExact) v = __fadd_rn(__fadd_rn(v, 1536.f), -1536.f);
-                c[e] = __float_as_uint(__fadd_rn(v, 12582912.f));
-            }
-            w[h] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-        } else {
-            if (kExact) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[4 * h + e] = __uint_as_float((__float_as_uint(y[4 * h + e]) + 0x20u) & ~0x3fu);
-            }
-            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h], y[4 * h + 1]), __NV_SATFINITE, __NV_E4M3);
-            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h + 2], y[4 * h + 3]), __NV_SATFINITE, __NV_E4M3);
-            w[h] = lo | (hi << 16);
+        for (int e = 0; e < 2; ++e) {
+            if (clamp) y[e] = make_float2(fminf(fmaxf(y[e].x, -127.f), 127.f), fminf(fmaxf(y[e].y, -127.f), 127.f));
+            if (kExact) y[e] = f2add(f2add(y[e], make_float2(1536.f, 1536.f)), make_float2(-1536.f, -1536.f));
+            y[e] = f2add(y[e], make_float2(12582912.f, 12582912.f));
         }
+        return __byte_perm(__byte_perm(__float_as_uint(y[0].x), __float_as_uint(y[0].y), 0x0040),
+                           __byte_perm(__float_as_uint(y[1].x), __float_as_uint(y[1].y), 0x0040), 0x5410);
+    } else {
+        if (kExact) {      // c - (c - y) with c = (2^6 + 1) y is y in 18 bits
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float2 c = f2mul(y[e], make_float2(65.f, 65.f));
+                y[e] = f2add(c, f2mul(f2add(c, make_float2(-y[e].x, -y[e].y)), make_float2(-1.f, -1.f)));
+            }
+        }
+        return (uint32_t)__nv_cvt_float2_to_fp8x2(y[0], __NV_SATFINITE, __NV_E4M3) |
+               ((uint32_t)__nv_cvt_float2_to_fp8x2(y[1], __NV_SATFINITE, __NV_E4M3) << 16);
     }
-    return make_uint2(w[0], w[1]);
 }
 
 __device__ __forceinline__ __nv_bfloat162 as_bf(uint32_t u) { return *reinterpret_cast<const __nv_bfloat162*>(&u); }
@@ -237,96 +247,97 @@ __device__ __forceinline__ void rope_turn(float pos, float2 turns, float* sn, fl
     sincospif(2.f * frac, sn, cs);
 }
 
-// RMSNorm + RoPE of one lane's 8 elements of a half-warp's head vector, in 32 bits.
-template <typename T>
-__device__ __forceinline__ void norm_rope8(const uint4& x, const float2* w2, float eps, const float* cs,
-                                           const float* sn, float* y) {
-    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-    float2 p[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) p[t] = StoreT<T>::unpack2(u[t]);
-    float2 s2 = f2mul(p[0], p[0]);
-#pragma unroll
-    for (int t = 1; t < 4; ++t) s2 = f2fma(p[t], p[t], s2);
-    float ss = s2.x + s2.y;
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = rsqrtf(ss * (1.0f / kHeadDim) + eps);
-    const float2 r2 = make_float2(r, r);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const float2 ab = f2mul(f2mul(p[t], r2), w2[t]);
-        y[2 * t] = ab.x * cs[t] - ab.y * sn[t];
-        y[2 * t + 1] = ab.y * cs[t] + ab.x * sn[t];
-    }
-}
-
-// Quantises a half-warp's head vector (8 values per lane) and stores its codes and scale.
-template <typename T, int F, bool kExact>
-__device__ __forceinline__ void quantise_store(const float* y, uint8_t* codes, T* scale, int sub, bool active) {
-    uint32_t amax = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(y[e]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float s = scale_of<T, F>(amax);
-    // (__frcp_rn overflows below 2^-126: such scales, and capped ones, are brought into range exactly)
-    const bool capped = s >= scale_cap<T, F>(), tiny = s < 0x1p-100f;
-    uint2 w;
-    if (__any_sync(0xffffffffu, capped || tiny)) {
-        const float up = tiny ? 0x1p+100f : 1.f;
-        float z[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] = y[e] * up;
-        w = encode8<F, kExact>(z, s * up, true);
-    } else {
-        w = encode8<F, kExact>(y, s, false);
-    }
-    if (active) {
-        *reinterpret_cast<uint2*>(codes + 8 * sub) = w;
-        if (sub == 0) {
-            const uint32_t p = StoreT<T>::pack2(s, s);
-            *reinterpret_cast<uint16_t*>(scale) = (uint16_t)p;
-        }
-    }
-}
-
 constexpr int kWriteThreads = 256;
 constexpr int kWriteWarps = kWriteThreads / 32;
+constexpr int kVecLanes = 8;                         // lanes of a head vector
+constexpr int kVecHeads = 32 / kVecLanes;            // heads that a warp works on at a time
+constexpr int kVecPairs = kHeadDim / kVecLanes / 2;  // element pairs of a lane
 
-// Executed rows into the 8-bit cache. A half-warp holds a 128-wide head vector, 8 values per lane, so
-// that rotary pairs are lane-local and the sum of squares and the largest magnitude are 4-step
-// shuffles; a warp runs two heads of Q, K and V at a time. A row's heads are divided over `parts`
-// warps, as many as give every warp of the grid work (a few rows: one head pair per warp).
-// Bound by memory: 3 rows of T read, one of T and two of bytes written, per token.
-template <typename T, int F, bool kRaw>
-__global__ void __launch_bounds__(kWriteThreads, 3) q8_write_kernel(const __grid_constant__ WriteArgs a) {
-    const int lane = threadIdx.x & 31, sub = lane & 15, half = lane >> 4;
-    const int32_t warp = blockIdx.x * kWriteWarps + (threadIdx.x >> 5), warps = gridDim.x * kWriteWarps;
-    float2 turns[4];
-    int axis[4];
-    float2 wq[4], wk[4];
-    if (!kRaw) {
+// A lane's 16 elements of a head vector in 32 bits.
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4* x, float2* y) {
+    const uint32_t u[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            turns[t] = a.turns[4 * sub + t];
-            axis[t] = a.axis[4 * sub + t];
-        }
+    for (int t = 0; t < kVecPairs; ++t) y[t] = StoreT<T>::unpack2(u[t]);
+}
+
+// RMSNorm (w: the lane's weights) + RoPE.
+__device__ __forceinline__ void norm_rope16(float2* y, const float2* w, float eps, const float* cs, const float* sn) {
+    float2 s2 = f2mul(y[0], y[0]);
+#pragma unroll
+    for (int t = 1; t < kVecPairs; ++t) s2 = f2fma(y[t], y[t], s2);
+    float ss = s2.x + s2.y;
+#pragma unroll
+    for (int o = kVecLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float r = rsqrtf(ss * (1.0f / kHeadDim) + eps);
+#pragma unroll
+    for (int t = 0; t < kVecPairs; ++t) {
+        const float2 ab = f2mul(f2mul(y[t], make_float2(r, r)), w[t]);
+        y[t] = make_float2(ab.x * cs[t] - ab.y * sn[t], ab.y * cs[t] + ab.x * sn[t]);
     }
+}
+
+// Quantises a head vector over its lanes and stores its codes and scale.
+template <typename T, int F, bool kExact>
+__device__ __forceinline__ void quantise_store(float2* y, uint8_t* codes, T* scale, int sub, bool active) {
+    float m[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = max2n(fabsf(y[e].x), fabsf(y[e].y));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = max3n(m[e], fabsf(y[4 + e].x), fabsf(y[4 + e].y));
+    float amax = max2n(max3n(m[0], m[1], m[2]), m[3]);
+#pragma unroll
+    for (int o = kVecLanes / 2; o > 0; o >>= 1) amax = max2n(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float s = scale_of<T, F>(amax);
+    // scales whose inverse is not a normal number are brought into range exactly; none: codes 0
+    const bool tiny = s < 0x1p-100f, none = !(s > 0.f), capped = s >= scale_cap<T, F>();
+    float r = __frcp_rn(s);
+    uint4 w;
+    if (__any_sync(0xffffffffu, tiny || none || capped)) {
+        const float up = none ? 0.f : tiny ? 0x1p+100f : 1.f;
+        r = none ? 0.f : __frcp_rn(s * up);
+#pragma unroll
+        for (int t = 0; t < kVecPairs; ++t)
+            y[t] = none ? make_float2(0.f, 0.f) : make_float2(y[t].x * up, y[t].y * up);
+        w = make_uint4(encode4<F, kExact>(y[0], y[1], r, true), encode4<F, kExact>(y[2], y[3], r, true),
+                       encode4<F, kExact>(y[4], y[5], r, true), encode4<F, kExact>(y[6], y[7], r, true));
+    } else {
+        w = make_uint4(encode4<F, kExact>(y[0], y[1], r, false), encode4<F, kExact>(y[2], y[3], r, false),
+                       encode4<F, kExact>(y[4], y[5], r, false), encode4<F, kExact>(y[6], y[7], r, false));
+    }
+    if (active) {
+        *reinterpret_cast<uint4*>(codes + 16 * sub) = w;
+        if (sub == 0) *reinterpret_cast<uint16_t*>(scale) = (uint16_t)StoreT<T>::pack2(s, s);
+    }
+}
+
+// Executed rows into the 8-bit cache. Eight lanes hold a 128-wide head vector, 16 values each, so that
+// rotary pairs are lane-local and the sum of squares and the largest magnitude are 3-step shuffles; a
+// warp runs four heads of Q, K and V at a time, and a row's heads are divided over `parts` warps. Three
+// rows of T are read, one of T and two of bytes written per token: bound by memory (16896 rows of 24
+// heads: 100 us, 5.2 TB/s; two lanes' worth of shuffles and a division per code took 211 us).
+template <typename T, int F, bool kRaw>
+__global__ void __launch_bounds__(kWriteThreads, 2) q8_write_kernel(const __grid_constant__ WriteArgs a) {
+    const int lane = threadIdx.x & 31, sub = lane & (kVecLanes - 1), of = lane / kVecLanes;
+    const int32_t warp = blockIdx.x * kWriteWarps + (threadIdx.x >> 5), warps = gridDim.x * kWriteWarps;
     pdl_launch_dependents();
     pdl_wait();
+    const int32_t m_all = min(a.count ? *a.count : a.host_count, a.n_tokens);
+    const int32_t quads = (a.n_heads + kVecHeads - 1) / kVecHeads;
+    // (dividing rows further, to even out the warps' last round, costs more than it gains: 1536 rows
+    // 16.5 us, in three parts each 17.1)
+    const int32_t parts = m_all > 0 ? max(1, min(quads, warps / m_all)) : 1;
+    const int64_t items = (int64_t)m_all * parts;
+    if (warp >= items) return;
+    float2 wq[kVecPairs], wk[kVecPairs];
     if (!kRaw) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            wq[t] = make_float2(a.norm_q[8 * sub + 2 * t], a.norm_q[8 * sub + 2 * t + 1]);
-            wk[t] = make_float2(a.norm_k[8 * sub + 2 * t], a.norm_k[8 * sub + 2 * t + 1]);
+        for (int t = 0; t < kVecPairs; ++t) {
+            const int e = 2 * (kVecPairs * sub + t);
+            wq[t] = make_float2(a.norm_q[e], a.norm_q[e + 1]);
+            wk[t] = make_float2(a.norm_k[e], a.norm_k[e + 1]);
         }
     }
-    const int32_t m_all = min(a.count ? *a.count : a.host_count, a.n_tokens);
-    if (m_all <= 0) return;
-    const int32_t pairs = (a.n_heads + 1) >> 1;
-    const int32_t parts = max(1, min(pairs, warps / m_all));
-    const int64_t items = (int64_t)m_all * parts;
     for (int64_t item = warp; item < items; item += warps) {
         const int32_t m = (int32_t)(item / parts), part = (int32_t)(item - (int64_t)m * parts);
         const int32_t i = a.idx ? a.idx[m] : m;
@@ -335,70 +346,70 @@ __global__ void __launch_bounds__(kWriteThreads, 3) q8_write_kernel(const __grid
             continue;
         }
         const bool keep = !kRaw && a.save != nullptr && a.mask[i] == 1;
-        float cs[4], sn[4];
-        if (!kRaw) {
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float at = a.n_axes > 0 ? (float)a.pos[(int64_t)i * a.n_axes + axis[t]] : 0.f;
-                rope_turn(at, turns[t], &sn[t], &cs[t]);
+        uint4 nq[2], nk[2], nv[2];      // the next heads' vectors are on their way while these are worked on
+        auto load = [&](int32_t quad) {
+            const int32_t h = kVecHeads * quad + of;
+            const int64_t at = (int64_t)i * a.ld_qkv + (int64_t)(h < a.n_heads ? h : 0) * kHeadDim + 16 * sub;
+            const uint4* k = reinterpret_cast<const uint4*>(static_cast<const T*>(a.k) + at);
+            const uint4* v = reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + at);
+            if (!kRaw) {
+                const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at);
+                nq[0] = __ldcs(q);
+                nq[1] = __ldcs(q + 1);
             }
-        }
-        uint4 nq, nk, nv;      // the next head pair's vectors are on their way while one is worked on
-        auto load = [&](int32_t pr) {
-            const int32_t h = 2 * pr + half;
-            const int64_t at = (int64_t)i * a.ld_qkv + (int64_t)(h < a.n_heads ? h : 0) * kHeadDim + 8 * sub;
-            if (!kRaw) nq = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at));
-            nk = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.k) + at));
-            nv = __ldcs(reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + at));
+            nk[0] = __ldcs(k);
+            nk[1] = __ldcs(k + 1);
+            nv[0] = __ldcs(v);
+            nv[1] = __ldcs(v + 1);
         };
         load(part);
-        for (int32_t pr = part; pr < pairs; pr += parts) {
-            const int32_t h = 2 * pr + half;
+        float cs[kVecPairs], sn[kVecPairs];
+        if (!kRaw) {
+#pragma unroll
+            for (int t = 0; t < kVecPairs; ++t) {
+                const int j = kVecPairs * sub + t;
+                const float at = a.n_axes > 0 ? (float)a.pos[(int64_t)i * a.n_axes + a.axis[j]] : 0.f;
+                rope_turn(at, a.turns[j], &sn[t], &cs[t]);
+            }
+        }
+        for (int32_t quad = part; quad < quads; quad += parts) {
+            const int32_t h = kVecHeads * quad + of;
             const bool active = h < a.n_heads;
-            const int64_t col = (int64_t)(active ? h : 0) * kHeadDim + 8 * sub;
-            const uint4 xq = nq, xk = nk, xv = nv;
-            if (pr + parts < pairs) load(pr + parts);
-            uint8_t* ck = a.c.k + (int64_t)i * a.c.ld + (col - 8 * sub);
-            uint8_t* cv = a.c.v + (int64_t)i * a.c.ld + (col - 8 * sub);
+            const int64_t col = (int64_t)(active ? h : 0) * kHeadDim;
+            uint8_t* ck = a.c.k + (int64_t)i * a.c.ld + col;
+            uint8_t* cv = a.c.v + (int64_t)i * a.c.ld + col;
             T* ks = static_cast<T*>(a.c.ks) + (int64_t)(active ? h : 0) * a.c.ld_scale + i;
             T* vs = static_cast<T*>(a.c.vs) + (int64_t)(active ? h : 0) * a.c.ld_scale + i;
             if (keep && active) {
                 uint8_t* sv = a.save + (int64_t)m * a.ld_save;
                 const int64_t C = (int64_t)a.n_heads * kHeadDim;
-                *reinterpret_cast<uint2*>(sv + col) = *reinterpret_cast<const uint2*>(ck + 8 * sub);
-                *reinterpret_cast<uint2*>(sv + C + col) = *reinterpret_cast<const uint2*>(cv + 8 * sub);
+                *reinterpret_cast<uint4*>(sv + col + 16 * sub) = *reinterpret_cast<const uint4*>(ck + 16 * sub);
+                *reinterpret_cast<uint4*>(sv + C + col + 16 * sub) = *reinterpret_cast<const uint4*>(cv + 16 * sub);
                 if (sub == 0) {
                     T* ss = reinterpret_cast<T*>(sv + 2 * C);
                     ss[h] = *ks;
                     ss[a.n_heads + h] = *vs;
                 }
             }
-            float y[8];
+            float2 y[kVecPairs];
             if (!kRaw) {
-                norm_rope8<T>(xq, wq, a.eps, cs, sn, y);
+                unpack16<T>(nq, y);
+                norm_rope16(y, wq, a.eps, cs, sn);
                 if (active) {
-                    const uint4 o = make_uint4(StoreT<T>::pack2(y[0], y[1]), StoreT<T>::pack2(y[2], y[3]),
-                                               StoreT<T>::pack2(y[4], y[5]), StoreT<T>::pack2(y[6], y[7]));
-                    *reinterpret_cast<uint4*>(static_cast<T*>(a.qc) + (int64_t)m * a.ld_qc + col) = o;
-                }
-                norm_rope8<T>(xk, wk, a.eps, cs, sn, y);
-            } else {
-                const uint32_t u[4] = {xk.x, xk.y, xk.z, xk.w};
+                    uint4* q = reinterpret_cast<uint4*>(static_cast<T*>(a.qc) + (int64_t)m * a.ld_qc + col + 16 * sub);
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const float2 p = StoreT<T>::unpack2(u[t]);
-                    y[2 * t] = p.x;
-                    y[2 * t + 1] = p.y;
+                    for (int e = 0; e < 2; ++e)
+                        q[e] = make_uint4(StoreT<T>::pack2(y[4 * e].x, y[4 * e].y), StoreT<T>::pack2(y[4 * e + 1].x, y[4 * e + 1].y),
+                                          StoreT<T>::pack2(y[4 * e + 2].x, y[4 * e + 2].y),
+                                          StoreT<T>::pack2(y[4 * e + 3].x, y[4 * e + 3].y));
                 }
             }
+            unpack16<T>(nk, y);
+            const uint4 xv[2] = {nv[0], nv[1]};
+            if (quad + parts < quads) load(quad + parts);
+            if (!kRaw) norm_rope16(y, wk, a.eps, cs, sn);
             quantise_store<T, F, kRaw>(y, ck, ks, sub, active);
-            const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const float2 p = StoreT<T>::unpack2(u[t]);
-                y[2 * t] = p.x;
-                y[2 * t + 1] = p.y;
-            }
+            unpack16<T>(xv, y);
             quantise_store<T, F, true>(y, cv, vs, sub, active);
         }
     }

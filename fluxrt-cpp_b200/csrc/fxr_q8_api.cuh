@@ -79,9 +79,9 @@ int32_t launch_q8_write(const fxr_frame_desc* d, const fxr_q8_cache* cache, fxr:
     a.eps = d->eps;
     a.ld_save = q8_save_bytes(d);
     fill_turns(d, &a);
-    const int64_t units = max_rows * ((d->n_heads + 1) / 2);
+    const int64_t units = max_rows * ((d->n_heads + fxr::q8::kVecHeads - 1) / fxr::q8::kVecHeads);
     const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((units + fxr::q8::kWriteWarps - 1) / fxr::q8::kWriteWarps,
-                                                                (int64_t)sm_count() * 3));
+                                                                (int64_t)sm_count() * 2));
     return q8_dispatch(d->dtype, cache->format, [&](auto t, auto f) -> int32_t {
         using T = decltype(t);
         constexpr int F = decltype(f)::value;
@@ -325,8 +325,10 @@ int32_t fxr_cache_read_q8(const fxr_frame_desc* desc, const fxr_q8_cache* cache,
         return fail(FXR_ERR_INVALID, "ld must be a multiple of 8, >= n_heads*head_dim");
     fxr::q8::ReadArgs a{q8_arg(cache), idx, count, host_count, k, v, ld, cache->n_rows, desc->n_heads};
     const int64_t units = (int64_t)(count ? cache->n_rows : host_count) * desc->n_heads * (fxr::kHeadDim / 16);
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((units + fxr::q8::kReadThreads - 1) / fxr::q8::kReadThreads,
-                                                                (int64_t)sm_count() * 8));
+    // CTAs per SM at most: short ones that the hardware balances for a whole cache (16896 rows: 58 us
+    // against 67 us with 16), fewer where most may find nothing to do (1153 of 4608 rows: 6.3 against 6.8)
+    const int64_t ctas = (units + fxr::q8::kReadThreads - 1) / fxr::q8::kReadThreads, sms = sm_count();
+    const int grid = (int)std::max<int64_t>(1, std::min(ctas, sms * (ctas > sms * 32 ? 64 : 16)));
     return q8_dispatch(desc->dtype, cache->format, [&](auto t, auto f) -> int32_t {
         using T = decltype(t);
         constexpr int F = decltype(f)::value;
