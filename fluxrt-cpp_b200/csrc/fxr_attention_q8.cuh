@@ -41,17 +41,17 @@ struct Params {
 
 // ---------------------------------------------------------------------------------------------
 // Few rows per stream: bound by reading the cache once. Work is laid on a line of columns, each the
-// keys of one source for one head and one group of 8 or 16 rows: first (head, group of the packed rows
-// of all streams) against the prefix, so that the prefix is read once for every 16 rows of all
+// keys of one source for one head and one group of 8, 16 or 32 rows: first (head, group of the packed
+// rows of all streams) against the prefix, so that the prefix is read once for every 32 rows of all
 // streams, then (stream, head, group) against the stream's own rows. Where there are at least as many
 // CTAs as columns, every column is cut into parts of one length, the shortest (in units of 64 keys)
 // that gives every part a CTA of its own. Otherwise the line is cut into one range per CTA, and a range
 // covers a few items (parts of columns). An item costs its CTA about 6 us besides its keys (queries,
 // first copies, exchange, arrival: as long as 700 keys), so ranges that straddle columns are avoided
 // where they can be.
-// A CTA's 16 warps walk an item in blocks of 16 keys, each warp with its own running maximum, sum and
-// O, so that none waits for another. A warp streams its blocks through a ring of 3 in shared memory
-// by TMA (4 KB of codes per block: ~130 KB in flight per SM; one lane issues a block's copies, where
+// A CTA's 8 or 16 warps walk an item in blocks of 16 keys, each warp with its own running maximum, sum and
+// O, so that none waits for another. A warp streams its blocks through a ring in shared memory by
+// TMA (4 KB of codes per block: ~130 KB in flight per SM; one lane issues a block's copies, where
 // 16-byte asynchronous copies cost every lane eight addresses). The codes
 // become 16-bit operands in registers, between shared memory and mma.m16n8k16 with keys, then dims,
 // as its 16 rows and queries as its 8 columns (tcgen05 reads its operands from memory and wants 128
@@ -70,27 +70,30 @@ struct Params {
 // Partial results (O, maximum, sum) meet in L2: the last of a row group's parts to arrive combines
 // them in key order, so the result does not depend on the order of arrival.
 // ---------------------------------------------------------------------------------------------
-constexpr int kRowsWarps = 16;
-constexpr int kRowsThreads = 32 * kRowsWarps;
-constexpr int kRowsMax = 16;                   // rows of a group, at most
+constexpr int kRowsMax = 32;                   // rows of a group, at most
 constexpr int kBlk = 16;                       // keys per block
-constexpr int kDepth = 3;                      // ring
-constexpr int kUnitKeys = 64;                  // the line is cut at multiples of this
-constexpr int kMaxRowsPerStream = 64;          // what the launch accepts
+constexpr int kUnitKeys = 64;                  // columns are cut at multiples of this
+constexpr int kMaxRowsPerStream = 32;          // what the launch accepts
 constexpr int kGroupsPerStream = kMaxRowsPerStream / 8;
 constexpr uint32_t kBlkBytes = kBlk * 128;     // codes of one of K, V (128-byte swizzle)
 constexpr uint32_t kRingSlot = 2 * kBlkBytes;
-constexpr uint32_t kRingWarp = kDepth * kRingSlot;
 constexpr uint32_t kScaleSlot = 2 * kBlk * 2;  // a block's K scales, V scales
 constexpr int kPadRow = 132;                   // floats per O row in the warps' exchange
 constexpr uint32_t kQPad = 272;                // bytes per query row
-constexpr uint32_t kRowsSmemScale = kRowsWarps * kRingWarp;
-constexpr uint32_t kRowsSmemQ = kRowsSmemScale + kRowsWarps * kDepth * kScaleSlot;
-constexpr uint32_t kRowsSmemM = kRowsSmemQ + kRowsMax * kQPad;             // maxima, then sums: [16 rows][warps]
-constexpr uint32_t kRowsSmemBar = kRowsSmemM + (2 * kRowsWarps + 1) * kRowsMax * 4;   // (and the queries' factors)
-constexpr uint32_t kRowsSmem = kRowsSmemBar + kRowsWarps * kDepth * 8 + 1024;   // + alignment slack
 constexpr int kRowsSlotFloats = kRowsMax * kHeadDim + 2 * kRowsMax;
-static_assert(kRowsWarps * kRowsMax * kPadRow * 4 <= kRowsWarps * kRingWarp, "exchange fits the ring");
+// Shape of the kernel for groups of 8 * NQ rows: up to 16 rows 16 warps with 128 registers and a ring of
+// 3 blocks each; 32 rows, whose O alone is 128 registers, 8 warps and rings of 5.
+template <int NQ> struct RowsShape {
+    static constexpr int rows = 8 * NQ, warps = NQ > 2 ? 8 : 16, threads = 32 * warps, depth = NQ > 2 ? 5 : 3;
+    static constexpr uint32_t ring_warp = depth * kRingSlot;
+    static constexpr uint32_t at_scale = warps * ring_warp;
+    static constexpr uint32_t at_q = at_scale + warps * depth * kScaleSlot;
+    static constexpr uint32_t at_m = at_q + rows * kQPad;               // maxima, sums: [rows][warps]; queries' factors
+    static constexpr uint32_t at_bar = at_m + (2 * warps + 1) * rows * 4;
+    static constexpr uint32_t smem = at_bar + warps * depth * 8 + 1024; // + alignment slack
+    static_assert(warps * rows * kPadRow * 4 <= warps * ring_warp, "the exchange fits the ring");
+    static_assert(smem <= 230000 && at_bar % 8 == 0, "shared memory budget");
+};
 
 // Orders this thread's shared-memory accesses before later ones of the asynchronous proxy.
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -197,94 +200,95 @@ __device__ __forceinline__ void parts_of(const RowsPlan& r, int32_t n_heads, int
     }
 }
 
-// Own group (stream b, group g) of head h: every part of its rows, in key order, a row per warp.
+// Own group (stream b, group g) of head h: every part of its rows, in key order, a warp per row.
 template <typename T, int R>
 __device__ __noinline__ void rows_combine(const Params& p, const RowsPlan& r, int32_t h, int32_t b, int32_t g) {
-    const int lane = threadIdx.x & 31;
-    const int32_t m = g * R + (threadIdx.x >> 5);
-    if ((threadIdx.x >> 5) >= R || m >= r.rows[b]) return;
-    const int32_t* idx = nullptr;
-    void* out_base = nullptr;
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    for (int32_t m = g * R + (threadIdx.x >> 5); m < min((g + 1) * R, r.rows[b]); m += warps) {
+        const int32_t* idx = nullptr;
+        void* out_base = nullptr;
 #pragma unroll
-    for (int k = 0; k < kMaxBatch; ++k)
-        if (k == b) {
-            idx = p.s[k].idx;
-            out_base = p.s[k].out;
-        }
-    const int32_t i = idx[m];
-    // parts: the packed row's prefix column's, then the own column's
-    int32_t n_pre = 0, pre_slot = 0, own_slot, n;
-    const int32_t pr = r.first[b] + m;
-    if (r.gp > 0) parts_of(r, p.n_heads, h * r.gp + pr / R, pre_slot, n_pre);
-    const int32_t groups = (r.rows[b] + R - 1) / R;
-    parts_of(r, p.n_heads, p.n_heads * (r.gp + r.group0[b]) + h * groups + g, own_slot, n);
-    n += n_pre;
-    auto slot = [&](int32_t c) {
-        return p.part + (int64_t)(c < n_pre ? pre_slot + c : own_slot + c - n_pre) * kRowsSlotFloats;
-    };
-    auto row_of = [&](int32_t c) { return c < n_pre ? pr % R : m % R; };
-    // 32 parts at a time: lane c holds part c's maximum and sum, all lanes 8 parts' positions, every load
-    // of a round in flight together (one round trip to L2 for up to 8 parts)
-    float top = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int32_t c0 = 0; c0 < n; c0 += 32) {
-        float m_c = -INFINITY, l_c = 0.f;
-        if (c0 + lane < n) {
-            const float* q = slot(c0 + lane) + kRowsMax * kHeadDim + row_of(c0 + lane);
-            m_c = __ldcg(q);
-            l_c = __ldcg(q + kRowsMax);
-        }
-        float w = 0.f;
-        for (int32_t c1 = c0; c1 < min(n, c0 + 32); c1 += 8) {
-            float4 x[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                x[k] = c1 + k < n ? __ldcg(reinterpret_cast<const float4*>(slot(c1 + k) + row_of(c1 + k) * kHeadDim) + lane)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-            if (c1 == c0) {
-                float t = m_c;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-                t = fmaxf(t, top);
-                const float base = t == -INFINITY ? 0.f : t, al = ex2_approx(top - base);
-                l *= al;
-                acc = make_float4(acc.x * al, acc.y * al, acc.z * al, acc.w * al);
-                top = t;
-                w = ex2_approx(m_c - base);
-                l += w * l_c;
+        for (int k = 0; k < kMaxBatch; ++k)
+            if (k == b) {
+                idx = p.s[k].idx;
+                out_base = p.s[k].out;
             }
+        const int32_t i = idx[m];
+        // parts: the packed row's prefix column's, then the own column's
+        int32_t n_pre = 0, pre_slot = 0, own_slot, n;
+        const int32_t pr = r.first[b] + m;
+        if (r.gp > 0) parts_of(r, p.n_heads, h * r.gp + pr / R, pre_slot, n_pre);
+        const int32_t groups = (r.rows[b] + R - 1) / R;
+        parts_of(r, p.n_heads, p.n_heads * (r.gp + r.group0[b]) + h * groups + g, own_slot, n);
+        n += n_pre;
+        auto slot = [&](int32_t c) {
+            return p.part + (int64_t)(c < n_pre ? pre_slot + c : own_slot + c - n_pre) * kRowsSlotFloats;
+        };
+        auto row_of = [&](int32_t c) { return c < n_pre ? pr % R : m % R; };
+        // 32 parts at a time: lane c holds part c's maximum and sum, all lanes 8 parts' positions, every load
+        // of a round in flight together (one round trip to L2 for up to 8 parts)
+        float top = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int32_t c0 = 0; c0 < n; c0 += 32) {
+            float m_c = -INFINITY, l_c = 0.f;
+            if (c0 + lane < n) {
+                const float* q = slot(c0 + lane) + kRowsMax * kHeadDim + row_of(c0 + lane);
+                m_c = __ldcg(q);
+                l_c = __ldcg(q + kRowsMax);
+            }
+            float w = 0.f;
+            for (int32_t c1 = c0; c1 < min(n, c0 + 32); c1 += 8) {
+                float4 x[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float wc = __shfl_sync(0xffffffffu, w, c1 + k - c0);
-                acc.x += wc * x[k].x;
-                acc.y += wc * x[k].y;
-                acc.z += wc * x[k].z;
-                acc.w += wc * x[k].w;
+                for (int k = 0; k < 8; ++k)
+                    x[k] = c1 + k < n ? __ldcg(reinterpret_cast<const float4*>(slot(c1 + k) + row_of(c1 + k) * kHeadDim) + lane)
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+                if (c1 == c0) {
+                    float t = m_c;
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+                    t = fmaxf(t, top);
+                    const float base = t == -INFINITY ? 0.f : t, al = ex2_approx(top - base);
+                    l *= al;
+                    acc = make_float4(acc.x * al, acc.y * al, acc.z * al, acc.w * al);
+                    top = t;
+                    w = ex2_approx(m_c - base);
+                    l += w * l_c;
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float wc = __shfl_sync(0xffffffffu, w, c1 + k - c0);
+                    acc.x += wc * x[k].x;
+                    acc.y += wc * x[k].y;
+                    acc.z += wc * x[k].z;
+                    acc.w += wc * x[k].w;
+                }
             }
         }
-    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (i < 0 || i >= p.n_tokens) {
-        if (lane == 0) atomicOr(&g_error_word, kErrBounds);
-        return;
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (i < 0 || i >= p.n_tokens) {
+            if (lane == 0) atomicOr(&g_error_word, kErrBounds);
+            continue;
+        }
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        // position 8 d + e of a stored row is dim 16 key_of(e) + d: this lane's e = 4 (lane & 1) + 0..3
+        uint16_t* out = reinterpret_cast<uint16_t*>(static_cast<T*>(out_base) + (int64_t)i * p.ld_out + (int64_t)h * kHeadDim) +
+                        (lane >> 1);
+        const uint32_t lo = StoreT<T>::pack2(acc.x * inv, acc.y * inv), hi = StoreT<T>::pack2(acc.z * inv, acc.w * inv);
+        const int e = 4 * (lane & 1);
+        out[16 * key_of(e)] = (uint16_t)lo;
+        out[16 * key_of(e + 1)] = (uint16_t)(lo >> 16);
+        out[16 * key_of(e + 2)] = (uint16_t)hi;
+        out[16 * key_of(e + 3)] = (uint16_t)(hi >> 16);
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    // position 8 d + e of a stored row is dim 16 key_of(e) + d: this lane's e = 4 (lane & 1) + 0..3
-    uint16_t* out = reinterpret_cast<uint16_t*>(static_cast<T*>(out_base) + (int64_t)i * p.ld_out + (int64_t)h * kHeadDim) +
-                    (lane >> 1);
-    const uint32_t lo = StoreT<T>::pack2(acc.x * inv, acc.y * inv), hi = StoreT<T>::pack2(acc.z * inv, acc.w * inv);
-    const int e = 4 * (lane & 1);
-    out[16 * key_of(e)] = (uint16_t)lo;
-    out[16 * key_of(e + 1)] = (uint16_t)(lo >> 16);
-    out[16 * key_of(e + 2)] = (uint16_t)hi;
-    out[16 * key_of(e + 3)] = (uint16_t)(hi >> 16);
 }
 
 // NQ: 8-row tiles of a group.
 template <typename T, int F, int NQ>
-__global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_constant__ RowsMaps maps, const __grid_constant__ Params p) {
-    constexpr int R = 8 * NQ;
+__global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const __grid_constant__ RowsMaps maps, const __grid_constant__ Params p) {
+    using Sh = RowsShape<NQ>;
+    constexpr int R = Sh::rows, kRowsWarps = Sh::warps, kDepth = Sh::depth;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ RowsPlan r;
@@ -293,8 +297,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
     __shared__ uint32_t ready;                 // own groups whose last part this CTA delivered
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
-    const uint32_t base = smem_u32(smem), ring = base + warp * kRingWarp, q_at = base + kRowsSmemQ;
-    const uint32_t bars = base + kRowsSmemBar + warp * kDepth * 8;
+    const uint32_t base = smem_u32(smem), ring = base + warp * Sh::ring_warp, q_at = base + Sh::at_q;
+    const uint32_t bars = base + Sh::at_bar + warp * kDepth * 8;
     uint32_t it = 0;                           // blocks of this warp so far
     if (threadIdx.x == 0) abort = 0;
     if (lane == 0) {
@@ -302,7 +306,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
         fence_mbar_init();
     }
     float* xo = reinterpret_cast<float*>(smem);                                     // [warp][R][kPadRow]
-    float* xm = reinterpret_cast<float*>(smem + kRowsSmemM);                        // [R][warp] maxima, then sums
+    float* xm = reinterpret_cast<float*>(smem + Sh::at_m);                        // [R][warp] maxima, then sums
     pdl_launch_dependents();
     pdl_wait();
     if (warp == 0) {
@@ -413,7 +417,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
         auto fetch = [&](int32_t b, uint32_t nth) {
             if (lane == 0) {
                 const uint32_t slot = nth % kDepth, bar = bars + 8 * slot, dst = ring + slot * kRingSlot;
-                const uint32_t sdst = base + kRowsSmemScale + (warp * kDepth + slot) * kScaleSlot;
+                const uint32_t sdst = base + Sh::at_scale + (warp * kDepth + slot) * kScaleSlot;
                 const uint32_t sbytes = n_keys - b * kBlk > 8 ? 32u : 16u;
                 mbar_arrive_expect_tx(bar, kRingSlot + 2 * sbytes);
                 tma_load_2d(dst, tk, bar, h * kHeadDim, k0 + b * kBlk);
@@ -459,14 +463,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                 if (k == b) st = &p.s[k];
             return st;
         };
-        float* q_factor = xm + 2 * kRowsWarps * kRowsMax;      // what a row's queries were divided by
-        if (threadIdx.x < R * 16) {                            // whole warps: a row per half-warp
+        float* q_factor = xm + 2 * kRowsWarps * R;      // what a row's queries were divided by
+        for (int e0 = threadIdx.x; e0 < R * 16; e0 += Sh::threads) {      // whole warps: a row per half-warp
             int32_t b, m;
             uint4 x = make_uint4(0, 0, 0, 0);
-            if (row_at(threadIdx.x >> 4, b, m)) {
+            if (row_at(e0 >> 4, b, m)) {
                 const Stream* st = stream_of(b);
                 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(st->qc) + (int64_t)m * st->ld_qc + (int64_t)h * kHeadDim +
-                                                    (threadIdx.x & 15) * 8);
+                                                    (e0 & 15) * 8);
             }
             float factor = 1.f;
             if constexpr (StoreT<T>::kUmmaFormat == 1) {
@@ -487,8 +491,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                     w[k] = StoreT<__half>::pack2(v.x * inv, v.y * inv);
                 }
             }
-            if ((threadIdx.x & 15) == 0) q_factor[threadIdx.x >> 4] = factor;
-            sts128(q_at + (threadIdx.x >> 4) * kQPad + (threadIdx.x & 15) * 16, x);
+            if ((e0 & 15) == 0) q_factor[e0 >> 4] = factor;
+            sts128(q_at + (e0 >> 4) * kQPad + (e0 & 15) * 16, x);
         }
         uint32_t qg[NQ][2];
 #pragma unroll
@@ -541,8 +545,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
             groups_of(b + kRowsWarps);
             const uint32_t slot = it % kDepth;
             if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * slot, (it / kDepth) & 1, &abort))) break;
-            const uint8_t* blk_p = smem + warp * kRingWarp + slot * kRingSlot;
-            const uint16_t* sc_p = reinterpret_cast<const uint16_t*>(smem + kRowsSmemScale + (warp * kDepth + slot) * kScaleSlot);
+            const uint8_t* blk_p = smem + warp * Sh::ring_warp + slot * kRingSlot;
+            const uint16_t* sc_p = reinterpret_cast<const uint16_t*>(smem + Sh::at_scale + (warp * kDepth + slot) * kScaleSlot);
             // S^T = K Q^T
             float s[NQ][4];
 #pragma unroll
@@ -558,7 +562,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                     uint4 q4[NQ];
 #pragma unroll
                     for (int q = 0; q < NQ; ++q)
-                        q4[q] = *reinterpret_cast<const uint4*>(smem + kRowsSmemQ + (g + 8 * q) * kQPad + (cc * 64 + t * 16 + jp * 8) * 2);
+                        q4[q] = *reinterpret_cast<const uint4*>(smem + Sh::at_q + (g + 8 * q) * kQPad + (cc * 64 + t * 16 + jp * 8) * 2);
 #pragma unroll
                     for (int jj = 0; jj < 2; ++jj) {
                         const int j = 2 * jp + jj;
@@ -713,17 +717,16 @@ __global__ void __launch_bounds__(kRowsThreads, 1) rows_kernel(const __grid_cons
                 }
             }
         __syncthreads();
-        if (warp < live) {
-            const int row = warp;
+        for (int row = warp; row < live; row += kRowsWarps) {
             const float m_w = lane < kRowsWarps ? xm[row * kRowsWarps + lane] : -INFINITY;
             float top = m_w;
 #pragma unroll
-            for (int e = 8; e > 0; e >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
+            for (int e = kRowsWarps / 2; e > 0; e >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
             top = __shfl_sync(0xffffffffu, top, 0);
             const float f = ex2_approx(m_w - (top == -INFINITY ? 0.f : top));
             float l = lane < kRowsWarps ? f * xm[(R + row) * kRowsWarps + lane] : 0.f;
 #pragma unroll
-            for (int e = 8; e > 0; e >>= 1) l += __shfl_xor_sync(0xffffffffu, l, e);
+            for (int e = kRowsWarps / 2; e > 0; e >>= 1) l += __shfl_xor_sync(0xffffffffu, l, e);
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < kRowsWarps; ++k) {
@@ -841,10 +844,11 @@ constexpr uint32_t kRegsSoftmax = 176, kRegsOther = 80;
 constexpr uint32_t kTileRegPool = 256 * kRegsSoftmax + 256 * kRegsOther;
 static_assert(kTileRegPool == kTileThreads * 128, "the warpgroups' shares are the launch's registers");
 constexpr int kPolyPeriod = 4;
-constexpr float kItemSteps = 2.0f, kCutSteps = 4.5f;   // an item's and the combine's cost, in steps (2.6 us each)
+// Costs in steps (2.6 us each): an item's start and end; a cut (partial results, the combine's launch);
+// a part in the combine of its unit.
+constexpr float kItemSteps = 2.0f, kCutSteps = 2.5f, kPartSteps = 0.25f;
 constexpr int kPartSlots = 4;                    // partial tiles a CTA may write
 constexpr int kPartFloats = kBM * kD + 2 * kBM;
-constexpr int kPartWarps = 8;                    // arrival counters per cut unit
 constexpr uint32_t kMixed = 1u << 24;            // step information: tile | left << 16 | kMixed
 
 struct TileMaps {
@@ -863,9 +867,7 @@ struct Item {
     void* out;
     const uint16_t* list;        // visible steps of the unit, NULL: all
     int32_t n, s0, head, row0, rows;
-    int32_t cut;                 // part of a unit
-    int32_t c_first, c_last;     // CTAs that hold the unit's parts
-    int32_t i0;                  // its first iteration in the launch
+    float* part;                 // where the item's partial result goes, NULL: it is a whole unit
     int32_t stream;
 };
 
@@ -889,6 +891,40 @@ constexpr uint32_t kTileSmem = kSmBar + 256 + 1024;
 static_assert(sizeof(Item) <= 160 && kNumBars * 8 + 8 <= 256 && kSmBar % 8 == 0 && kSmItem % 16 == 0, "shared memory layout");
 static_assert(kTileSmem <= 232448, "shared memory budget");
 
+// How n_units units of `total` steps together run on `grid` CTAs: whole, round-robin (per = parts = 0);
+// each unit in `parts` equal parts with a CTA each; or the launch's steps, unit after unit, in ranges of
+// `per` per CTA. The cheapest by the costs above.
+struct TileSchedule {
+    int32_t per, parts;
+};
+__host__ __device__ inline TileSchedule tile_schedule(int32_t total, int32_t n_units, int32_t grid) {
+    TileSchedule s{0, 0};
+    if (n_units == 0) return s;
+    const int32_t each = (total + grid - 1) / grid, most = grid / n_units;
+    const float avg = (float)total / (float)n_units;
+    float best = (float)((n_units + grid - 1) / grid) * (avg + kItemSteps);
+    const float cut = (float)each + kItemSteps * ((float)each / avg + 1.f) + kCutSteps + kPartSteps * (avg / (float)each + 1.f);
+    if (cut < best) {
+        best = cut;
+        s.per = each;
+    }
+    for (int32_t n = 2; n <= most && (float)n <= avg + 1.f; ++n) {
+        const float even = ceilf(avg / (float)n) + kItemSteps + kCutSteps + kPartSteps * (float)n;
+        if (even <= best) {
+            best = even;
+            s = TileSchedule{0, n};
+        }
+    }
+    return s;
+}
+
+// A unit that was cut, written by the scheduler that starts it: slot 2 c + k for part slot k of CTA c.
+struct CutUnit {
+    int32_t parts;               // 0: none
+    int32_t stream, head, row0, rows;
+    int32_t c_first, i0, per;
+};
+
 struct TileParams {
     Params p;
     int32_t n_pre, n_own;        // key tiles of the prefix and of a stream's own rows
@@ -896,8 +932,9 @@ struct TileParams {
     const int32_t* steps;        // [stream][units_cap] listed steps, NULL: every unit runs all tiles
     const uint16_t* list;        // [stream][units_cap][n_pre + n_own] tile | 0x8000 where it needs the masks
     const uint32_t* groups;      // [n_pre + n_streams * n_own][128] key groups, zeros past a source's end
+    int32_t may_cut;             // 0: whole units only (no combine follows)
     float* part;                 // [grid][kPartSlots][kPartFloats]
-    int32_t* cnt;                // [grid][kPartWarps], zero between launches
+    CutUnit* cuts;               // [grid][2]
 };
 
 // ---- visible steps --------------------------------------------------------------------------------
@@ -1047,101 +1084,107 @@ __device__ __forceinline__ int64_t part_at(int32_t i0, int32_t per, int32_t c, i
     return (((int64_t)c * 2 + k) * 2 + t) * kPartFloats;
 }
 
-// The last part of a unit to arrive combines row r of tile t over all parts, in key order.
-template <typename T>
-__device__ __forceinline__ void combine_parts(const float* part, int32_t i0, int32_t per, int32_t c0, int32_t c1, int t, int r,
-                                              T* out_row) {
-    float top = -INFINITY, l = 0.f;
-    for (int32_t c = c0; c <= c1; c += 4) {              // four parts' maxima and sums in flight together
-        float m4[4], l4[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float* q = part + part_at(i0, per, min(c + e, c1), t) + kBM * kD + r;
-            m4[e] = c + e <= c1 ? __ldcg(q) : -INFINITY;
-            l4[e] = c + e <= c1 ? __ldcg(q + kBM) : 0.f;
-        }
-        const float next = fmaxf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), top);
-        const float base = next == -INFINITY ? 0.f : next;
-        l *= ex2_approx(top - base);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) l += ex2_approx(m4[e] - base) * l4[e];
-        top = next;
-    }
-    if (top == -INFINITY) top = 0.f;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+// End of an item that is part of a unit: its O rows, maxima and sums go to scratch and O is released.
+// Out of line, as in the 16-bit kernel, so that the step loop around it keeps its code.
+__device__ __noinline__ void cut_epilogue(float* slot, int r, uint32_t tO, float m_run, float l_run, bool blind, bool live,
+                                          uint32_t ofree) {
+    if (__any_sync(0xffffffffu, live)) {
 #pragma unroll 1
-    for (int h = 0; h < 4; ++h) {
-        float acc[32];
+        for (int h = 0; h < 4; ++h) {
+            uint32_t o[32];
+            FXR_TMEM_LD32(tO + h * 32u, o);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) acc[k] = 0.f;
-#pragma unroll 1
-        for (int32_t c = c0; c <= c1; c += 2) {          // two parts' loads in flight together
-            float4 x[2][8];
-            float w[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const bool in = c + e <= c1;
-                const float* q = part + part_at(i0, per, in ? c + e : c, t);
-                w[e] = in ? __ldcg(q + kBM * kD + r) : -INFINITY;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[e][k] = __ldcg(reinterpret_cast<const float4*>(q) + (h * 8 + k) * kBM + r);
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float f = ex2_approx(w[e] - top);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    acc[4 * k] += f * x[e][k].x;
-                    acc[4 * k + 1] += f * x[e][k].y;
-                    acc[4 * k + 2] += f * x[e][k].z;
-                    acc[4 * k + 3] += f * x[e][k].w;
-                }
-            }
+            for (int k = 0; k < 8; ++k)
+                reinterpret_cast<float4*>(slot)[(h * 8 + k) * kBM + r] =
+                    blind ? make_float4(0.f, 0.f, 0.f, 0.f)
+                          : make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]),
+                                        __uint_as_float(o[4 * k + 3]));
         }
-        if (out_row != nullptr) {
-            uint4* dst = reinterpret_cast<uint4*>(out_row + 32 * h);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                dst[k] = make_uint4(StoreT<T>::pack2(acc[8 * k] * inv, acc[8 * k + 1] * inv),
-                                    StoreT<T>::pack2(acc[8 * k + 2] * inv, acc[8 * k + 3] * inv),
-                                    StoreT<T>::pack2(acc[8 * k + 4] * inv, acc[8 * k + 5] * inv),
-                                    StoreT<T>::pack2(acc[8 * k + 6] * inv, acc[8 * k + 7] * inv));
-        }
+        slot[kBM * kD + r] = m_run;
+        slot[kBM * kD + kBM + r] = l_run;
     }
-}
-
-// End of an item that is part of a unit: its O rows, maxima and sums go to scratch, O is released,
-// and the warp whose arrival completes the unit combines its 32 rows. Out of line, as in the 16-bit
-// kernel, so that the step loop around it keeps its code.
-template <typename T>
-__device__ __noinline__ void cut_epilogue(float* part, int32_t* counters, int32_t per, const Item* it, int t, int r, int warp,
-                                          uint32_t tO, float m_run, float l_run, bool blind, uint32_t ofree, T* out_row) {
-    const int32_t c = (int32_t)blockIdx.x, i0 = it->i0, c_first = it->c_first, c_last = it->c_last;
-    float* slot = part + part_at(i0, per, c, t);
-#pragma unroll 1
-    for (int h = 0; h < 4; ++h) {
-        uint32_t o[32];
-        FXR_TMEM_LD32(tO + h * 32u, o);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            reinterpret_cast<float4*>(slot)[(h * 8 + k) * kBM + r] =
-                blind ? make_float4(0.f, 0.f, 0.f, 0.f)
-                      : make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]),
-                                    __uint_as_float(o[4 * k + 3]));
-    }
-    slot[kBM * kD + r] = m_run;
-    slot[kBM * kD + kBM + r] = l_run;
     tc_fence_before();
     mbar_arrive(ofree);
-    __threadfence();
-    __syncwarp();
-    int32_t before = 0;
-    if (lane_id() == 0) before = atom_add_acq_rel_gpu(counters + c_last * kPartWarps + warp, 1);
-    before = __shfl_sync(0xffffffffu, before, 0);
-    if (before != c_last - c_first) return;
-    if (lane_id() == 0) counters[c_last * kPartWarps + warp] = 0;   // for the next launch
-    __threadfence();
-    combine_parts<T>(part, i0, per, c_first, c_last, t, r, out_row);
+}
+
+// Cut units' parts into their rows, in key order: a warp takes 32 rows by 16 columns of a unit (a row per
+// lane; partial O is stored column chunk by column chunk, so that its loads are whole lines), four CTAs
+// a unit. A launch of its own, chained to the tile kernel's end: its warps spread over all SMs, where a
+// combine by the last part to arrive read all of a unit's parts through one SM, 2.5 us per part (601 rows
+// of two streams, documents: 50 us with that, 41 with this). It costs a call about 5 us, so calls whose
+// units the host knows to stay whole go without.
+constexpr int kCombineThreads = 512, kCombineCtas = 4;   // threads of a CTA, CTAs of a unit
+
+template <typename T>
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ Params p, const float* part,
+                                                                  const CutUnit* cuts) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const CutUnit u = cuts[blockIdx.x / kCombineCtas];
+    if (u.parts == 0) return;
+    const int lane = threadIdx.x & 31, w = (int)(blockIdx.x % kCombineCtas) * (kCombineThreads / 32) + (threadIdx.x >> 5);
+    const int t = w >> 5, r = ((w >> 3) & 3) * 32 + lane, h = w & 7;     // tile, row, 16 columns
+    const int32_t row = u.row0 + t * kBM + r;
+    const bool live = row < u.rows;
+    if (!__any_sync(0xffffffffu, live)) return;
+    const int32_t* idx = nullptr;
+    void* out = nullptr;
+#pragma unroll
+    for (int b = 0; b < kMaxBatch; ++b)
+        if (b == u.stream) {
+            idx = p.s[b].idx;
+            out = p.s[b].out;
+        }
+    const int32_t i = live ? idx[row] : -1;
+    constexpr int kAhead = 4;                            // parts whose loads are in flight together
+    float top = -INFINITY, l = 0.f, acc[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) acc[k] = 0.f;
+    for (int32_t c = 0; c < u.parts; c += kAhead) {
+        float4 x[kAhead][4];
+        float m[kAhead], ls[kAhead], next = top;
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+            const bool in = c + e < u.parts;
+            const float* q = part + part_at(u.i0, u.per, u.c_first + (in ? c + e : c), t);
+            m[e] = in ? __ldcg(q + kBM * kD + r) : -INFINITY;
+            ls[e] = in ? __ldcg(q + kBM * kD + kBM + r) : 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[e][k] = __ldcg(reinterpret_cast<const float4*>(q) + (h * 4 + k) * kBM + r);
+        }
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) next = fmaxf(next, m[e]);
+        const float base = next == -INFINITY ? 0.f : next, al = ex2_approx(top - base);
+        top = next;
+        l *= al;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) acc[k] *= al;
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+            const float f = ex2_approx(m[e] - base);
+            l += f * ls[e];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                acc[4 * k] += f * x[e][k].x;
+                acc[4 * k + 1] += f * x[e][k].y;
+                acc[4 * k + 2] += f * x[e][k].z;
+                acc[4 * k + 3] += f * x[e][k].w;
+            }
+        }
+    }
+    if (!live) return;
+    if (i < 0 || i >= p.n_tokens) {
+        if (h == 0) atomicOr(&g_error_word, kErrBounds);
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(out) + (int64_t)i * p.ld_out + (int64_t)u.head * kD + 16 * h);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        dst[k] = make_uint4(StoreT<T>::pack2(acc[8 * k] * inv, acc[8 * k + 1] * inv),
+                            StoreT<T>::pack2(acc[8 * k + 2] * inv, acc[8 * k + 3] * inv),
+                            StoreT<T>::pack2(acc[8 * k + 4] * inv, acc[8 * k + 5] * inv),
+                            StoreT<T>::pack2(acc[8 * k + 6] * inv, acc[8 * k + 7] * inv));
 }
 
 template <typename T, int F>
@@ -1189,6 +1232,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
         tmem_alloc(smem_u32((const void*)tmem_slot), kTmemColumns);
         tmem_relinquish();
     }
+    if (warp == kProducerWarp && (int32_t)lane < p.n_streams) {
+        prefetch_tmap(&maps.q[lane]);
+        prefetch_tmap(&maps.k[lane]);
+        prefetch_tmap(&maps.v[lane]);
+        if (lane == 0 && p.n_prefix > 0) {
+            prefetch_tmap(&maps.pk);
+            prefetch_tmap(&maps.pv);
+        }
+    }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -1206,43 +1258,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
         stream_rows[threadIdx.x] = max(0, min(c, p.max_rows));
     }
     __syncthreads();
-    // The schedule, the same on every thread: whole units round-robin (per = parts = 0), units cut into
-    // `parts` equal parts with a CTA each (where there are at least twice as many CTAs as units), or
-    // the launch's iterations cut into ranges of `per` per CTA.
-    const int32_t n_steps = a.n_pre + a.n_own;
-    int32_t per = 0, parts = 0, total = 0, n_units = 0;
-    {
-#pragma unroll
-        for (int b = 0; b < kMaxBatch; ++b)
-            if (b < p.n_streams) {
-                const int32_t units = (stream_rows[b] + kUnitRows - 1) / kUnitRows;
-                n_units += units * p.n_heads;
-                if (a.steps == nullptr) {
-                    total += units * p.n_heads * n_steps;
-                } else {
-                    int32_t sum = 0;
-                    for (int32_t u = (int32_t)lane; u < units; u += 32) sum += a.steps[b * a.units_cap + u];
-                    total += __reduce_add_sync(0xffffffffu, sum) * p.n_heads;
-                }
-            }
-        const int32_t grid = (int32_t)gridDim.x;
-        const int32_t each = (total + grid - 1) / grid, split = n_units > 0 ? grid / n_units : 0;
-        const float avg = n_units > 0 ? (float)total / (float)n_units : 0.f;
-        const float whole = (float)((n_units + grid - 1) / grid) * (avg + kItemSteps);
-        const float cut = (float)each + kItemSteps * ((float)each / fmaxf(avg, 1.f) + 1.f) + kCutSteps;
-        const float even = split > 1 ? ceilf(avg / (float)split) + kItemSteps + kCutSteps : INFINITY;
-        if (fminf(cut, even) < whole) {
-            if (even <= cut) parts = split;
-            else per = each;
-        }
-    }
-
     if (warp >= kConvWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
         // ---------------- converters: one row of the tile per thread ----------------
         auto wwait = [&](uint32_t b_, uint32_t par_) -> bool { return __all_sync(0xffffffffu, mbar_wait(b_, par_, abort)); };
         const uint32_t r = (uint32_t)(warp - kConvWarp) * 32 + lane, x = r & 7;
-        constexpr uint32_t fmt16 = StoreT<T>::kUmmaFormat;
         uint32_t in = 0, step = 0;     // tiles converted, steps
         bool ok = true;
         for (uint32_t k = 0; ok; ++k) {
@@ -1294,31 +1314,40 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                         const int32_t left = pre ? p.n_prefix - tile * kBN : p.n_tokens - (tile - a.n_pre) * kBN;
                         info[step & 3] = (uint32_t)tile | ((uint32_t)min(left, kBN) << 16) | (list && (word & 0x8000u) ? kMixed : 0u);
                     }
-                    uint4 q[8];
-#pragma unroll
-                    for (uint32_t c = 0; c < 8; ++c) q[c] = lds128(src + ((c ^ x) << 4));
-                    if (in >= kTiles && !wwait(bar(kEmpty + ts), (in / kTiles - 1) & 1)) { ok = false; break; }
+                    const uint32_t f2 = StoreT<T>::pack2(f, f);
+                    auto store = [&](uint32_t c, const uint4& lo, const uint4& hi) {
+                        const uint32_t d = dst + (c >> 2) * kSpan;
+                        sts128(d + (((2 * (c & 3)) ^ x) << 4), lo);
+                        sts128(d + (((2 * (c & 3) + 1) ^ x) << 4), hi);
+                    };
+                    auto tile_free = [&]() { return in < kTiles || wwait(bar(kEmpty + ts), (in / kTiles - 1) & 1); };
+                    auto raw_done = [&]() {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar(kRawEmpty + rs));
+                    };
+                    if (!tile_free()) { ok = false; break; }
+                    // a loop of 4 chunks, not all 8 unrolled: the roles' code is longer than the instruction
+                    // caches hold (a quarter of a 2048 px frame: 1070 us, unrolled 1195)
                     auto convert = [&](auto dec) {
-                        dec.scale(StoreT<T>::pack2(f, f));
-#pragma unroll
+                        dec.scale(f2);
+                        uint4 next = lds128(src + (x << 4));
+#pragma unroll 4
                         for (uint32_t c = 0; c < 8; ++c) {
+                            const uint4 q = next;
+                            if (c < 7) next = lds128(src + (((c + 1) ^ x) << 4));
                             uint4 lo, hi;
-                            q8::decode16(q[c], dec, lo, hi);
-                            if (c == 7) {        // the codes are in registers: their buffer is free
-                                __syncwarp();
-                                if (lane == 0) mbar_arrive(bar(kRawEmpty + rs));
-                            }
-                            const uint32_t d = dst + (c >> 2) * kSpan;
-                            sts128(d + (((2 * (c & 3)) ^ x) << 4), lo);
-                            sts128(d + (((2 * (c & 3) + 1) ^ x) << 4), hi);
+                            q8::decode16(q, dec, lo, hi);
+                            store(c, lo, hi);
                         }
                     };
-                    if constexpr (F == q8::kE4m3 && fmt16 == 1) {
-                        if (__all_sync(0xffffffffu, !(f >= q8::kSmallScale))) convert(q8::SmallScaleDecoder{});
+                    if constexpr (q8::TileDecoder<T, F>::has_limit) {
+                        using Fast = typename q8::TileDecoder<T, F>::type;
+                        if (!__any_sync(0xffffffffu, f >= Fast::limit)) convert(Fast{});
                         else convert(q8::Decoder<T, F>{});
                     } else {
                         convert(q8::Decoder<T, F>{});
                     }
+                    raw_done();
                     fence_async_smem();      // the tensor core reads the tile through the async proxy
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(kFull + ts));
@@ -1461,19 +1490,38 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                 }
             }
         } else if (warp == kSchedWarp) {
-            // ---------------- scheduler ----------------
+            // ---------------- scheduler: the CTA's items, by a schedule that every CTA computes alike ----------
+            const int32_t n_steps = a.n_pre + a.n_own;
+            int32_t per = 0, parts = 0, total = 0, n_units = 0;
+#pragma unroll 1
+            for (int b = 0; b < p.n_streams; ++b) {
+                    const int32_t units = (stream_rows[b] + kUnitRows - 1) / kUnitRows;
+                    n_units += units * p.n_heads;
+                    if (a.steps == nullptr) {
+                        total += units * p.n_heads * n_steps;
+                    } else {
+                        int32_t sum = 0;
+                        for (int32_t u = (int32_t)lane; u < units; u += 32) sum += a.steps[b * a.units_cap + u];
+                        total += __reduce_add_sync(0xffffffffu, sum) * p.n_heads;
+                    }
+                }
+            if (a.may_cut) {
+                const TileSchedule sc = tile_schedule(total, n_units, (int32_t)gridDim.x);
+                per = sc.per;
+                parts = sc.parts;
+            }
             const int32_t grid = (int32_t)gridDim.x, c = (int32_t)blockIdx.x;
             int32_t cur = per > 0 ? (int32_t)min((int64_t)total, (int64_t)c * per) : parts > 0 ? c / parts : c;
             const int32_t end = per > 0 ? (int32_t)min((int64_t)total, (int64_t)cur + per) : n_units;
+            uint32_t cuts_made = 0;
             for (uint32_t k = 0;; ++k) {
                 bool more = cur < end;
                 // the unit: stream, head, first row, steps, first iteration
                 int32_t b = -1, rows = 0, head = 0, unit = 0, cnt = n_steps, rest = cur, i0 = cur;
                 if (more) {
                     int32_t units = 1;
-#pragma unroll
-                    for (int s = 0; s < kMaxBatch; ++s)
-                        if (b < 0 && s < p.n_streams) {
+#pragma unroll 1
+                    for (int s = 0; b < 0 && s < p.n_streams; ++s) {
                             const int32_t m = stream_rows[s];
                             const int32_t u = (m + kUnitRows - 1) / kUnitRows;
                             int32_t span = u;             // per head, in units or iterations
@@ -1526,49 +1574,46 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                         }
                     }
                 }
-                // the item's steps, and the CTAs that hold the unit's parts
-                int32_t s0 = 0, n = cnt, c_first = c, c_last = c;
+                // the item's steps
+                int32_t s0 = 0, n = cnt, of = 1;
                 if (per > 0) {
                     s0 = cur - i0;
                     n = min(cnt - s0, end - cur);
-                    c_first = i0 / per;
-                    c_last = (i0 + cnt - 1) / per;
+                    of = (i0 + cnt - 1) / per - i0 / per + 1;
                 } else if (parts > 0) {
-                    const int32_t e = c - cur * parts, of = min(parts, cnt);
+                    const int32_t e = c - cur * parts;
+                    of = min(parts, cnt);
                     more = more && e < of;
                     s0 = cnt * e / of;
                     n = cnt * (e + 1) / of - s0;
-                    c_first = c - e;
-                    c_last = c_first + of - 1;
                     i0 = 0;                               // the part is the CTA's first item
                 }
                 if (!more) n = 0;
+                if (lane == 0 && n > 0 && n < cnt && s0 == 0) {
+                    const int slot = i0 > c * per ? 1 : 0;
+                    a.cuts[2 * c + slot] = CutUnit{of, b, head, unit * kUnitRows, rows, c, i0, per};
+                    cuts_made |= 1u << slot;
+                }
                 if (k >= 2 && !__all_sync(0xffffffffu, mbar_wait(bar(kItemEmpty + (k & 1)), ((k >> 1) - 1) & 1, abort))) break;
                 Item* it = item_at(k);
                 if (lane == 0) {
                     it->n = n;
                     if (n > 0) {
-#pragma unroll
-                        for (int s = 0; s < kMaxBatch; ++s)
-                            if (s == b) {
-                                it->tq = &maps.q[s];
-                                it->tk = &maps.k[s];
-                                it->tv = &maps.v[s];
-                                it->ks = static_cast<const T*>(p.s[s].c.ks) + (int64_t)head * p.s[s].c.ld_scale;
-                                it->vs = static_cast<const T*>(p.s[s].c.vs) + (int64_t)head * p.s[s].c.ld_scale;
-                                it->idx = p.s[s].idx;
-                                it->qg = p.s[s].qg;
-                                it->out = p.s[s].out;
-                            }
+                        const Stream& st = a.p.s[b];
+                        it->tq = &maps.q[b];
+                        it->tk = &maps.k[b];
+                        it->tv = &maps.v[b];
+                        it->ks = static_cast<const T*>(st.c.ks) + (int64_t)head * st.c.ld_scale;
+                        it->vs = static_cast<const T*>(st.c.vs) + (int64_t)head * st.c.ld_scale;
+                        it->idx = st.idx;
+                        it->qg = st.qg;
+                        it->out = st.out;
                         it->s0 = s0;
                         it->head = head;
                         it->row0 = unit * kUnitRows;
                         it->rows = rows;
                         it->list = a.steps ? a.list + ((int64_t)b * a.units_cap + unit) * n_steps : nullptr;
-                        it->cut = n < cnt;
-                        it->i0 = i0;
-                        it->c_first = c_first;
-                        it->c_last = c_last;
+                        it->part = n < cnt ? a.part + part_at(i0, per, c, 0) : nullptr;
                         it->stream = b;
                     }
                     mbar_arrive(bar(kItemFull + (k & 1)));
@@ -1577,6 +1622,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                 if (n == 0) break;
                 cur = per > 0 ? cur + n : parts > 0 ? end : cur + grid;
             }
+            if (a.may_cut && lane < 2 && (cuts_made >> lane & 1u) == 0) a.cuts[2 * c + lane].parts = 0;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
@@ -1700,20 +1746,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
             if (!ok) break;
             if (!wwait(bar(kPVDone + t), (s_it - 1) & 1)) break;
             tc_fence_after();
-            T* out_row = nullptr;
-            if (live) {
-                const int32_t i = it->idx[it->row0 + t * kBM + r];
-                if (i >= 0 && i < p.n_tokens)
-                    out_row = static_cast<T*>(it->out) + (int64_t)i * p.ld_out + (int64_t)it->head * kD;
-                else
-                    atomicOr(&g_error_word, kErrBounds);
-            }
             const bool blind = it->list != nullptr && *my_groups == 0;   // the row's set is empty
             if (blind) m_run = -INFINITY;
             if (m_run == -INFINITY) l_run = 0.f;      // the row saw nothing
-            if (it->cut) {
-                cut_epilogue<T>(a.part, a.cnt, per, it, t, r, warp, tO, m_run, l_run, blind, bar(kOFree + t), out_row);
+            if (it->part != nullptr) {
+                cut_epilogue(it->part + t * kPartFloats, r, tO, m_run, l_run, blind, live, bar(kOFree + t));
             } else {
+                T* out_row = nullptr;
+                if (live) {
+                    const int32_t i = it->idx[it->row0 + t * kBM + r];
+                    if (i >= 0 && i < p.n_tokens)
+                        out_row = static_cast<T*>(it->out) + (int64_t)i * p.ld_out + (int64_t)it->head * kD;
+                    else
+                        atomicOr(&g_error_word, kErrBounds);
+                }
                 const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
 #pragma unroll 1
                 for (int h = 0; h < 4; ++h) {

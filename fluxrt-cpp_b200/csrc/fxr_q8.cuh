@@ -182,9 +182,9 @@ template <> struct Decoder<__nv_bfloat16, kE4m3> {
         return bits(__hmul2(__hmul2(as_bf(fields(w, a, b)), as_bf(0x7b807b80u)), s));
     }
 };
-// e4m3 -> bf16 for scales below kSmallScale (or NaN): one multiplication.
-constexpr float kSmallScale = 128.f;
+// e4m3 -> bf16 for scales below `limit` (or NaN): one multiplication.
 struct SmallScaleDecoder {
+    static constexpr float limit = 128.f;
     __nv_bfloat162 s;
     __device__ __forceinline__ void scale(uint32_t s2) { s = __hmul2(as_bf(s2), as_bf(0x7b807b80u)); }
     static __device__ __forceinline__ uint32_t word(uint32_t w) { return w; }
@@ -192,6 +192,13 @@ struct SmallScaleDecoder {
         return bits(__hmul2(as_bf(Decoder<__nv_bfloat16, kE4m3>::fields(w, a, b)), s));
     }
 };
+// The decoder for a tile whose scales are all below its limit; Decoder serves the others.
+template <typename T, int F> struct TileDecoder { static constexpr bool has_limit = false; };
+template <> struct TileDecoder<__nv_bfloat16, kE4m3> {
+    static constexpr bool has_limit = true;
+    using type = SmallScaleDecoder;
+};
+
 // Codes alone as a pair of f16, which holds every code exactly. word: four codes prepared by code_word;
 // upper: its codes 2 and 3, not 0 and 1. e4m3 has an instruction for it.
 template <int F> __device__ __forceinline__ uint32_t code_word(uint32_t w) { return F == kInt8 ? w ^ 0x80808080u : w; }

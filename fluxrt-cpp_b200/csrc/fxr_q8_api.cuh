@@ -91,20 +91,24 @@ int32_t launch_q8_write(const fxr_frame_desc* d, const fxr_q8_cache* cache, fxr:
     });
 }
 
-// Streams of at most this many rows take the kernel for few rows.
-constexpr int32_t kQ8RowsLimit = fxr::attn8::kMaxRowsPerStream;
+// The kernel for few rows serves streams of up to 32 rows: with more, a second group of rows reads the
+// cache again (24 heads over 4608 keys: 32 rows 27 us, and 34 with the other kernel; 64 rows 35.5, and
+// 35; 100 rows of 8 heads 30, and 27).
+constexpr int32_t kQ8FewRows = fxr::attn8::kMaxRowsPerStream;
 
 // Workspace of the attention: arrivals (zero before and after a call), then partial results, then the
 // visible steps of the kernel for many rows.
 struct Q8Work {
     int32_t* cnt;
     float* part;
+    fxr::attn8::CutUnit* cuts;
     int32_t* steps;
     uint16_t* list;
     uint32_t* groups;
     int32_t rows;         // bound of a stream's rows
+    bool bounded;         // by the caller
     bool few;             // the kernel for few rows
-    bool one_tile;        // it takes groups of 8 rows, not of 16
+    int32_t tiles;        // it takes groups of 8 * tiles rows
     int64_t line;         // bound of its work line
     int32_t slots;        // its partial results: one per column and CTA boundary
     int32_t units;        // 256-row units of a stream, key tiles: the kernel for many
@@ -115,8 +119,9 @@ struct Q8Work {
 
 Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, int32_t max_rows, void* ws) {
     Q8Work w{};
-    w.rows = max_rows > 0 ? std::min(max_rows, d->n_tokens) : d->n_tokens;
-    w.few = w.rows <= kQ8RowsLimit;
+    w.bounded = max_rows > 0;
+    w.rows = w.bounded ? std::min(max_rows, d->n_tokens) : d->n_tokens;
+    w.few = w.rows <= kQ8FewRows;
     const int64_t S = std::min<int32_t>(n_streams, FXR_MAX_BATCH), R = w.rows;
     size_t off = 0;
     char* b = static_cast<char*>(ws);
@@ -125,14 +130,17 @@ Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, in
         off = align_up(off + bytes, 256);
         return p;
     };
-    // one place and size for the arrivals of either kernel: calls with other bounds may share a workspace
+    // one place and size for the arrivals, whichever kernel a call takes: calls with other bounds may
+    // share a workspace
     const size_t ctas = (size_t)sm_count();
-    w.cnt = reinterpret_cast<int32_t*>(take(std::max(ctas * fxr::attn8::kPartWarps,
-                                                     (size_t)d->n_heads * FXR_MAX_BATCH * fxr::attn8::kGroupsPerStream) * sizeof(int32_t)));
+    w.cnt = reinterpret_cast<int32_t*>(take((size_t)d->n_heads * FXR_MAX_BATCH * fxr::attn8::kGroupsPerStream * sizeof(int32_t)));
     w.zero_bytes = off;
     if (w.few) {
-        const int64_t tile = S * R <= 8 ? 8 : 16;    // rows of a group
-        w.one_tile = tile == 8;
+        // groups as large as a stream's rows need; the packed rows of a prefix fill 16 of them at least
+        // (32, with own groups half empty, took 89 us where 16 take 79: 8 streams of 15 rows, 4608 + 2304 keys)
+        const int64_t packed = n_prefix > 0 ? std::max(R, std::min<int64_t>(S * R, 16)) : R;
+        w.tiles = packed <= 8 ? 1 : packed <= 16 ? 2 : 4;
+        const int64_t tile = 8 * w.tiles;
         const int64_t groups = (n_prefix > 0 ? (S * R + tile - 1) / tile : 0) + S * ((R + tile - 1) / tile);
         w.slots = (int32_t)std::min<int64_t>(INT32_MAX, sm_count() + groups * d->n_heads);
         w.line = groups * d->n_heads * ((std::max(n_prefix, d->n_tokens) + fxr::attn8::kUnitKeys - 1) / fxr::attn8::kUnitKeys);
@@ -142,6 +150,7 @@ Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, in
         w.n_pre = (n_prefix + fxr::attn8::kBN - 1) / fxr::attn8::kBN;
         w.n_own = (d->n_tokens + fxr::attn8::kBN - 1) / fxr::attn8::kBN;
         w.part = reinterpret_cast<float*>(take(ctas * fxr::attn8::kPartSlots * fxr::attn8::kPartFloats * sizeof(float)));
+        w.cuts = reinterpret_cast<fxr::attn8::CutUnit*>(take(2 * ctas * sizeof(fxr::attn8::CutUnit)));
         w.steps = reinterpret_cast<int32_t*>(take((size_t)(S * w.units) * sizeof(int32_t)));
         w.list = reinterpret_cast<uint16_t*>(take((size_t)(S * w.units) * (size_t)(w.n_pre + w.n_own) * sizeof(uint16_t)));
         w.groups = reinterpret_cast<uint32_t*>(take((size_t)(w.n_pre + S * w.n_own) * fxr::attn8::kBN * sizeof(uint32_t)));
@@ -173,7 +182,7 @@ int32_t launch_q8_rows(const fxr_frame_desc* d, const fxr::attn8::Params& p, cud
     if (dev < 0 || dev >= kMaxDevices) return fail(FXR_ERR_CUDA, "device %d", dev);
     if (!configured[dev]) {
         const cudaError_t e = cudaFuncSetAttribute(fxr::attn8::rows_kernel<T, F, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (int)fxr::attn8::kRowsSmem);
+                                                   (int)fxr::attn8::RowsShape<NQ>::smem);
         if (e != cudaSuccess) return cuda_status(e, "cudaFuncSetAttribute(rows_kernel)");
         configured[dev] = true;
     }
@@ -189,8 +198,8 @@ int32_t launch_q8_rows(const fxr_frame_desc* d, const fxr::attn8::Params& p, cud
         if ((rc = make_code_tmap(&maps.pk, p.prefix.k, C, p.n_prefix, p.prefix.ld, fxr::attn8::kBlk)) != FXR_OK) return rc;
         if ((rc = make_code_tmap(&maps.pv, p.prefix.v, C, p.n_prefix, p.prefix.ld, fxr::attn8::kBlk)) != FXR_OK) return rc;
     }
-    return cuda_status(launch_pdl(fxr::attn8::rows_kernel<T, F, NQ>, dim3(sm_count()), dim3(fxr::attn8::kRowsThreads),
-                                  fxr::attn8::kRowsSmem, s, maps, p),
+    return cuda_status(launch_pdl(fxr::attn8::rows_kernel<T, F, NQ>, dim3(sm_count()), dim3(fxr::attn8::RowsShape<NQ>::threads),
+                                  fxr::attn8::RowsShape<NQ>::smem, s, maps, p),
                        "rows_kernel launch");
 }
 
@@ -232,7 +241,11 @@ int32_t launch_q8_tiles(const fxr_frame_desc* d, const fxr::attn8::Params& p, co
     a.n_own = w.n_own;
     a.units_cap = w.units;
     a.part = w.part;
-    a.cnt = w.cnt;
+    a.cuts = w.cuts;
+    // a bound that the caller gave is taken to be tight: where its units would run whole, they do
+    const int64_t units = (int64_t)w.units * d->n_heads * p.n_streams;
+    const fxr::attn8::TileSchedule sc = fxr::attn8::tile_schedule((int32_t)(units * (w.n_pre + w.n_own)), (int32_t)units, sm_count());
+    a.may_cut = groups || !w.bounded || sc.per > 0 || sc.parts > 0;
     if (groups) {
         const cudaError_t e = launch_pdl(fxr::attn8::visible_steps_kernel, dim3(w.units, p.n_streams), dim3(fxr::attn8::kVisThreads), 0,
                                          s, a, w.steps, w.list, w.groups);
@@ -241,9 +254,13 @@ int32_t launch_q8_tiles(const fxr_frame_desc* d, const fxr::attn8::Params& p, co
         a.list = w.list;
         a.groups = w.groups;
     }
-    return cuda_status(launch_pdl(fxr::attn8::tile_kernel<T, F>, dim3(sm_count()), dim3(fxr::attn8::kTileThreads),
-                                  fxr::attn8::kTileSmem, s, maps, a),
-                       "tile_kernel launch");
+    cudaError_t e = launch_pdl(fxr::attn8::tile_kernel<T, F>, dim3(sm_count()), dim3(fxr::attn8::kTileThreads),
+                               fxr::attn8::kTileSmem, s, maps, a);
+    if (e != cudaSuccess) return cuda_status(e, "tile_kernel launch");
+    if (!a.may_cut) return FXR_OK;
+    e = launch_pdl(fxr::attn8::combine_kernel<T>, dim3(2 * sm_count() * fxr::attn8::kCombineCtas), dim3(fxr::attn8::kCombineThreads), 0,
+                   s, p, static_cast<const float*>(w.part), static_cast<const fxr::attn8::CutUnit*>(w.cuts));
+    return cuda_status(e, "combine_kernel launch");
 }
 
 int32_t check_groups(const uint32_t* g, const char* what) {
@@ -413,7 +430,9 @@ int32_t fxr_attention_q8(const fxr_frame_desc* desc, int32_t n_streams, const fx
             constexpr int F = decltype(f)::value;
             const cudaStream_t cs = static_cast<cudaStream_t>(stream);
             if (!w.few) return launch_q8_tiles<T, F>(desc, p, w, cs);
-            return w.one_tile ? launch_q8_rows<T, F, 1>(desc, p, cs) : launch_q8_rows<T, F, 2>(desc, p, cs);
+            return w.tiles == 1   ? launch_q8_rows<T, F, 1>(desc, p, cs)
+                   : w.tiles == 2 ? launch_q8_rows<T, F, 2>(desc, p, cs)
+                                  : launch_q8_rows<T, F, 4>(desc, p, cs);
         });
         if (st != FXR_OK) return st;
     }
