@@ -918,7 +918,8 @@ __host__ __device__ inline TileSchedule tile_schedule(int32_t total, int32_t n_u
     return s;
 }
 
-// A unit that was cut, written by the scheduler that starts it: slot 2 c + k for part slot k of CTA c.
+// A unit that was cut, in the entry of the CTA that holds its first part (which ends that CTA's range, so
+// that there is one at most).
 struct CutUnit {
     int32_t parts;               // 0: none
     int32_t stream, head, row0, rows;
@@ -934,7 +935,7 @@ struct TileParams {
     const uint32_t* groups;      // [n_pre + n_streams * n_own][128] key groups, zeros past a source's end
     int32_t may_cut;             // 0: whole units only (no combine follows)
     float* part;                 // [grid][kPartSlots][kPartFloats]
-    CutUnit* cuts;               // [grid][2]
+    CutUnit* cuts;               // [grid]
 };
 
 // ---- visible steps --------------------------------------------------------------------------------
@@ -1108,12 +1109,12 @@ __device__ __noinline__ void cut_epilogue(float* slot, int r, uint32_t tO, float
 }
 
 // Cut units' parts into their rows, in key order: a warp takes 32 rows by 16 columns of a unit (a row per
-// lane; partial O is stored column chunk by column chunk, so that its loads are whole lines), four CTAs
+// lane; partial O is stored column chunk by column chunk, so that its loads are whole lines), 16 CTAs
 // a unit. A launch of its own, chained to the tile kernel's end: its warps spread over all SMs, where a
 // combine by the last part to arrive read all of a unit's parts through one SM, 2.5 us per part (601 rows
 // of two streams, documents: 50 us with that, 41 with this). It costs a call about 5 us, so calls whose
 // units the host knows to stay whole go without.
-constexpr int kCombineThreads = 512, kCombineCtas = 4;   // threads of a CTA, CTAs of a unit
+constexpr int kCombineThreads = 128, kCombineCtas = 16;   // threads of a CTA, CTAs of a unit
 
 template <typename T>
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const __grid_constant__ Params p, const float* part,
@@ -1513,7 +1514,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
             const int32_t grid = (int32_t)gridDim.x, c = (int32_t)blockIdx.x;
             int32_t cur = per > 0 ? (int32_t)min((int64_t)total, (int64_t)c * per) : parts > 0 ? c / parts : c;
             const int32_t end = per > 0 ? (int32_t)min((int64_t)total, (int64_t)cur + per) : n_units;
-            uint32_t cuts_made = 0;
+            bool cut_made = false;                        // (of lane 0)
             for (uint32_t k = 0;; ++k) {
                 bool more = cur < end;
                 // the unit: stream, head, first row, steps, first iteration
@@ -1590,9 +1591,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                 }
                 if (!more) n = 0;
                 if (lane == 0 && n > 0 && n < cnt && s0 == 0) {
-                    const int slot = i0 > c * per ? 1 : 0;
-                    a.cuts[2 * c + slot] = CutUnit{of, b, head, unit * kUnitRows, rows, c, i0, per};
-                    cuts_made |= 1u << slot;
+                    a.cuts[c] = CutUnit{of, b, head, unit * kUnitRows, rows, c, i0, per};
+                    cut_made = true;
                 }
                 if (k >= 2 && !__all_sync(0xffffffffu, mbar_wait(bar(kItemEmpty + (k & 1)), ((k >> 1) - 1) & 1, abort))) break;
                 Item* it = item_at(k);
@@ -1622,7 +1622,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                 if (n == 0) break;
                 cur = per > 0 ? cur + n : parts > 0 ? end : cur + grid;
             }
-            if (a.may_cut && lane < 2 && (cuts_made >> lane & 1u) == 0) a.cuts[2 * c + lane].parts = 0;
+            if (a.may_cut && lane == 0 && !cut_made) a.cuts[c].parts = 0;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));

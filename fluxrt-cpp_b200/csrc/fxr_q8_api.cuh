@@ -136,8 +136,9 @@ Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, in
     w.cnt = reinterpret_cast<int32_t*>(take((size_t)d->n_heads * FXR_MAX_BATCH * fxr::attn8::kGroupsPerStream * sizeof(int32_t)));
     w.zero_bytes = off;
     if (w.few) {
-        // groups as large as a stream's rows need; the packed rows of a prefix fill 16 of them at least
-        // (32, with own groups half empty, took 89 us where 16 take 79: 8 streams of 15 rows, 4608 + 2304 keys)
+        // groups as large as a stream's rows need; the packed rows of a prefix fill groups of 16 at most
+        // otherwise (of 32, and 8 warps, took 85 us where 16 rows and 16 warps take 79: 8 streams of 15
+        // rows, 4608 + 2304 keys; 3 streams 77 and 48)
         const int64_t packed = n_prefix > 0 ? std::max(R, std::min<int64_t>(S * R, 16)) : R;
         w.tiles = packed <= 8 ? 1 : packed <= 16 ? 2 : 4;
         const int64_t tile = 8 * w.tiles;
@@ -150,7 +151,7 @@ Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, in
         w.n_pre = (n_prefix + fxr::attn8::kBN - 1) / fxr::attn8::kBN;
         w.n_own = (d->n_tokens + fxr::attn8::kBN - 1) / fxr::attn8::kBN;
         w.part = reinterpret_cast<float*>(take(ctas * fxr::attn8::kPartSlots * fxr::attn8::kPartFloats * sizeof(float)));
-        w.cuts = reinterpret_cast<fxr::attn8::CutUnit*>(take(2 * ctas * sizeof(fxr::attn8::CutUnit)));
+        w.cuts = reinterpret_cast<fxr::attn8::CutUnit*>(take(ctas * sizeof(fxr::attn8::CutUnit)));
         w.steps = reinterpret_cast<int32_t*>(take((size_t)(S * w.units) * sizeof(int32_t)));
         w.list = reinterpret_cast<uint16_t*>(take((size_t)(S * w.units) * (size_t)(w.n_pre + w.n_own) * sizeof(uint16_t)));
         w.groups = reinterpret_cast<uint32_t*>(take((size_t)(w.n_pre + S * w.n_own) * fxr::attn8::kBN * sizeof(uint32_t)));
@@ -258,7 +259,7 @@ int32_t launch_q8_tiles(const fxr_frame_desc* d, const fxr::attn8::Params& p, co
                                fxr::attn8::kTileSmem, s, maps, a);
     if (e != cudaSuccess) return cuda_status(e, "tile_kernel launch");
     if (!a.may_cut) return FXR_OK;
-    e = launch_pdl(fxr::attn8::combine_kernel<T>, dim3(2 * sm_count() * fxr::attn8::kCombineCtas), dim3(fxr::attn8::kCombineThreads), 0,
+    e = launch_pdl(fxr::attn8::combine_kernel<T>, dim3(sm_count() * fxr::attn8::kCombineCtas), dim3(fxr::attn8::kCombineThreads), 0,
                    s, p, static_cast<const float*>(w.part), static_cast<const fxr::attn8::CutUnit*>(w.cuts));
     return cuda_status(e, "combine_kernel launch");
 }
