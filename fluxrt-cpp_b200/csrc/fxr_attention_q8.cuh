@@ -65,8 +65,9 @@ struct Params {
 // All operands are f16, whatever the frame's type: it holds the codes exactly, and the codes reach it in
 // fewer instructions than bf16. bf16 queries are brought to f16 by a power of two per row (exactly, but
 // for elements below 2^-24 of the row's largest). K scales multiply the scores in 32 bits. V scales
-// multiply P before its one rounding, relative to the largest that the warp has met, so that P stays in
-// f16's range whatever the scales are.
+// multiply P before its one rounding; the running maximum is that of score + log2(V scale), the weight of
+// a key's codes, so that P stays in f16's range whatever the scales are, and a large V that a row hardly
+// sees, or not at all, costs the others no precision.
 // Partial results (O, maximum, sum) meet in L2: the last of a row group's parts to arrive combines
 // them in key order, so the result does not depend on the order of arrival.
 // ---------------------------------------------------------------------------------------------
@@ -116,6 +117,12 @@ __device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uin
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ float lg2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -529,7 +536,6 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
                 l_run[q][e] = 0.f;
             }
         }
-        float v_top = 0.f, v_inv = 0.f;      // the largest V scale so far (of the warp), its inverse
         float qs[NQ][2];                     // score factors of this lane's queries
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
@@ -575,37 +581,23 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
                 }
             }
             // scales and masks: this lane's keys, key_of(g) and 8 behind it
-            float v_sc[2];               // V scales, then relative to v_top: what P is multiplied with
+            float v_sc[2], v_log[2];     // what P is multiplied with, its logarithm
             const int32_t left = n_keys - b * kBlk;
             bool grow = false;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int key = key_of(g) + 8 * e;
                 const float kk = StoreT<T>::unpack2(sc_p[key]).x, vv = StoreT<T>::unpack2(sc_p[kBlk + key]).x;
-                const bool in = key < left, v_ok = q8::valid_scale<T, F>(vv);
+                const bool v_ok = q8::valid_scale<T, F>(vv);
                 const float f = v_ok && q8::valid_scale<T, F>(kk) ? kk : __uint_as_float(0x7fc00000u);
-                v_sc[e] = v_ok && in ? vv : 0.f;
+                v_sc[e] = v_ok ? vv : 0.f;
+                // (bounded below, so that exp2(score - maximum) stays finite: V scales under 2^-100 lose bits)
+                v_log[e] = fmaxf(lg2_approx(v_sc[e]), -100.f);
 #pragma unroll
                 for (int q = 0; q < NQ; ++q)
 #pragma unroll
                     for (int d = 0; d < 2; ++d) s[q][2 * e + d] *= f * qs[q][d];
             }
-            if (__any_sync(0xffffffffu, fmaxf(v_sc[0], v_sc[1]) > v_top)) {
-                float x = fmaxf(v_sc[0], v_sc[1]);
-#pragma unroll
-                for (int e = 16; e > 0; e >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, e));
-                const float inv = 1.f / fmaxf(x, 0x1p-126f), al = v_inv > 0.f ? inv / v_inv : 0.f;
-                v_top = x;
-                v_inv = inv;
-#pragma unroll
-                for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[q][j][e] *= al;
-            }
-            v_sc[0] *= v_inv;
-            v_sc[1] *= v_inv;
             if (kg != nullptr || left < kBlk) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -626,14 +618,15 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
 #pragma unroll
             for (int q = 0; q < NQ; ++q)
 #pragma unroll
-                for (int d = 0; d < 2; ++d) grow = grow || fmaxf(s[q][d], s[q][2 + d]) > m_run[q][d] + 8.f;
-            // the running maxima move only where a score passes one by more than 2^8 (P stays below that)
+                for (int d = 0; d < 2; ++d)
+                    grow = grow || fmaxf(s[q][d] + v_log[0], s[q][2 + d] + v_log[1]) > m_run[q][d] + 8.f;
+            // the running maxima move only where a weight passes one by more than 2^8 (P stays below that)
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                 for (int q = 0; q < NQ; ++q)
 #pragma unroll
                     for (int d = 0; d < 2; ++d) {
-                        float x = fmaxf(s[q][d], s[q][2 + d]);
+                        float x = fmaxf(s[q][d] + v_log[0], s[q][2 + d] + v_log[1]);
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -693,7 +686,6 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
         // ---- the warps' results meet: position 8 d + g of a row is d of lane g's 16 dims (tile j holds
         // d = 2 j and 2 j + 1), then a row per warp, four positions per lane
         const int live = item.live;
-        const float v_unit = v_inv > 0.f ? 1.f / v_inv : 0.f;     // of P's V factors
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
@@ -703,8 +695,8 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
                 if (row < live) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        dst[16 * j] = o[q][j][d] * v_unit;
-                        dst[16 * j + 8] = o[q][j][2 + d] * v_unit;
+                        dst[16 * j] = o[q][j][d];
+                        dst[16 * j + 8] = o[q][j][2 + d];
                     }
                 }
                 float l = l_run[q][d];

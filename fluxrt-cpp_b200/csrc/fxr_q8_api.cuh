@@ -268,6 +268,25 @@ int32_t check_groups(const uint32_t* g, const char* what) {
     return (reinterpret_cast<uintptr_t>(g) & 3u) ? fail(FXR_ERR_INVALID, "%s must be 4-byte aligned", what) : FXR_OK;
 }
 
+int32_t check_q8_attention(const fxr_frame_desc* desc, int32_t n_streams, const fxr_q8_stream* streams, const fxr_q8_cache* prefix,
+                           const uint32_t* prefix_groups) {
+    int32_t st;
+    if (prefix && (st = check_q8_cache(desc, prefix, 0, "prefix")) != FXR_OK) return st;
+    if ((st = check_groups(prefix_groups, "prefix_groups")) != FXR_OK) return st;
+    const int64_t C = (int64_t)desc->n_heads * desc->head_dim;
+    for (int32_t b = 0; b < n_streams; ++b) {
+        const fxr_q8_stream& s = streams[b];
+        if ((st = check_q8_cache(desc, &s.cache, desc->n_tokens, "stream cache")) != FXR_OK) return st;
+        if (s.cache.format != streams[0].cache.format || (prefix && s.cache.format != prefix->format))
+            return fail(FXR_ERR_INVALID, "stream %d: the caches of a call share one format", b);
+        if (!s.qc || !s.idx || !s.count || !s.out) return fail(FXR_ERR_INVALID, "stream %d: null pointer", b);
+        if (!aligned16(s.qc) || !aligned16(s.out)) return fail(FXR_ERR_INVALID, "stream %d: qc/out must be 16-byte aligned", b);
+        if (s.ld_qc < C || (s.ld_qc % 8)) return fail(FXR_ERR_INVALID, "stream %d: ld_qc must be a multiple of 8, >= n_heads*head_dim", b);
+        if ((st = check_groups(s.q_groups, "q_groups")) != FXR_OK || (st = check_groups(s.k_groups, "k_groups")) != FXR_OK) return st;
+    }
+    return FXR_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -386,20 +405,8 @@ int32_t fxr_attention_q8(const fxr_frame_desc* desc, int32_t n_streams, const fx
     if (n_streams < 0) return fail(FXR_ERR_INVALID, "n_streams < 0");
     if (n_streams == 0 || desc->n_tokens == 0) return FXR_OK;
     if (!streams) return fail(FXR_ERR_INVALID, "null streams");
+    if ((st = check_q8_attention(desc, n_streams, streams, prefix, prefix_groups)) != FXR_OK) return st;
     const int32_t n_prefix = prefix ? prefix->n_rows : 0;
-    if (prefix && (st = check_q8_cache(desc, prefix, 0, "prefix")) != FXR_OK) return st;
-    if ((st = check_groups(prefix_groups, "prefix_groups")) != FXR_OK) return st;
-    const int64_t C = (int64_t)desc->n_heads * desc->head_dim;
-    for (int32_t b = 0; b < n_streams; ++b) {
-        const fxr_q8_stream& s = streams[b];
-        if ((st = check_q8_cache(desc, &s.cache, desc->n_tokens, "stream cache")) != FXR_OK) return st;
-        if (s.cache.format != streams[0].cache.format || (prefix && s.cache.format != prefix->format))
-            return fail(FXR_ERR_INVALID, "stream %d: the caches of a call share one format", b);
-        if (!s.qc || !s.idx || !s.count || !s.out) return fail(FXR_ERR_INVALID, "stream %d: null pointer", b);
-        if (!aligned16(s.qc) || !aligned16(s.out)) return fail(FXR_ERR_INVALID, "stream %d: qc/out must be 16-byte aligned", b);
-        if (s.ld_qc < C || (s.ld_qc % 8)) return fail(FXR_ERR_INVALID, "stream %d: ld_qc must be a multiple of 8, >= n_heads*head_dim", b);
-        if ((st = check_groups(s.q_groups, "q_groups")) != FXR_OK || (st = check_groups(s.k_groups, "k_groups")) != FXR_OK) return st;
-    }
     const Q8Work w = carve_q8(desc, n_streams, n_prefix, max_rows, workspace);
     if (!workspace) return fail(FXR_ERR_INVALID, "null workspace");
     if (!aligned16(workspace)) return fail(FXR_ERR_INVALID, "workspace must be 16-byte aligned");
@@ -500,6 +507,11 @@ int32_t fxr_frame_forward_q8(const fxr_frame_desc* desc, const void* q, const vo
     const Q8FrameViews w = carve_q8_frame(desc, n_prefix, max_rows, workspace);
     if (workspace_bytes < w.total) return fail(FXR_ERR_WORKSPACE, "workspace %zu < required %zu", workspace_bytes, w.total);
     const int64_t C = (int64_t)desc->n_heads * desc->head_dim;
+    // every argument is looked at before the first launch
+    const fxr_q8_stream s{w.qc, C, w.idx, w.count, out, q_groups, k_groups, *cache};
+    if ((st = check_q8_attention(desc, 1, &s, prefix, prefix_groups)) != FXR_OK) return st;
+    if (!q || !k || !v || !norm_q || !norm_k || (desc->rope_n_axes > 0 && !pos)) return fail(FXR_ERR_INVALID, "null pointer argument");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return fail(FXR_ERR_INVALID, "Q/K/V must be 16-byte aligned");
     fxr::CompactArgs ca{};
     ca.s[0] = fxr::CompactStream{mask, valid, w.idx, w.count, fxr::RestoreList{}};
     // the compaction also zeroes the attention's arrivals
@@ -508,7 +520,6 @@ int32_t fxr_frame_forward_q8(const fxr_frame_desc* desc, const void* q, const vo
     if (st != FXR_OK) return st;
     if ((st = fxr_gather_norm_rope_q8(desc, q, k, v, mask, w.idx, w.count, pos, norm_q, norm_k, w.qc, C, cache, w.save, stream)) != FXR_OK)
         return st;
-    const fxr_q8_stream s{w.qc, C, w.idx, w.count, out, q_groups, k_groups, *cache};
     if ((st = fxr_attention_q8(desc, 1, &s, prefix, prefix_groups, max_rows, w.attn, w.attn_bytes, stream)) != FXR_OK) return st;
     return fxr_restore_rows_q8(desc, mask, w.idx, w.count, w.save, cache, stream);
 }

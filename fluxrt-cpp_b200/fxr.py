@@ -771,10 +771,14 @@ def _refuse(msg: str):
     raise FxrError(FXR_ERR_INVALID, msg)
 
 
-def _raw_stream(device: int, stream=None) -> int:
-    """The cudaStream_t of `stream` or of the current stream of `device`, the current device. These
-    calls take a few microseconds on the GPU, so the handle is asked for without a Stream object."""
+def _raw_stream(device: int, stream, *tensors) -> int:
+    """The cudaStream_t of `stream` or of the current stream of `device`, which has to be the current
+    device and hold the tensors (None entries apart). These calls take a few microseconds on the GPU,
+    so the handle is asked for without a Stream object."""
     import torch
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            _refuse(f"tensor on {t.device}, the cache is on cuda:{device}")
     if torch._C._cuda_getDevice() != device:
         _refuse(f"tensor on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
     return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
@@ -851,7 +855,8 @@ def gather_norm_rope_q8(cfg: FrameConfig, q, k, v, mask, idx, count, pos, norm_q
     _check(load().fxr_gather_norm_rope_q8(cfg.ref(), q.data_ptr(), k.data_ptr(), v.data_ptr(), mask.data_ptr(),
                                           idx.data_ptr(), count.data_ptr(), _ptr(pos), norm_q.data_ptr(),
                                           norm_k.data_ptr(), qc.data_ptr(), qc.stride(0), cache.ref, _ptr(save),
-                                          _raw_stream(cache.device, stream)))
+                                          _raw_stream(cache.device, stream, q, k, v, mask, idx, count, pos, norm_q,
+                                                      norm_k, qc, save)))
 
 
 def cache_write_q8(cfg: FrameConfig, cache_k, cache_v, cache: CacheQ8, idx=None, count=None, host_count: int = -1,
@@ -862,7 +867,7 @@ def cache_write_q8(cfg: FrameConfig, cache_k, cache_v, cache: CacheQ8, idx=None,
     if idx is None and count is None and host_count < 0:
         host_count = cfg.n_tokens
     _check(load().fxr_cache_write_q8(cfg.ref(), _ptr(cache_k), _ptr(cache_v), _ptr(idx), _ptr(count), host_count,
-                                     cache.ref, _raw_stream(cache.device, stream)))
+                                     cache.ref, _raw_stream(cache.device, stream, cache_k, cache_v, idx, count)))
 
 
 def cache_read_q8(cfg: FrameConfig, cache: CacheQ8, k, v, idx=None, count=None, host_count: int = -1, stream=None):
@@ -873,13 +878,13 @@ def cache_read_q8(cfg: FrameConfig, cache: CacheQ8, k, v, idx=None, count=None, 
     if idx is None and count is None and host_count < 0:
         host_count = cache.n_rows
     _check(load().fxr_cache_read_q8(cfg.ref(), cache.ref, _ptr(idx), _ptr(count), host_count, k.data_ptr(),
-                                    v.data_ptr(), k.stride(0), _raw_stream(cache.device, stream)))
+                                    v.data_ptr(), k.stride(0), _raw_stream(cache.device, stream, k, v, idx, count)))
 
 
 def restore_rows_q8(cfg: FrameConfig, mask, idx, count, save, cache: CacheQ8, stream=None):
     cache.check(cfg, cfg.n_tokens)
     _check(load().fxr_restore_rows_q8(cfg.ref(), _ptr(mask), _ptr(idx), _ptr(count), _ptr(save), cache.ref,
-                                      _raw_stream(cache.device, stream)))
+                                      _raw_stream(cache.device, stream, mask, idx, count, save)))
 
 
 class Q8Streams:
@@ -896,6 +901,7 @@ class Q8Streams:
                                            _ptr(f["count"]), _ptr(out), _ptr(f.get("q_groups")),
                                            _ptr(f.get("k_groups")), cache.struct)
         self.rows = min((f["qc"].shape[0] for f in streams), default=0)
+        self.device = streams[0]["cache"].device if streams else None
         self.tokens = min((f["out"].shape[0] for f in streams), default=0)
 
     def check(self, cfg: FrameConfig, max_rows: int = 0):
@@ -939,7 +945,8 @@ def attention_q8(cfg: FrameConfig, streams, workspace, prefix: CacheQ8 | None = 
     _check(load().fxr_attention_q8(cfg.ref(), len(streams.streams), streams.array, prefix.ref if prefix is not None else None,
                                    _ptr(prefix_groups), max_rows, workspace.data_ptr(),
                                    workspace.numel() * workspace.element_size(),
-                                   _raw_stream(workspace.device.index, stream)))
+                                   _raw_stream(workspace.get_device() if streams.device is None else streams.device, stream,
+                                               workspace, prefix_groups, prefix.k if prefix is not None else None)))
 
 
 def frame_q8_workspace_size(cfg: FrameConfig, n_prefix: int = 0, max_rows: int = 0) -> int:
@@ -960,7 +967,9 @@ def frame_forward_q8(cfg: FrameConfig, q, k, v, mask, valid, pos, norm_q, norm_k
                                        _ptr(norm_q), _ptr(norm_k), cache.ref, _ptr(q_groups), _ptr(k_groups),
                                        prefix.ref if prefix is not None else None, _ptr(prefix_groups), max_rows,
                                        _ptr(out), _ptr(workspace), workspace.numel() * workspace.element_size(),
-                                       _raw_stream(cache.device, stream)))
+                                       _raw_stream(cache.device, stream, q, k, v, mask, valid, pos, norm_q, norm_k, out,
+                                                   workspace, q_groups, k_groups, prefix_groups,
+                                                   prefix.k if prefix is not None else None)))
 
 
 def qkv_project(cfg: FrameConfig, hidden, w_qkv, bias, idx, count, q, k, v, scratch=None,
