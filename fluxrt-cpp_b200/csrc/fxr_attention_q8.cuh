@@ -36,7 +36,7 @@ struct Params {
     int64_t ld_out;
     float scale_log2;
     float* part;                 // partial results, kRowsSlotFloats each
-    int32_t* cnt;                // [n_heads] arrivals, zero between launches
+    int32_t* cnt;                // [own group][n_heads] arrivals, zero between launches
 };
 
 // ---------------------------------------------------------------------------------------------
@@ -810,15 +810,15 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many rows per stream: bound by the tensor core. The two-tile schedule of the 16-bit attention
+// Many rows per stream (but those that q8_expand_kernel and the 16-bit kernel serve): bound by the tensor core. The two-tile schedule of the 16-bit attention
 // (fxr_attention2.cuh: 256 compact query rows of one head per unit, 128 keys per step, S and O in
 // tensor memory, P written over S, lazy rescaling, units cut between CTAs when whole ones would leave
 // SMs idle) with K and V tiles that arrive as codes: a fourth warpgroup turns each 128 x 128 tile of
 // codes in shared memory into the 16-bit tile that tcgen05.mma reads, T(code * scale), one row per
 // thread, in the 128-byte swizzle on both sides (every access of 8 lanes covers all banks). TMA moves
 // codes only: half the bytes of the 16-bit cache.
-// Warps (512 threads): 0-7 softmax of tile 0 / 1, 8 TMA producer, 9 tensor memory and the MMA-issuing
-// thread, 10 scheduler (writes the CTA's items into a 2-slot ring in shared memory, so that no other
+// Warps (512 threads): 0-7 softmax of tile 0 / 1, 8 TMA producer, 9 tensor memory and the MMA
+// issuer, 10 scheduler (writes the CTA's items into a 2-slot ring in shared memory, so that no other
 // role carries the bookkeeping), 11 idle, 12-15 converters.
 // Prefix rows come first, then the stream's own; a source's last tile is filled with zeros and its
 // scores masked. With visibility groups, visible_steps_kernel lists for every 256-row unit the tiles
@@ -1104,7 +1104,7 @@ __device__ __noinline__ void cut_epilogue(float* slot, int r, uint32_t tO, float
 // lane; partial O is stored column chunk by column chunk, so that its loads are whole lines), 16 CTAs
 // a unit. A launch of its own, chained to the tile kernel's end: its warps spread over all SMs, where a
 // combine by the last part to arrive read all of a unit's parts through one SM, 2.5 us per part (601 rows
-// of two streams, documents: 50 us with that, 41 with this). It costs a call about 5 us, so calls whose
+// of two streams, documents: 50 us with that, 38.5 with this). It costs a call about 5 us, so calls whose
 // units the host knows to stay whole go without.
 constexpr int kCombineThreads = 128, kCombineCtas = 16;   // threads of a CTA, CTAs of a unit
 
@@ -1392,95 +1392,102 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                 }
             }
         } else if (warp == kMmaWarp) {
-            if (lane == 0) {
-                // ---------------- MMA issuer (order and waits of the 16-bit kernel) ----------------
-                constexpr uint32_t fmt = StoreT<T>::kUmmaFormat;
-                constexpr uint32_t idesc_qk = make_idesc_f16(fmt, 0, kBM, kBN);
-                constexpr uint32_t idesc_pv = make_idesc_f16(fmt, 1, kBM, kD);
-                uint32_t acq = 0, rel = 0, q_it = 0, g = 0, done = 0;
-                bool ok = true, issued = false;
-                auto wait = [&](uint32_t b_, uint32_t par_) { return mbar_wait_spin(b_, par_, abort); };
-                auto acquire = [&]() -> uint32_t {
-                    const uint32_t st = acq % kTiles;
-                    if (!wait(bar(kFull + st), (acq / kTiles) & 1)) return 0;
-                    ++acq;
-                    return base + kSmTiles + st * kTile;
-                };
-                auto release = [&]() {
-                    umma_commit(bar(kEmpty + rel % kTiles));
-                    ++rel;
-                };
-                auto qk = [&](int t, uint32_t sK) {
-                    const uint64_t dq = smem_desc_sw128(base + kSmQ + t * kTile, 16, 1024);
-                    const uint64_t dk = smem_desc_sw128(sK, 16, 1024);
+            // ---------------- MMA issuer (order and waits of the 16-bit kernel) ----------------
+            // The whole warp walks, and its waits end alike on every lane, so that counters and
+            // descriptors are uniform; one elected lane issues (1536 rows over 4608 keys: 93 us,
+            // and 100 with a single lane that walks and issues).
+            constexpr uint32_t fmt = StoreT<T>::kUmmaFormat;
+            constexpr uint32_t idesc_qk = make_idesc_f16(fmt, 0, kBM, kBN);
+            constexpr uint32_t idesc_pv = make_idesc_f16(fmt, 1, kBM, kD);
+            uint32_t acq = 0, rel = 0, q_it = 0, g = 0, done = 0;
+            bool ok = true, issued = false;
+            auto wait = [&](uint32_t b_, uint32_t par_) -> bool { return __all_sync(0xffffffffu, mbar_wait_spin(b_, par_, abort)); };
+            auto acquire = [&]() -> uint32_t {
+                const uint32_t st = acq % kTiles;
+                if (!wait(bar(kFull + st), (acq / kTiles) & 1)) return 0;
+                ++acq;
+                return base + kSmTiles + st * kTile;
+            };
+            auto release = [&]() {
+                if (elect_one()) umma_commit(bar(kEmpty + rel % kTiles));
+                ++rel;
+            };
+            auto qk = [&](int t, uint32_t sK) {
+                const uint64_t dq = smem_desc_sw128(base + kSmQ + t * kTile, 16, 1024);
+                const uint64_t dk = smem_desc_sw128(sK, 16, 1024);
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < kD / 16; ++k) {
                         const uint64_t off = ((k >> 2) * kSpan + (k & 3) * 32u) >> 4;
                         umma_ss(tmem + kColS + t * 128u, dq + off, dk + off, idesc_qk, k > 0 ? 1u : 0u);
                     }
                     umma_commit(bar(kSFull + t));
-                };
-                auto pv = [&](int t, uint32_t sV, int h, bool acc) {
-                    const uint64_t dv = smem_desc_sw128(sV, kSpan, 1024);
+                }
+                __syncwarp();
+            };
+            auto pv = [&](int t, uint32_t sV, int h, bool acc) {
+                const uint64_t dv = smem_desc_sw128(sV, kSpan, 1024);
+                if (elect_one()) {
 #pragma unroll
                     for (int k = 4 * h; k < 4 * h + 4; ++k)
                         umma_ts(tmem + kColO + t * 128u, tmem + kColS + t * 128u + k * 8u, dv + (uint64_t)((k * 2048u) >> 4),
                                 idesc_pv, (acc || k > 0) ? 1u : 0u);
-                };
-                for (uint32_t it_no = 0; ok; ++it_no) {
-                    if (!wait(bar(kItemFull + (it_no & 1)), (it_no >> 1) & 1)) break;
-                    const int32_t n = item_at(it_no)->n;
-                    mbar_arrive(bar(kItemEmpty + (it_no & 1)));
-                    if (n == 0) break;
-                    if (!wait(bar(kQFull), q_it & 1)) break;
-                    ++q_it;
-                    if (g > 0 && (!wait(bar(kPVDone + 0), (g - 1) & 1) || !wait(bar(kPVDone + 1), (g - 1) & 1))) break;
-                    uint32_t sK = acquire();
-                    if (!sK) break;
-                    tc_fence_after();
-                    issued = true;
-                    qk(0, sK);
-                    qk(1, sK);
-                    release();
-                    if (n == 1) umma_commit(bar(kQEmpty));
-                    for (int32_t j = 0; j < n; ++j, ++g) {
-                        const uint32_t sV = acquire();
-                        if (!sV) { ok = false; break; }
-                        const bool more = j + 1 < n;
+                    if (h == 1) umma_commit(bar(kPVDone + t));
+                }
+                __syncwarp();
+            };
+            for (uint32_t it_no = 0; ok; ++it_no) {
+                if (!wait(bar(kItemFull + (it_no & 1)), (it_no >> 1) & 1)) break;
+                const int32_t n = __shfl_sync(0xffffffffu, item_at(it_no)->n, 0);
+                if (elect_one()) mbar_arrive(bar(kItemEmpty + (it_no & 1)));
+                if (n == 0) break;
+                if (!wait(bar(kQFull), q_it & 1)) break;
+                ++q_it;
+                if (g > 0 && (!wait(bar(kPVDone + 0), (g - 1) & 1) || !wait(bar(kPVDone + 1), (g - 1) & 1))) break;
+                uint32_t sK = acquire();
+                if (!sK) break;
+                tc_fence_after();
+                issued = true;
+                qk(0, sK);
+                qk(1, sK);
+                release();
+                if (n == 1 && elect_one()) umma_commit(bar(kQEmpty));
+                for (int32_t j = 0; j < n; ++j, ++g) {
+                    const uint32_t sV = acquire();
+                    if (!sV) { ok = false; break; }
+                    const bool more = j + 1 < n;
 #pragma unroll 1
-                        for (int t = 0; t < 2; ++t) {
-                            if (!wait(bar(kPHalf0 + t), g & 1)) { ok = false; break; }
-                            if (j == 0 && done > 0 && !wait(bar(kOFree + t), (done - 1) & 1)) { ok = false; break; }
+                    for (int t = 0; t < 2; ++t) {
+                        if (!wait(bar(kPHalf0 + t), g & 1)) { ok = false; break; }
+                        if (j == 0 && done > 0 && !wait(bar(kOFree + t), (done - 1) & 1)) { ok = false; break; }
+                        tc_fence_after();
+                        pv(t, sV, 0, j > 0);
+                        if (!wait(bar(kPHalf1 + t), g & 1)) { ok = false; break; }
+                        tc_fence_after();
+                        pv(t, sV, 1, true);
+                        if (t == 1) release();
+                        if (more) {
+                            if (t == 0) {
+                                sK = acquire();
+                                if (!sK) { ok = false; break; }
+                            }
+                            // S_t(j+1) overwrites P_t(j): O_t += P_t(j) V_j has to be complete
+                            if (!wait(bar(kPVDone + t), g & 1)) { ok = false; break; }
                             tc_fence_after();
-                            pv(t, sV, 0, j > 0);
-                            if (!wait(bar(kPHalf1 + t), g & 1)) { ok = false; break; }
-                            tc_fence_after();
-                            pv(t, sV, 1, true);
-                            umma_commit(bar(kPVDone + t));
-                            if (t == 1) release();
-                            if (more) {
-                                if (t == 0) {
-                                    sK = acquire();
-                                    if (!sK) { ok = false; break; }
-                                }
-                                // S_t(j+1) overwrites P_t(j): O_t += P_t(j) V_j has to be complete
-                                if (!wait(bar(kPVDone + t), g & 1)) { ok = false; break; }
-                                tc_fence_after();
-                                qk(t, sK);
-                                if (t == 1) {
-                                    release();
-                                    if (j + 2 == n) umma_commit(bar(kQEmpty));
-                                }
+                            qk(t, sK);
+                            if (t == 1) {
+                                release();
+                                if (j + 2 == n && elect_one()) umma_commit(bar(kQEmpty));
                             }
                         }
-                        if (!ok) break;
                     }
-                    ++done;
+                    if (!ok) break;
                 }
-                if (*abort && issued) {
-                    umma_commit(bar(kDrain));
-                    attn::mbar_wait_drain(bar(kDrain), 0);
-                }
+                ++done;
+            }
+            if (__any_sync(0xffffffffu, *abort != 0) && issued && elect_one()) {
+                umma_commit(bar(kDrain));
+                attn::mbar_wait_drain(bar(kDrain), 0);
             }
         } else if (warp == kSchedWarp) {
             // ---------------- scheduler: the CTA's items, by a schedule that every CTA computes alike ----------

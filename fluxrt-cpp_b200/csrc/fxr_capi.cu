@@ -318,6 +318,7 @@ struct AttnStreamArgs {
     void* out;
     // the frame whose mask==1 cache rows the attention may restore itself (nullptr: it does not)
     const Views* frame = nullptr;
+    int64_t q_rows = 0;   // rows that qc holds (0: n_tokens)
 };
 
 // Whether the two-tile kernel serves attention launches of this dtype on the current device (it
@@ -371,7 +372,7 @@ int32_t launch_attention_streams(const fxr_frame_desc* d, int32_t n_streams, con
     fxr::attn::Params p{};
     int32_t rc;
     for (int32_t b = 0; b < n_streams; ++b) {
-        if ((rc = make_tmap(&maps.q[b], st[b].qc, d->dtype, C, N, st[b].ld_qc)) != FXR_OK) return rc;
+        if ((rc = make_tmap(&maps.q[b], st[b].qc, d->dtype, C, st[b].q_rows > 0 ? st[b].q_rows : N, st[b].ld_qc)) != FXR_OK) return rc;
         if ((rc = make_tmap(&maps.k[b], st[b].ck, d->dtype, C, N, d->ld_cache)) != FXR_OK) return rc;
         if ((rc = make_tmap(&maps.v[b], st[b].cv, d->dtype, C, N, d->ld_cache)) != FXR_OK) return rc;
         p.s[b].count = st[b].count;

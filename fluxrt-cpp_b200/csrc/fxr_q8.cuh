@@ -13,6 +13,7 @@
 //   q8_write_kernel     executed rows: gather + QK-RMSNorm + RoPE + quantised cache rows, or (raw)
 //                       the quantised rows of an attention-ready 16-bit cache
 //   q8_read_kernel      rows back in 16 bits
+//   q8_expand_kernel    whole caches in 16 bits, for the attention over many rows
 //   q8_restore_kernel   puts back the cache rows of mask==1 tokens
 #pragma once
 
@@ -469,6 +470,68 @@ __global__ void __launch_bounds__(kReadThreads) q8_read_kernel(const __grid_cons
         uint4* vo = reinterpret_cast<uint4*>(static_cast<T*>(a.v) + dst);
         __stcs(vo, lo);
         __stcs(vo + 1, hi);
+    }
+}
+
+// Rows of every stream's cache in T, packed [n_streams][n_tokens][n_heads * 128], for the 16-bit
+// attention. There every row of a stream sees every key, so that a key whose K or V scale is not valid
+// makes the head's rows NaN: its V row is NaN (and NaN times any weight), its K row zeros, since the
+// 16-bit kernel's maximum and exponential may pass over a NaN score. The kernel also sets what the
+// attention's launch needs: row counts that the bound holds, and zeroed arrivals. Bound by memory.
+struct ExpandArgs {
+    Cache src[kMaxBatch];
+    const int32_t* count[kMaxBatch];
+    int32_t n_streams, n_tokens, n_heads, max_rows;
+    void* k;
+    void* v;
+    int32_t* rows;               // [n_streams] counts, clamped to max_rows
+    uint4* zero;
+    int32_t n_zero;
+};
+
+template <typename T, int F>
+__global__ void __launch_bounds__(kReadThreads) q8_expand_kernel(const __grid_constant__ ExpandArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int64_t first = (int64_t)blockIdx.x * kReadThreads + threadIdx.x, stride = (int64_t)gridDim.x * kReadThreads;
+    if (blockIdx.x == 0 && threadIdx.x < kMaxBatch) {
+#pragma unroll
+        for (int b = 0; b < kMaxBatch; ++b)
+            if (b == (int)threadIdx.x && b < a.n_streams) {
+                const int32_t m = *a.count[b];
+                if (m > a.max_rows) atomicOr(&g_error_word, kErrBounds);
+                a.rows[b] = max(0, min(m, a.max_rows));
+            }
+    }
+    for (int64_t e = first; e < a.n_zero; e += stride) a.zero[e] = make_uint4(0, 0, 0, 0);
+    const uint32_t per_row = (uint32_t)a.n_heads * (kHeadDim / 16);
+    const int64_t total = (int64_t)a.n_tokens * per_row;
+    const bool small = total <= 0xffffffffll;
+    const Cache c = a.src[blockIdx.y];
+    T* ko = static_cast<T*>(a.k) + blockIdx.y * total * 16;
+    T* vo = static_cast<T*>(a.v) + blockIdx.y * total * 16;
+    for (int64_t e = first; e < total; e += stride) {
+        const int32_t i = small ? (int32_t)((uint32_t)e / per_row) : (int32_t)(e / per_row);
+        const int32_t h16 = (int32_t)(e - (int64_t)i * per_row);
+        const uint4 ck = __ldcs(reinterpret_cast<const uint4*>(c.k + i * c.ld + h16 * 16));
+        const uint4 cv = __ldcs(reinterpret_cast<const uint4*>(c.v + i * c.ld + h16 * 16));
+        const int64_t at = (int64_t)(h16 >> 3) * c.ld_scale + i;
+        uint32_t sk = static_cast<const uint16_t*>(c.ks)[at], sv = static_cast<const uint16_t*>(c.vs)[at];
+        const bool ok = valid_scale<T, F>(StoreT<T>::unpack2(sk).x) && valid_scale<T, F>(StoreT<T>::unpack2(sv).x);
+        if (!ok) sk = 0;
+        Decoder<T, F> dk, dv;
+        dk.scale(0x10001u * sk);
+        dv.scale(0x10001u * sv);
+        uint4 lo, hi;
+        decode16(ck, dk, lo, hi);
+        uint4* o = reinterpret_cast<uint4*>(ko + e * 16);
+        o[0] = lo;
+        o[1] = hi;
+        decode16(cv, dv, lo, hi);
+        if (!ok) lo = hi = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);   // NaN of either type
+        o = reinterpret_cast<uint4*>(vo + e * 16);
+        o[0] = lo;
+        o[1] = hi;
     }
 }
 

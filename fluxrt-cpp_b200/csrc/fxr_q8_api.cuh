@@ -96,6 +96,14 @@ int32_t launch_q8_write(const fxr_frame_desc* d, const fxr_q8_cache* cache, fxr:
 // 35; 100 rows of 8 heads 30, and 27).
 constexpr int32_t kQ8FewRows = fxr::attn8::kMaxRowsPerStream;
 
+// A call without groups and prefix turns its caches into 16 bits and runs the 16-bit kernel on them, where
+// a stream has at least this many 256-row units and the SMs this many steps (256 rows x 128 keys) each: a
+// step takes 2.0 us there, and 2.6 where converters work along; the rows cost 3.4 ns each (24 heads) and a
+// launch. 24 heads: 2304 rows over 4608 keys 142 us, and 156 with the converters; 4224 over 16896 905, and
+// 1010; the frame of 16896 tokens 586, and 826. Below: 1536 rows over 4608 keys 94.5, and 93; 6 heads with 2304
+// rows 67, and 60. A call without a bound is taken to run a quarter of the tokens.
+constexpr int32_t kQ8WideUnits = 8, kQ8WideSteps = 32;
+
 // Workspace of the attention: arrivals (zero before and after a call), then partial results, then the
 // visible steps of the kernel for many rows.
 struct Q8Work {
@@ -113,6 +121,11 @@ struct Q8Work {
     int32_t slots;        // its partial results: one per column and CTA boundary
     int32_t units;        // 256-row units of a stream, key tiles: the kernel for many
     int32_t n_pre, n_own;
+    bool wide;            // without groups: the 16-bit kernel, in the same place of the workspace
+    char* wide_k;
+    char* wide_v;
+    char* split;
+    int32_t* wide_rows;
     size_t zero_bytes;    // from the start: what has to be zero before a launch
     size_t total;
 };
@@ -155,6 +168,18 @@ Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, in
         w.steps = reinterpret_cast<int32_t*>(take((size_t)(S * w.units) * sizeof(int32_t)));
         w.list = reinterpret_cast<uint16_t*>(take((size_t)(S * w.units) * (size_t)(w.n_pre + w.n_own) * sizeof(uint16_t)));
         w.groups = reinterpret_cast<uint32_t*>(take((size_t)(w.n_pre + S * w.n_own) * fxr::attn8::kBN * sizeof(uint32_t)));
+        const int32_t likely = w.bounded ? w.rows : w.rows / 4;
+        const int64_t units = (likely + fxr::attn8::kUnitRows - 1) / fxr::attn8::kUnitRows;
+        w.wide = n_prefix == 0 && units >= kQ8WideUnits && S * units * d->n_heads * w.n_own >= (int64_t)kQ8WideSteps * sm_count();
+        if (w.wide) {
+            const size_t end = off, bytes = (size_t)S * (size_t)d->n_tokens * (size_t)d->n_heads * (size_t)d->head_dim * 2;
+            off = w.zero_bytes;
+            w.wide_rows = reinterpret_cast<int32_t*>(take(FXR_MAX_BATCH * sizeof(int32_t)));
+            w.split = take(split_bytes(kSplitSlotsPerSm * sm_count()));
+            w.wide_k = take(bytes);
+            w.wide_v = take(bytes);
+            off = std::max(off, end);
+        }
     }
     w.total = off;
     return w;
@@ -262,6 +287,49 @@ int32_t launch_q8_tiles(const fxr_frame_desc* d, const fxr::attn8::Params& p, co
     e = launch_pdl(fxr::attn8::combine_kernel<T>, dim3(sm_count() * fxr::attn8::kCombineCtas), dim3(fxr::attn8::kCombineThreads), 0,
                    s, p, static_cast<const float*>(w.part), static_cast<const fxr::attn8::CutUnit*>(w.cuts));
     return cuda_status(e, "combine_kernel launch");
+}
+
+// Without groups and prefix: the caches in 16 bits, then the 16-bit attention.
+template <typename T, int F>
+int32_t launch_q8_wide(const fxr_frame_desc* d, const fxr::attn8::Params& p, const Q8Work& w, cudaStream_t s) {
+    const int32_t slots = kSplitSlotsPerSm * sm_count();
+    const SplitArea split = split_area(0, w.split, split_bytes(slots), d->n_heads);
+    const int64_t C = (int64_t)d->n_heads * d->head_dim;
+    fxr::q8::ExpandArgs a{};
+    AttnStreamArgs st[FXR_MAX_BATCH];
+    for (int32_t b = 0; b < p.n_streams; ++b) {
+        const size_t first = (size_t)b * (size_t)d->n_tokens * (size_t)C * 2;
+        a.src[b] = p.s[b].c;
+        a.count[b] = p.s[b].count;
+        st[b] = AttnStreamArgs{p.s[b].qc, p.s[b].ld_qc, w.wide_rows + b, w.wide_k + first, w.wide_v + first, p.s[b].idx, p.s[b].out,
+                               nullptr, p.max_rows};
+    }
+    a.n_streams = p.n_streams;
+    a.n_tokens = p.n_tokens;
+    a.n_heads = p.n_heads;
+    a.max_rows = p.max_rows;
+    a.k = w.wide_k;
+    a.v = w.wide_v;
+    a.rows = w.wide_rows;
+    a.zero = reinterpret_cast<uint4*>(split.cnt);
+    a.n_zero = (int32_t)((size_t)split.slots * kSplitCntBytes / sizeof(uint4));
+    const int64_t units = (int64_t)d->n_tokens * d->n_heads * (fxr::kHeadDim / 16);
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((units + fxr::q8::kReadThreads - 1) / fxr::q8::kReadThreads,
+                                                                (int64_t)sm_count() * 64));
+    const int32_t rc = cuda_status(launch_pdl(fxr::q8::q8_expand_kernel<T, F>, dim3(grid, p.n_streams), dim3(fxr::q8::kReadThreads), 0, s, a),
+                                   "q8_expand_kernel launch");
+    if (rc != FXR_OK) return rc;
+    fxr_frame_desc packed = *d;
+    packed.ld_cache = C;
+    // Units cut between CTAs read their keys out of step, which costs L2 hits: a step then takes 1.1 times
+    // one of whole units and more (4224 rows over 16896 keys: 1000 us cut, 905 whole; 3300 rows 818, and 845;
+    // 2304 rows over 4608 keys 142, and 158). The kernel would cut at equal steps; without a bound (the rows are not known here) it decides.
+    const int64_t n = (int64_t)w.units * d->n_heads * p.n_streams, ctas = sm_count();
+    const float whole = (float)((n + ctas - 1) / ctas) * ((float)w.n_own + fxr::attn2::kItemOverheadSteps);
+    const float each = (float)(n * w.n_own) / (float)ctas;
+    const float cut = each + fxr::attn2::kItemOverheadSteps * (each / (float)w.n_own + 1.f) + 2.f * fxr::attn2::kCutOverheadSteps;
+    const bool may_cut = !w.bounded || whole > 1.1f * cut;
+    return launch_attention_streams<T>(&packed, p.n_streams, st, may_cut ? split : SplitArea{}, s);
 }
 
 int32_t check_groups(const uint32_t* g, const char* what) {
@@ -423,6 +491,8 @@ int32_t fxr_attention_q8(const fxr_frame_desc* desc, int32_t n_streams, const fx
             const fxr_q8_stream& s = streams[b0 + b];
             p.s[b] = fxr::attn8::Stream{s.qc, s.idx, s.count, s.out, s.q_groups, s.k_groups, s.ld_qc, q8_arg(&s.cache)};
         }
+        bool groups = false;
+        for (int32_t b = 0; b < p.n_streams; ++b) groups = groups || p.s[b].qg != nullptr || p.s[b].kg != nullptr;
         if (prefix) p.prefix = q8_arg(prefix);
         p.pg = prefix_groups;
         p.n_tokens = desc->n_tokens;
@@ -437,7 +507,7 @@ int32_t fxr_attention_q8(const fxr_frame_desc* desc, int32_t n_streams, const fx
             using T = decltype(t);
             constexpr int F = decltype(f)::value;
             const cudaStream_t cs = static_cast<cudaStream_t>(stream);
-            if (!w.few) return launch_q8_tiles<T, F>(desc, p, w, cs);
+            if (!w.few) return w.wide && !groups ? launch_q8_wide<T, F>(desc, p, w, cs) : launch_q8_tiles<T, F>(desc, p, w, cs);
             return w.tiles == 1   ? launch_q8_rows<T, F, 1>(desc, p, cs)
                    : w.tiles == 2 ? launch_q8_rows<T, F, 2>(desc, p, cs)
                                   : launch_q8_rows<T, F, 4>(desc, p, cs);

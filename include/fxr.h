@@ -687,11 +687,15 @@ int32_t fxr_restore_rows_q8(const fxr_frame_desc* desc, const int32_t* mask, con
  * all bits. A row that sees no key gets zeros. Masked keys contribute nothing, whatever they hold.
  * max_rows: the caller's bound of *count for every stream (<= 0: n_tokens). Rows past it are not
  * computed and set the device error word (FXR_ERR_BOUNDS). qc has to hold max_rows rows: those past
- * *count are read, never used. A tight bound lets calls of few rows take the kernel made for them. Rows of out that are not listed are left as they are.
+ * *count are read, never used. A tight bound lets calls of few rows take the kernel made for them. Rows of
+ * out that are not listed are left as they are.
  * More than FXR_MAX_BATCH streams run as consecutive groups. workspace: at least
  * fxr_attention_q8_workspace_size() bytes, 16-byte aligned, ZERO before its first use and then reused
  * as is by calls on one stream (each call leaves its counters at zero; after FXR_ERR_TIMEOUT zero it
- * again). Calls that may run at the same time need a workspace each. The caches of a call share one
+ * again). With a bound of many rows (about 2000 and more, or a quarter of n_tokens without one) and no
+ * prefix it has room for the K and V rows of one layer in 16 bits, n_tokens * n_heads * head_dim * 4 bytes
+ * per stream of a group, since such calls turn the cache into 16 bits once; one workspace serves every
+ * layer. Calls that may run at the same time need a workspace each. The caches of a call share one
  * format. The result of a call does not depend on the order in which its CTAs run. */
 typedef struct fxr_q8_stream {
     const void* qc;          /* [max_rows, ld_qc] compact queries (fxr_gather_norm_rope_q8), 16-byte aligned */

@@ -700,6 +700,64 @@ def test_scales_far_apart(cuda, dtype, fmt, m, kind):
         check_streams(cfg, [st], what=kind)
 
 
+# calls of many rows without groups and prefix, which read the cache through its 16-bit rows
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, fmt", [("bf16", "int8"), ("bf16", "e4m3"), ("f16", "int8"), ("f16", "e4m3")])
+@pytest.mark.parametrize("counts, n, heads, bound", [((2049,), 4700, 18, 2049), ((2100, 0, 1900), 2501, 16, 2100), ((300,), 8003, 12, 0),
+                                                     ((4224,), 4224, 24, 4224)])
+def test_attention_of_many_rows(cuda, dtype, fmt, counts, n, heads, bound):
+    """Against 64 bits; the same buffers used again, larger rows between; rows behind the counts stay."""
+    g = rng_of(sum(counts) + n)
+    cfg = cfg_of(n, heads, dtype, ld_out=heads * D + 8)
+    streams = []
+    for m in counts:
+        st = stream_of(g, cfg, m, ld_extra=8, out_extra=8)
+        st["cache"] = filled_cache(g, cfg, n + 1, fmt, pad=16, extra_scale=8)
+        streams.append(st)
+    ws = workspace_for(cfg, streams, max_rows=bound)
+    for _ in range(2):
+        for st in streams:
+            st["out"].fill_(7.0)
+        fxr.attention_q8(cfg, streams, ws, max_rows=bound)
+    sync_ok()
+    check_streams(cfg, streams)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, fmt", [("bf16", "e4m3"), ("f16", "int8")])
+def test_many_rows_with_nan_and_beyond_the_bound(cuda, dtype, fmt):
+    """A key without a valid scale makes its head NaN; a count above the bound is an error, and its rows are left."""
+    n, heads, m, bound = 2400, 32, 1950, 1900
+    g = rng_of(5)
+    cfg = cfg_of(n, heads, dtype)
+    st = stream_of(g, cfg, m)
+    st["cache"] = filled_cache(g, cfg, n, fmt)
+    st["cache"].k_scale[3, 3] = math.nan          # a pair of columns whose exponential is the polynomial's
+    st["cache"].v_scale[5, n - 1] = math.inf
+    before = st["out"].clone()
+    fxr.attention_q8(cfg, [st], workspace_for(cfg, [st], max_rows=bound), max_rows=bound)
+    with pytest.raises(fxr.FxrError) as e:
+        fxr.check_device_error()
+    assert e.value.status == fxr.FXR_ERR_BOUNDS
+    rows = st["idx"][:m].long()
+    assert torch.equal(st["out"][rows[bound:]], before[rows[bound:]])
+    out = st["out"][rows[:bound]].view(bound, heads, D)
+    bad = torch.zeros(heads, dtype=torch.bool, device="cuda")
+    bad[3] = bad[5] = True
+    assert torch.equal(torch.isnan(out).all(-1), bad.expand(bound, heads)) and torch.isnan(out).any(-1).sum() == 2 * bound
+    # a call with groups in the same workspace, which the other kernel takes, and the first again
+    st["cache"] = filled_cache(g, cfg, n, fmt)
+    st["m"] = bound
+    st["count"].fill_(bound)
+    ws = workspace_for(cfg, [st], max_rows=bound)
+    for groups in (None, torch.ones(n, dtype=torch.int32, device="cuda"), None):
+        st["q_groups"] = st["k_groups"] = groups
+        st["out"].fill_(7.0)
+        fxr.attention_q8(cfg, [st], ws, max_rows=bound)
+        sync_ok()
+        check_streams(cfg, [st])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m", [6, 280])
 def test_groups_of_queries_alone_and_queries_that_are_nan(cuda, m):
