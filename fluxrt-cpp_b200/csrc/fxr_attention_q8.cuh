@@ -824,6 +824,8 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
 // scores masked. With visibility groups, visible_steps_kernel lists for every 256-row unit the tiles
 // that some row of it sees, and which of them all its rows see whole; the others are masked score by
 // score. Rows that see nothing end with a maximum of -inf and store zeros.
+// Rounded to T: K and V, as the read-back does, and P, since the products take 16-bit operands (half a step each);
+// scores, maxima, sums and O are held in 32 bits.
 // ---------------------------------------------------------------------------------------------
 constexpr int kBM = 128, kUnitRows = 2 * kBM, kBN = 128, kD = kHeadDim;
 constexpr int kTileThreads = 512;

@@ -168,10 +168,13 @@ Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, in
         w.steps = reinterpret_cast<int32_t*>(take((size_t)(S * w.units) * sizeof(int32_t)));
         w.list = reinterpret_cast<uint16_t*>(take((size_t)(S * w.units) * (size_t)(w.n_pre + w.n_own) * sizeof(uint16_t)));
         w.groups = reinterpret_cast<uint32_t*>(take((size_t)(w.n_pre + S * w.n_own) * fxr::attn8::kBN * sizeof(uint32_t)));
-        const int32_t likely = w.bounded ? w.rows : w.rows / 4;
-        const int64_t units = (likely + fxr::attn8::kUnitRows - 1) / fxr::attn8::kUnitRows;
-        w.wide = n_prefix == 0 && units >= kQ8WideUnits && S * units * d->n_heads * w.n_own >= (int64_t)kQ8WideSteps * sm_count();
-        if (w.wide) {
+        // room for it wherever a bound of w.rows takes it, so that the size is one of the bound alone
+        auto many = [&](int32_t rows) {
+            const int64_t units = (rows + fxr::attn8::kUnitRows - 1) / fxr::attn8::kUnitRows;
+            return n_prefix == 0 && units >= kQ8WideUnits && S * units * d->n_heads * w.n_own >= (int64_t)kQ8WideSteps * sm_count();
+        };
+        w.wide = many(w.bounded ? w.rows : w.rows / 4);
+        if (many(w.rows)) {
             const size_t end = off, bytes = (size_t)S * (size_t)d->n_tokens * (size_t)d->n_heads * (size_t)d->head_dim * 2;
             off = w.zero_bytes;
             w.wide_rows = reinterpret_cast<int32_t*>(take(FXR_MAX_BATCH * sizeof(int32_t)));

@@ -692,7 +692,7 @@ int32_t fxr_restore_rows_q8(const fxr_frame_desc* desc, const int32_t* mask, con
  * More than FXR_MAX_BATCH streams run as consecutive groups. workspace: at least
  * fxr_attention_q8_workspace_size() bytes, 16-byte aligned, ZERO before its first use and then reused
  * as is by calls on one stream (each call leaves its counters at zero; after FXR_ERR_TIMEOUT zero it
- * again). With a bound of many rows (about 2000 and more, or a quarter of n_tokens without one) and no
+ * again). With a bound of many rows (about 2000 and more, n_tokens without one) and no
  * prefix it has room for the K and V rows of one layer in 16 bits, n_tokens * n_heads * head_dim * 4 bytes
  * per stream of a group, since such calls turn the cache into 16 bits once; one workspace serves every
  * layer. Calls that may run at the same time need a workspace each. The caches of a call share one

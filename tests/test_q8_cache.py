@@ -721,6 +721,17 @@ def test_attention_of_many_rows(cuda, dtype, fmt, counts, n, heads, bound):
         fxr.attention_q8(cfg, streams, ws, max_rows=bound)
     sync_ok()
     check_streams(cfg, streams)
+    # captured, and replayed with other counts
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fxr.attention_q8(cfg, streams, ws, max_rows=bound)
+    for st in streams:
+        st["m"] = st["m"] * 2 // 3
+        st["count"].fill_(st["m"])
+        st["out"].fill_(7.0)
+    graph.replay()
+    sync_ok()
+    check_streams(cfg, streams)
 
 
 @pytest.mark.gpu
