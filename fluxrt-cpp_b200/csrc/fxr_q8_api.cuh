@@ -126,7 +126,7 @@ struct Q8Work {
     char* wide_v;
     char* split;
     int32_t* wide_rows;
-    size_t zero_bytes;    // from the start: what has to be zero before a launch
+    size_t zero_bytes;    // from the start: what has to be zero before a launch, and is after it
     size_t total;
 };
 
@@ -143,11 +143,13 @@ Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, in
         off = align_up(off + bytes, 256);
         return p;
     };
-    // one place and size for the arrivals, whichever kernel a call takes: calls with other bounds may
-    // share a workspace
-    const size_t ctas = (size_t)sm_count();
-    w.cnt = reinterpret_cast<int32_t*>(take((size_t)d->n_heads * FXR_MAX_BATCH * fxr::attn8::kGroupsPerStream * sizeof(int32_t)));
-    w.zero_bytes = off;
+    // one place and size for the arrivals, whichever kernel a call takes and however many heads it has (up
+    // to 256): calls of other bounds and head counts may share a workspace, and none writes anything else
+    // where another has its arrivals
+    const size_t ctas = (size_t)sm_count(), per_head = (size_t)FXR_MAX_BATCH * fxr::attn8::kGroupsPerStream * sizeof(int32_t);
+    w.cnt = reinterpret_cast<int32_t*>(take((size_t)std::max(d->n_heads, 256) * per_head));
+    w.zero_bytes = align_up((size_t)d->n_heads * per_head, 16);
+    const size_t body = off;
     if (w.few) {
         // groups as large as a stream's rows need; the packed rows of a prefix fill groups of 16 at most
         // otherwise (of 32, and 8 warps, took 85 us where 16 rows and 16 warps take 79: 8 streams of 15
@@ -176,7 +178,7 @@ Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, in
         w.wide = many(w.bounded ? w.rows : w.rows / 4);
         if (many(w.rows)) {
             const size_t end = off, bytes = (size_t)S * (size_t)d->n_tokens * (size_t)d->n_heads * (size_t)d->head_dim * 2;
-            off = w.zero_bytes;
+            off = body;
             w.wide_rows = reinterpret_cast<int32_t*>(take(FXR_MAX_BATCH * sizeof(int32_t)));
             w.split = take(split_bytes(kSplitSlotsPerSm * sm_count()));
             w.wide_k = take(bytes);

@@ -691,8 +691,8 @@ int32_t fxr_restore_rows_q8(const fxr_frame_desc* desc, const int32_t* mask, con
  * out that are not listed are left as they are.
  * More than FXR_MAX_BATCH streams run as consecutive groups. workspace: at least
  * fxr_attention_q8_workspace_size() bytes, 16-byte aligned, ZERO before its first use and then reused
- * as is by calls on one stream (each call leaves its counters at zero; after FXR_ERR_TIMEOUT zero it
- * again). With a bound of many rows (about 2000 and more, n_tokens without one) and no
+ * as is by calls on one stream, of any bound, format and (up to 256) head count, where it is large enough
+ * (each call leaves its counters at zero; after FXR_ERR_TIMEOUT zero it again). With a bound of many rows (about 2000 and more, n_tokens without one) and no
  * prefix it has room for the K and V rows of one layer in 16 bits, n_tokens * n_heads * head_dim * 4 bytes
  * per stream of a group, since such calls turn the cache into 16 bits once; one workspace serves every
  * layer. Calls that may run at the same time need a workspace each. The caches of a call share one
@@ -700,7 +700,7 @@ int32_t fxr_restore_rows_q8(const fxr_frame_desc* desc, const int32_t* mask, con
 typedef struct fxr_q8_stream {
     const void* qc;          /* [max_rows, ld_qc] compact queries (fxr_gather_norm_rope_q8), 16-byte aligned */
     int64_t ld_qc;           /* elements, a multiple of 8 */
-    const int32_t* idx;
+    const int32_t* idx;      /* distinct tokens */
     const int32_t* count;
     void* out;               /* [n_tokens, desc->ld_out], 16-byte aligned */
     const uint32_t* q_groups;/* [n_tokens] or NULL */

@@ -700,6 +700,26 @@ def test_scales_far_apart(cuda, dtype, fmt, m, kind):
         check_streams(cfg, [st], what=kind)
 
 
+@pytest.mark.gpu
+def test_one_workspace_for_calls_of_other_shapes(cuda):
+    """Calls of few, more and many rows, with few heads and many, one after the other in one workspace."""
+    g = rng_of(11)
+    calls = []
+    for n, heads, m, dtype, fmt in ((600, 2, 300, "bf16", "int8"), (900, 24, 5, "f16", "e4m3"), (2049, 48, 1900, "f16", "int8"),
+                                    (700, 32, 17, "bf16", "e4m3"), (400, 1, 9, "bf16", "int8")):
+        cfg = cfg_of(n, heads, dtype)
+        st = stream_of(g, cfg, m)
+        st["cache"] = filled_cache(g, cfg, n, fmt)
+        calls.append((cfg, st, m))
+    ws = torch.zeros(max(fxr.attention_q8_workspace_size(cfg, 1, 0, m) for cfg, _, m in calls), dtype=torch.uint8, device="cuda")
+    for _ in range(2):
+        for cfg, st, m in calls:
+            st["out"].fill_(7.0)
+            fxr.attention_q8(cfg, [st], ws, max_rows=m)
+            sync_ok()
+            check_streams(cfg, [st])
+
+
 # calls of many rows without groups and prefix, which read the cache through its 16-bit rows
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype, fmt", [("bf16", "int8"), ("bf16", "e4m3"), ("f16", "int8"), ("f16", "e4m3")])
