@@ -321,7 +321,9 @@ __device__ __forceinline__ void quantise_store(float2* y, uint8_t* codes, T* sca
 
 // Executed rows into the 8-bit cache. Eight lanes hold a 128-wide head vector, 16 values each, so that
 // rotary pairs are lane-local and the sum of squares and the largest magnitude are 3-step shuffles; a
-// warp runs four heads of Q, K and V at a time, and a row's heads are divided over `parts` warps. Three
+// warp runs four heads of Q, K and V at a time (a unit). The launch's units are divided evenly over the
+// warps, and a warp loads its next unit, also the next row's, while it works on one (1536 rows of 24 heads
+// 13.6 us; 16.5 with a warp per row, which leaves a third of them idle, 17.1 with three per row). Three
 // rows of T are read, one of T and two of bytes written per token: bound by memory (16896 rows of 24
 // heads: 100 us, 5.2 TB/s; two lanes' worth of shuffles and a division per code took 211 us).
 template <typename T, int F, bool kRaw>
@@ -331,12 +333,12 @@ __global__ void __launch_bounds__(kWriteThreads, 2) q8_write_kernel(const __grid
     pdl_launch_dependents();
     pdl_wait();
     const int32_t m_all = min(a.count ? *a.count : a.host_count, a.n_tokens);
+    // the launch's line of (row, quad of heads) units, one range per warp
     const int32_t quads = (a.n_heads + kVecHeads - 1) / kVecHeads;
-    // (dividing rows further, to even out the warps' last round, costs more than it gains: 1536 rows
-    // 16.5 us, in three parts each 17.1)
-    const int32_t parts = m_all > 0 ? max(1, min(quads, warps / m_all)) : 1;
-    const int64_t items = (int64_t)m_all * parts;
-    if (warp >= items) return;
+    const int64_t total = (int64_t)max(m_all, 0) * quads, per = max((int64_t)1, (total + warps - 1) / warps);
+    const int64_t first = warp * per;
+    int32_t left = (int32_t)(min(total, first + per) - first);
+    if (left <= 0) return;
     float2 wq[kVecPairs], wk[kVecPairs];
     if (!kRaw) {
 #pragma unroll
@@ -346,41 +348,50 @@ __global__ void __launch_bounds__(kWriteThreads, 2) q8_write_kernel(const __grid
             wk[t] = make_float2(a.norm_k[e], a.norm_k[e + 1]);
         }
     }
-    for (int64_t item = warp; item < items; item += warps) {
-        const int32_t m = (int32_t)(item / parts), part = (int32_t)(item - (int64_t)m * parts);
-        const int32_t i = a.idx ? a.idx[m] : m;
-        if (i < 0 || i >= a.n_tokens) {
-            if (lane == 0) atomicOr(&g_error_word, kErrBounds);
-            continue;
-        }
-        const bool keep = !kRaw && a.save != nullptr && a.mask[i] == 1;
-        uint4 nq[2], nk[2], nv[2];      // the next heads' vectors are on their way while these are worked on
-        auto load = [&](int32_t quad) {
-            const int32_t h = kVecHeads * quad + of;
-            const int64_t at = (int64_t)i * a.ld_qkv + (int64_t)(h < a.n_heads ? h : 0) * kHeadDim + 16 * sub;
-            const uint4* k = reinterpret_cast<const uint4*>(static_cast<const T*>(a.k) + at);
-            const uint4* v = reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + at);
-            if (!kRaw) {
-                const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at);
-                nq[0] = __ldcs(q);
-                nq[1] = __ldcs(q + 1);
-            }
-            nk[0] = __ldcs(k);
-            nk[1] = __ldcs(k + 1);
-            nv[0] = __ldcs(v);
-            nv[1] = __ldcs(v + 1);
-        };
-        load(part);
-        float cs[kVecPairs], sn[kVecPairs];
+    int32_t m = (int32_t)(first / quads), quad = (int32_t)(first - (int64_t)m * quads);
+    auto token = [&](int32_t row) { return row < m_all ? (a.idx ? a.idx[row] : row) : -1; };
+    auto listed = [&](int32_t i) { return i >= 0 && i < a.n_tokens; };
+    uint4 nq[2], nk[2], nv[2];      // the next heads' vectors are on their way while these are worked on
+    auto load = [&](int32_t i, int32_t quad) {
+        const int32_t h = kVecHeads * quad + of;
+        const int64_t at = (int64_t)i * a.ld_qkv + (int64_t)(h < a.n_heads ? h : 0) * kHeadDim + 16 * sub;
+        const uint4* k = reinterpret_cast<const uint4*>(static_cast<const T*>(a.k) + at);
+        const uint4* v = reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + at);
         if (!kRaw) {
+            const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + at);
+            nq[0] = __ldcs(q);
+            nq[1] = __ldcs(q + 1);
+        }
+        nk[0] = __ldcs(k);
+        nk[1] = __ldcs(k + 1);
+        nv[0] = __ldcs(v);
+        nv[1] = __ldcs(v + 1);
+    };
+    float cs[kVecPairs], sn[kVecPairs];
+    int32_t i = token(m), next_i = -1;
+    bool fresh = true, keep = false;
+    if (listed(i)) load(i, quad);
+    for (; left > 0; --left) {
+        if (fresh) {
+            fresh = false;
+            next_i = token(m + 1);
+            if (listed(i)) {
+                keep = !kRaw && a.save != nullptr && a.mask[i] == 1;
+                if (!kRaw) {
 #pragma unroll
-            for (int t = 0; t < kVecPairs; ++t) {
-                const int j = kVecPairs * sub + t;
-                const float at = a.n_axes > 0 ? (float)a.pos[(int64_t)i * a.n_axes + a.axis[j]] : 0.f;
-                rope_turn(at, a.turns[j], &sn[t], &cs[t]);
+                    for (int t = 0; t < kVecPairs; ++t) {
+                        const int j = kVecPairs * sub + t;
+                        const float at = a.n_axes > 0 ? (float)a.pos[(int64_t)i * a.n_axes + a.axis[j]] : 0.f;
+                        rope_turn(at, a.turns[j], &sn[t], &cs[t]);
+                    }
+                }
+            } else if (lane == 0) {
+                atomicOr(&g_error_word, kErrBounds);
             }
         }
-        for (int32_t quad = part; quad < quads; quad += parts) {
+        const bool last = quad + 1 == quads;
+        const int32_t then_i = last ? next_i : i, then_quad = last ? 0 : quad + 1;
+        if (listed(i)) {
             const int32_t h = kVecHeads * quad + of;
             const bool active = h < a.n_heads;
             const int64_t col = (int64_t)(active ? h : 0) * kHeadDim;
@@ -414,12 +425,18 @@ __global__ void __launch_bounds__(kWriteThreads, 2) q8_write_kernel(const __grid
             }
             unpack16<T>(nk, y);
             const uint4 xv[2] = {nv[0], nv[1]};
-            if (quad + parts < quads) load(quad + parts);
+            if (left > 1 && listed(then_i)) load(then_i, then_quad);
             if (!kRaw) norm_rope16(y, wk, a.eps, cs, sn);
             quantise_store<T, F, kRaw>(y, ck, ks, sub, active);
             unpack16<T>(xv, y);
             quantise_store<T, F, true>(y, cv, vs, sub, active);
+        } else if (left > 1 && listed(then_i)) {
+            load(then_i, then_quad);
         }
+        i = then_i;
+        quad = then_quad;
+        m += last;
+        fresh = last;
     }
 }
 
