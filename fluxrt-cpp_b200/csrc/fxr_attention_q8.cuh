@@ -78,7 +78,6 @@ constexpr int kMaxRowsPerStream = 32;          // what the launch accepts
 constexpr int kGroupsPerStream = kMaxRowsPerStream / 8;
 constexpr uint32_t kBlkBytes = kBlk * 128;     // codes of one of K, V (128-byte swizzle)
 constexpr uint32_t kRingSlot = 2 * kBlkBytes;
-constexpr uint32_t kScaleSlot = 2 * kBlk * 2;  // a block's K scales, V scales
 constexpr int kPadRow = 132;                   // floats per O row in the warps' exchange
 constexpr uint32_t kQPad = 272;                // bytes per query row
 constexpr int kRowsSlotFloats = kRowsMax * kHeadDim + 2 * kRowsMax;
@@ -87,8 +86,7 @@ constexpr int kRowsSlotFloats = kRowsMax * kHeadDim + 2 * kRowsMax;
 template <int NQ> struct RowsShape {
     static constexpr int rows = 8 * NQ, warps = NQ > 2 ? 8 : 16, threads = 32 * warps, depth = NQ > 2 ? 5 : 3;
     static constexpr uint32_t ring_warp = depth * kRingSlot;
-    static constexpr uint32_t at_scale = warps * ring_warp;
-    static constexpr uint32_t at_q = at_scale + warps * depth * kScaleSlot;
+    static constexpr uint32_t at_q = warps * ring_warp;
     static constexpr uint32_t at_m = at_q + rows * kQPad;               // maxima, sums: [rows][warps]; queries' factors
     static constexpr uint32_t at_bar = at_m + (2 * warps + 1) * rows * 4;
     static constexpr uint32_t smem = at_bar + warps * depth * 8 + 1024; // + alignment slack
@@ -419,19 +417,21 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
         const uint16_t* ks = static_cast<const uint16_t*>(ks0) + (int64_t)h * ld_scale + k0;
         const uint16_t* vs = static_cast<const uint16_t*>(vs0) + (int64_t)h * ld_scale + k0;
         if (kg != nullptr) kg += k0;
-        // ---- copies of block b of this warp's walk, the `at`-th it takes. Codes past the source are
-        // zeros; scales come in groups of 8, to which their rows are padded.
+        // ---- copies of block b of this warp's walk, the `nth` that it takes. Codes past the source are zeros.
         auto fetch = [&](int32_t b, uint32_t nth) {
             if (lane == 0) {
                 const uint32_t slot = nth % kDepth, bar = bars + 8 * slot, dst = ring + slot * kRingSlot;
-                const uint32_t sdst = base + Sh::at_scale + (warp * kDepth + slot) * kScaleSlot;
-                const uint32_t sbytes = n_keys - b * kBlk > 8 ? 32u : 16u;
-                mbar_arrive_expect_tx(bar, kRingSlot + 2 * sbytes);
+                mbar_arrive_expect_tx(bar, kRingSlot);
                 tma_load_2d(dst, tk, bar, h * kHeadDim, k0 + b * kBlk);
                 tma_load_2d(dst + kBlkBytes, tv, bar, h * kHeadDim, k0 + b * kBlk);
-                bulk_load(sdst, ks + b * kBlk, sbytes, bar);
-                bulk_load(sdst + kBlk * 2, vs + b * kBlk, sbytes, bar);
             }
+        };
+        // a block's 16 K and 16 V scales, one per lane, a block ahead (two copies fewer per block than by TMA: 12
+        // rows over 16896 keys 32.2 us, and 32.6)
+        uint32_t sc_next = 0;
+        auto scales_of = [&](int32_t b) {
+            const int32_t key = b * kBlk + (int32_t)(lane & 15);
+            sc_next = key < n_keys ? __ldg((lane < 16 ? ks : vs) + key) : 0u;
         };
         uint32_t g_next[2] = {0xffffffffu, 0xffffffffu};     // groups of this lane's keys, a block ahead
         auto groups_of = [&](int32_t b) {
@@ -448,6 +448,7 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
             const int32_t b = warp + d * kRowsWarps;
             if (b < n_blk) fetch(b, it + d);
         }
+        scales_of(warp);
         groups_of(warp);
 
         // ---- queries into shared memory (a 16-byte piece per thread), this lane's rows' groups
@@ -548,11 +549,12 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
                 ++issued;
             }
             const uint32_t seen[2] = {g_next[0], g_next[1]};
+            const uint32_t sc = sc_next;
+            scales_of(b + kRowsWarps);
             groups_of(b + kRowsWarps);
             const uint32_t slot = it % kDepth;
             if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * slot, (it / kDepth) & 1, &abort))) break;
             const uint8_t* blk_p = smem + warp * Sh::ring_warp + slot * kRingSlot;
-            const uint16_t* sc_p = reinterpret_cast<const uint16_t*>(smem + Sh::at_scale + (warp * kDepth + slot) * kScaleSlot);
             // S^T = K Q^T
             float s[NQ][4];
 #pragma unroll
@@ -587,7 +589,8 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int key = key_of(g) + 8 * e;
-                const float kk = StoreT<T>::unpack2(sc_p[key]).x, vv = StoreT<T>::unpack2(sc_p[kBlk + key]).x;
+                const float kk = StoreT<T>::unpack2(__shfl_sync(0xffffffffu, sc, key)).x;
+                const float vv = StoreT<T>::unpack2(__shfl_sync(0xffffffffu, sc, kBlk + key)).x;
                 const bool v_ok = q8::valid_scale<T, F>(vv);
                 const float f = v_ok && q8::valid_scale<T, F>(kk) ? kk : __uint_as_float(0x7fc00000u);
                 v_sc[e] = v_ok ? vv : 0.f;
