@@ -100,7 +100,7 @@ constexpr int32_t kQ8FewRows = fxr::attn8::kMaxRowsPerStream;
 // a stream has at least this many 256-row units and the SMs this many steps (256 rows x 128 keys) each: a
 // step takes 2.0 us there, and 2.6 where converters work along; the rows cost 3.4 ns each (24 heads) and a
 // launch. 24 heads: 2304 rows over 4608 keys 142 us, and 156 with the converters; 4224 over 16896 905, and
-// 1010; the frame of 16896 tokens 586, and 826. Below: 1536 rows over 4608 keys 94.5, and 93; 6 heads with 2304
+// 1010; the frame of 16896 tokens 586 to 662, and 826. Below: 1536 rows over 4608 keys 94.5, and 93; 6 heads with 2304
 // rows 67, and 60. A call without a bound is taken to run a quarter of the tokens.
 constexpr int32_t kQ8WideUnits = 8, kQ8WideSteps = 32;
 
