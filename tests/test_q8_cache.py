@@ -724,7 +724,7 @@ def test_one_workspace_for_calls_of_other_shapes(cuda):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype, fmt", [("bf16", "int8"), ("bf16", "e4m3"), ("f16", "int8"), ("f16", "e4m3")])
 @pytest.mark.parametrize("counts, n, heads, bound", [((2049,), 4700, 18, 2049), ((2100, 0, 1900), 2501, 16, 2100), ((300,), 8003, 12, 0),
-                                                     ((4224,), 4224, 24, 4224)])
+                                                     ((4224,), 4224, 24, 4224), ((2600,), 7003, 8, 2600)])
 def test_attention_of_many_rows(cuda, dtype, fmt, counts, n, heads, bound):
     """Against 64 bits; the same buffers used again, larger rows between; rows behind the counts stay."""
     g = rng_of(sum(counts) + n)
