@@ -443,13 +443,16 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
                 }
             }
         };
+        auto begin_walk = [&]() {
 #pragma unroll
-        for (int d = 0; d < kDepth - 1; ++d) {
-            const int32_t b = warp + d * kRowsWarps;
-            if (b < n_blk) fetch(b, it + d);
-        }
-        scales_of(warp);
-        groups_of(warp);
+            for (int d = 0; d < kDepth - 1; ++d) {
+                const int32_t b = warp + d * kRowsWarps;
+                if (b < n_blk) fetch(b, it + d);
+            }
+            scales_of(warp);
+            groups_of(warp);
+        };
+        begin_walk();
 
         // ---- queries into shared memory (a 16-byte piece per thread), this lane's rows' groups
         auto row_at = [&](int32_t e, int32_t& b, int32_t& m) -> bool {      // row e of the group
@@ -525,165 +528,188 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
         __syncthreads();
 
         float o[NQ][8][4], m_run[NQ][2], l_run[NQ][2];
-#pragma unroll
-        for (int q = 0; q < NQ; ++q) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[q][j][e] = 0.f;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                m_run[q][e] = -INFINITY;
-                l_run[q][e] = 0.f;
-            }
-        }
         float qs[NQ][2];                     // score factors of this lane's queries
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
 #pragma unroll
             for (int d = 0; d < 2; ++d) qs[q][d] = p.scale_log2 * q_factor[8 * q + 2 * t + d];
-        uint32_t issued = it + min(kDepth - 1, (n_blk - warp + kRowsWarps - 1) / kRowsWarps);
-        for (int32_t b = warp; b < n_blk; b += kRowsWarps, ++it) {
-            if (b + (kDepth - 1) * kRowsWarps < n_blk) {
-                fetch(b + (kDepth - 1) * kRowsWarps, it + kDepth - 1);
-                ++issued;
-            }
-            const uint32_t seen[2] = {g_next[0], g_next[1]};
-            const uint32_t sc = sc_next;
-            scales_of(b + kRowsWarps);
-            groups_of(b + kRowsWarps);
-            const uint32_t slot = it % kDepth;
-            if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * slot, (it / kDepth) & 1, &abort))) break;
-            const uint8_t* blk_p = smem + warp * Sh::ring_warp + slot * kRingSlot;
-            // S^T = K Q^T
-            float s[NQ][4];
+        auto walk = [&](auto any_code) {
+            constexpr bool kAnyCode = decltype(any_code)::value;
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) s[q][0] = s[q][1] = s[q][2] = s[q][3] = 0.f;
+            for (int q = 0; q < NQ; ++q) {
 #pragma unroll
-            for (int cc = 0; cc < 2; ++cc) {
-                const uint32_t off = key_of(g) * 128 + ((uint32_t)((cc * 4 + t) ^ key_of(g)) << 4);
-                const uint4 ka = *reinterpret_cast<const uint4*>(blk_p + off), kb = *reinterpret_cast<const uint4*>(blk_p + off + 8 * 128);
-                const uint32_t wa[4] = {q8::code_word<F>(ka.x), q8::code_word<F>(ka.y), q8::code_word<F>(ka.z), q8::code_word<F>(ka.w)};
-                const uint32_t wb[4] = {q8::code_word<F>(kb.x), q8::code_word<F>(kb.y), q8::code_word<F>(kb.z), q8::code_word<F>(kb.w)};
+                for (int j = 0; j < 8; ++j)
 #pragma unroll
-                for (int jp = 0; jp < 2; ++jp) {
-                    uint4 q4[NQ];
-#pragma unroll
-                    for (int q = 0; q < NQ; ++q)
-                        q4[q] = *reinterpret_cast<const uint4*>(smem + Sh::at_q + (g + 8 * q) * kQPad + (cc * 64 + t * 16 + jp * 8) * 2);
-#pragma unroll
-                    for (int jj = 0; jj < 2; ++jj) {
-                        const int j = 2 * jp + jj;
-                        const uint32_t a0 = q8::code_pair<F>(wa[j], false), a1 = q8::code_pair<F>(wb[j], false);
-                        const uint32_t a2 = q8::code_pair<F>(wa[j], true), a3 = q8::code_pair<F>(wb[j], true);
-#pragma unroll
-                        for (int q = 0; q < NQ; ++q)
-                            mma16816(s[q], a0, a1, a2, a3, jj ? q4[q].z : q4[q].x, jj ? q4[q].w : q4[q].y);
-                    }
-                }
-            }
-            // scales and masks: this lane's keys, key_of(g) and 8 behind it
-            float v_sc[2], v_log[2];     // what P is multiplied with, its logarithm
-            const int32_t left = n_keys - b * kBlk;
-            bool grow = false;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int key = key_of(g) + 8 * e;
-                const float kk = StoreT<T>::unpack2(__shfl_sync(0xffffffffu, sc, key)).x;
-                const float vv = StoreT<T>::unpack2(__shfl_sync(0xffffffffu, sc, kBlk + key)).x;
-                const bool v_ok = q8::valid_scale<T, F>(vv);
-                const float f = v_ok && q8::valid_scale<T, F>(kk) ? kk : __uint_as_float(0x7fc00000u);
-                v_sc[e] = v_ok ? vv : 0.f;
-                // (bounded below, so that exp2(score - maximum) stays finite: V scales under 2^-100 lose bits)
-                v_log[e] = fmaxf(lg2_approx(v_sc[e]), -100.f);
-#pragma unroll
-                for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                    for (int d = 0; d < 2; ++d) s[q][2 * e + d] *= f * qs[q][d];
-            }
-            if (kg != nullptr || left < kBlk) {
+                    for (int e = 0; e < 4; ++e) o[q][j][e] = 0.f;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const bool in = key_of(g) + 8 * e < left;
+                    m_run[q][e] = -INFINITY;
+                    l_run[q][e] = 0.f;
+                }
+            }
+            uint32_t issued = it + min(kDepth - 1, (n_blk - warp + kRowsWarps - 1) / kRowsWarps);
+            for (int32_t b = warp; b < n_blk; b += kRowsWarps, ++it) {
+                if (b + (kDepth - 1) * kRowsWarps < n_blk) {
+                    fetch(b + (kDepth - 1) * kRowsWarps, it + kDepth - 1);
+                    ++issued;
+                }
+                const uint32_t seen[2] = {g_next[0], g_next[1]};
+                const uint32_t sc = sc_next;
+                scales_of(b + kRowsWarps);
+                groups_of(b + kRowsWarps);
+                const uint32_t slot = it % kDepth;
+                if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * slot, (it / kDepth) & 1, &abort))) break;
+                const uint8_t* blk_p = smem + warp * Sh::ring_warp + slot * kRingSlot;
+                // S^T = K Q^T
+                float s[NQ][4];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) s[q][0] = s[q][1] = s[q][2] = s[q][3] = 0.f;
+#pragma unroll
+                for (int cc = 0; cc < 2; ++cc) {
+                    const uint32_t off = key_of(g) * 128 + ((uint32_t)((cc * 4 + t) ^ key_of(g)) << 4);
+                    const uint4 ka = *reinterpret_cast<const uint4*>(blk_p + off), kb = *reinterpret_cast<const uint4*>(blk_p + off + 8 * 128);
+                    const uint32_t wa[4] = {q8::code_word<F>(ka.x), q8::code_word<F>(ka.y), q8::code_word<F>(ka.z), q8::code_word<F>(ka.w)};
+                    const uint32_t wb[4] = {q8::code_word<F>(kb.x), q8::code_word<F>(kb.y), q8::code_word<F>(kb.z), q8::code_word<F>(kb.w)};
+#pragma unroll
+                    for (int jp = 0; jp < 2; ++jp) {
+                        uint4 q4[NQ];
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q)
+                            q4[q] = *reinterpret_cast<const uint4*>(smem + Sh::at_q + (g + 8 * q) * kQPad + (cc * 64 + t * 16 + jp * 8) * 2);
+#pragma unroll
+                        for (int jj = 0; jj < 2; ++jj) {
+                            const int j = 2 * jp + jj;
+                            const uint32_t a0 = q8::code_pair<F, kAnyCode>(wa[j], false), a1 = q8::code_pair<F, kAnyCode>(wb[j], false);
+                            const uint32_t a2 = q8::code_pair<F, kAnyCode>(wa[j], true), a3 = q8::code_pair<F, kAnyCode>(wb[j], true);
+#pragma unroll
+                            for (int q = 0; q < NQ; ++q)
+                                mma16816(s[q], a0, a1, a2, a3, jj ? q4[q].z : q4[q].x, jj ? q4[q].w : q4[q].y);
+                        }
+                    }
+                }
+                // scales and masks: this lane's keys, key_of(g) and 8 behind it
+                float v_sc[2], v_log[2];     // what P is multiplied with, its logarithm
+                const int32_t left = n_keys - b * kBlk;
+                bool grow = false;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int key = key_of(g) + 8 * e;
+                    const float kk = StoreT<T>::unpack2(__shfl_sync(0xffffffffu, sc, key)).x;
+                    const float vv = StoreT<T>::unpack2(__shfl_sync(0xffffffffu, sc, kBlk + key)).x;
+                    const bool v_ok = q8::valid_scale<T, F>(vv);
+                    const float f = v_ok && q8::valid_scale<T, F>(kk) ? kk : __uint_as_float(0x7fc00000u);
+                    v_sc[e] = v_ok ? vv : 0.f;
+                    // (bounded below, so that exp2(score - maximum) stays finite: V scales under 2^-100 lose bits)
+                    v_log[e] = fmaxf(lg2_approx(v_sc[e]), -100.f);
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) s[q][2 * e + d] *= f * qs[q][d];
+                }
+                if (kg != nullptr || left < kBlk) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const bool in = key_of(g) + 8 * e < left;
+#pragma unroll
+                        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                            for (int d = 0; d < 2; ++d)
+                                if (!in || (seen[e] & qg[q][d]) == 0) s[q][2 * e + d] = -INFINITY;
+                    }
+                } else if (any_empty) {
 #pragma unroll
                     for (int q = 0; q < NQ; ++q)
 #pragma unroll
                         for (int d = 0; d < 2; ++d)
-                            if (!in || (seen[e] & qg[q][d]) == 0) s[q][2 * e + d] = -INFINITY;
+                            if (qg[q][d] == 0) s[q][d] = s[q][2 + d] = -INFINITY;
                 }
-            } else if (any_empty) {
 #pragma unroll
                 for (int q = 0; q < NQ; ++q)
 #pragma unroll
                     for (int d = 0; d < 2; ++d)
-                        if (qg[q][d] == 0) s[q][d] = s[q][2 + d] = -INFINITY;
+                        grow = grow || fmaxf(s[q][d] + v_log[0], s[q][2 + d] + v_log[1]) > m_run[q][d] + 8.f;
+                // the running maxima move only where a weight passes one by more than 2^8 (P stays below that)
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            float x = fmaxf(s[q][d] + v_log[0], s[q][2 + d] + v_log[1]);
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                            const float mn = fmaxf(m_run[q][d], x);
+                            const float al = mn == m_run[q][d] ? 1.f : ex2_approx(m_run[q][d] - mn);
+                            m_run[q][d] = mn;
+                            l_run[q][d] *= al;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                o[q][j][d] *= al;
+                                o[q][j][2 + d] *= al;
+                            }
+                        }
+                }
+                uint32_t pb[NQ][2];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    float e_[4];
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        const float mu = m_run[q][d] == -INFINITY ? 0.f : m_run[q][d];
+                        e_[d] = ex2_approx(s[q][d] - mu);
+                        e_[2 + d] = ex2_approx(s[q][2 + d] - mu);
+                        l_run[q][d] += e_[d] + e_[2 + d];
+                    }
+                    pb[q][0] = transpose8(StoreT<__half>::pack2(e_[0] * v_sc[0], e_[1] * v_sc[0]));
+                    pb[q][1] = transpose8(StoreT<__half>::pack2(e_[2] * v_sc[1], e_[3] * v_sc[1]));
+                }
+                // O^T += V^T P^T
+                // (operand row index 2 t + x of a half is key key_of(2 t + x) = t + 4 x)
+                uint32_t w[4][4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t row = t + 4 * (e & 1) + 8 * (e >> 1);
+                    const uint4 v4 = *reinterpret_cast<const uint4*>(blk_p + kBlkBytes + row * 128 + (((uint32_t)key_of(g) ^ (row & 7)) << 4));
+                    w[e][0] = q8::code_word<F>(v4.x);
+                    w[e][1] = q8::code_word<F>(v4.y);
+                    w[e][2] = q8::code_word<F>(v4.z);
+                    w[e][3] = q8::code_word<F>(v4.w);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    // dims 2 j and 2 j + 1 of the lane's 16: the two keys' bytes side by side
+                    const uint32_t lo = __byte_perm(w[0][j >> 1], w[1][j >> 1], (j & 1) ? 0x7362 : 0x5140);
+                    const uint32_t hi = __byte_perm(w[2][j >> 1], w[3][j >> 1], (j & 1) ? 0x7362 : 0x5140);
+                    const uint32_t a0 = q8::code_pair<F, kAnyCode>(lo, false), a1 = q8::code_pair<F, kAnyCode>(lo, true);
+                    const uint32_t a2 = q8::code_pair<F, kAnyCode>(hi, false), a3 = q8::code_pair<F, kAnyCode>(hi, true);
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q) mma16816(o[q][j], a0, a1, a2, a3, pb[q][0], pb[q][1]);
+                }
+                __syncwarp();
             }
+            // after a timeout only: nothing may land in shared memory any more
+            for (; it < issued; ++it) mbar_wait_drain_bounded(bars + 8 * (it % kDepth), (it / kDepth) & 1);
+        };
+        walk(std::false_type{});
+        if constexpr (F == q8::kE4m3) {
+            // The codes 0x7f and 0xff come out of the conversion as NaN, and 0 * NaN also reaches rows that do not
+            // see them: where any row of the item is NaN, it runs again with the conversion that takes every code
+            // for a number. (That conversion for all items: 12 rows over 16896 keys 35.6 us, and 31.4; 8 streams
+            // of 48 rows together, 4608 shared + 2304 own keys, 84.6 and 75.4.)
+            float sum = 0.f;
 #pragma unroll
             for (int q = 0; q < NQ; ++q)
 #pragma unroll
-                for (int d = 0; d < 2; ++d)
-                    grow = grow || fmaxf(s[q][d] + v_log[0], s[q][2 + d] + v_log[1]) > m_run[q][d] + 8.f;
-            // the running maxima move only where a weight passes one by more than 2^8 (P stays below that)
-            if (__any_sync(0xffffffffu, grow)) {
+                for (int e = 0; e < 2; ++e) {
+                    sum = fmaf(l_run[q][e], 0.f, sum);
 #pragma unroll
-                for (int q = 0; q < NQ; ++q)
-#pragma unroll
-                    for (int d = 0; d < 2; ++d) {
-                        float x = fmaxf(s[q][d] + v_log[0], s[q][2 + d] + v_log[1]);
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                        const float mn = fmaxf(m_run[q][d], x);
-                        const float al = mn == m_run[q][d] ? 1.f : ex2_approx(m_run[q][d] - mn);
-                        m_run[q][d] = mn;
-                        l_run[q][d] *= al;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            o[q][j][d] *= al;
-                            o[q][j][2 + d] *= al;
-                        }
-                    }
-            }
-            uint32_t pb[NQ][2];
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                float e_[4];
-#pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    const float mu = m_run[q][d] == -INFINITY ? 0.f : m_run[q][d];
-                    e_[d] = ex2_approx(s[q][d] - mu);
-                    e_[2 + d] = ex2_approx(s[q][2 + d] - mu);
-                    l_run[q][d] += e_[d] + e_[2 + d];
+                    for (int j = 0; j < 8; ++j) sum = fmaf(o[q][j][e], 0.f, fmaf(o[q][j][2 + e], 0.f, sum));
                 }
-                pb[q][0] = transpose8(StoreT<__half>::pack2(e_[0] * v_sc[0], e_[1] * v_sc[0]));
-                pb[q][1] = transpose8(StoreT<__half>::pack2(e_[2] * v_sc[1], e_[3] * v_sc[1]));
+            if (__syncthreads_or(sum != sum) && !abort) {
+                begin_walk();
+                walk(std::true_type{});
             }
-            // O^T += V^T P^T
-            // (operand row index 2 t + x of a half is key key_of(2 t + x) = t + 4 x)
-            uint32_t w[4][4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t row = t + 4 * (e & 1) + 8 * (e >> 1);
-                const uint4 v4 = *reinterpret_cast<const uint4*>(blk_p + kBlkBytes + row * 128 + (((uint32_t)key_of(g) ^ (row & 7)) << 4));
-                w[e][0] = q8::code_word<F>(v4.x);
-                w[e][1] = q8::code_word<F>(v4.y);
-                w[e][2] = q8::code_word<F>(v4.z);
-                w[e][3] = q8::code_word<F>(v4.w);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                // dims 2 j and 2 j + 1 of the lane's 16: the two keys' bytes side by side
-                const uint32_t lo = __byte_perm(w[0][j >> 1], w[1][j >> 1], (j & 1) ? 0x7362 : 0x5140);
-                const uint32_t hi = __byte_perm(w[2][j >> 1], w[3][j >> 1], (j & 1) ? 0x7362 : 0x5140);
-                const uint32_t a0 = q8::code_pair<F>(lo, false), a1 = q8::code_pair<F>(lo, true);
-                const uint32_t a2 = q8::code_pair<F>(hi, false), a3 = q8::code_pair<F>(hi, true);
-#pragma unroll
-                for (int q = 0; q < NQ; ++q) mma16816(o[q][j], a0, a1, a2, a3, pb[q][0], pb[q][1]);
-            }
-            __syncwarp();
         }
-        // after a timeout only: nothing may land in shared memory any more
-        for (; it < issued; ++it) mbar_wait_drain_bounded(bars + 8 * (it % kDepth), (it / kDepth) & 1);
         __syncthreads();
         if (abort) return;
         // ---- the warps' results meet: position 8 d + g of a row is d of lane g's 16 dims (tile j holds

@@ -133,7 +133,9 @@ template <> __device__ __forceinline__ uint32_t mul2<__half>(uint32_t a, uint32_
 //   e4m3 -> bf16: the same gives the value times 2^-120; products of bf16 keep subnormal operands, so
 //     a multiplication by 2^120 restores it. Where s < 2^7, as for every vector of magnitude below
 //     57344, the scale's multiplier holds the 2^120 (SmallScaleDecoder).
-// The e4m3 NaN codes, which the write never produces, are not told apart from +-480.
+// The codes 0x7f and 0xff, NaN in other uses of e4m3, which the write never produces, are +-480: a cache
+// may hold rows that nobody wrote, and a code that decodes to NaN would reach the rows that do not see it
+// (0 * NaN).
 template <typename T, int F> struct Decoder;
 
 // word(): prepares four codes, once; pair(): two of them as values.
@@ -166,9 +168,12 @@ template <> struct Decoder<__half, kE4m3> {
     __half2 s;
     __device__ __forceinline__ void scale(uint32_t s2) { s = __hmul2(as_h(s2), as_h(0x5c005c00u)); }   // * 2^8: s <= 146.125
     static __device__ __forceinline__ uint32_t word(uint32_t w) { return w; }
-    __device__ __forceinline__ uint32_t pair(uint32_t w, int a, int b) const {
+    static __device__ __forceinline__ uint32_t fields(uint32_t w, int a, int b) {
         const uint32_t u = __byte_perm(w, 0u, (uint32_t)(a | (a << 4) | (b << 8) | (b << 12)));
-        return bits(__hmul2(as_h(((u << 7) & 0x3f803f80u) | (u & 0x80008000u)), s));
+        return ((u << 7) & 0x3f803f80u) | (u & 0x80008000u);
+    }
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int a, int b) const {
+        return bits(__hmul2(as_h(fields(w, a, b)), s));
     }
 };
 template <> struct Decoder<__nv_bfloat16, kE4m3> {
@@ -201,11 +206,14 @@ template <> struct TileDecoder<__nv_bfloat16, kE4m3> {
 };
 
 // Codes alone as a pair of f16, which holds every code exactly. word: four codes prepared by code_word;
-// upper: its codes 2 and 3, not 0 and 1. e4m3 has an instruction for it.
+// upper: its codes 2 and 3, not 0 and 1. e4m3 has an instruction for it, which makes 0x7f and 0xff NaN;
+// kAnyCode: +-480, in five instructions.
 template <int F> __device__ __forceinline__ uint32_t code_word(uint32_t w) { return F == kInt8 ? w ^ 0x80808080u : w; }
-template <int F> __device__ __forceinline__ uint32_t code_pair(uint32_t w, bool upper) {
+template <int F, bool kAnyCode> __device__ __forceinline__ uint32_t code_pair(uint32_t w, bool upper) {
     if constexpr (F == kInt8) {
         return bits(__hsub2(as_h(__byte_perm(w, 0x64646464u, upper ? 0x4342 : 0x4140)), as_h(0x64806480u)));
+    } else if constexpr (kAnyCode) {
+        return bits(__hmul2(as_h(Decoder<__half, kE4m3>::fields(w, upper ? 2 : 0, upper ? 3 : 1)), as_h(0x5c005c00u)));
     } else {
         uint32_t r;
         asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(upper ? w >> 16 : w));

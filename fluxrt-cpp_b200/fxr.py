@@ -801,7 +801,8 @@ def _groups(t, rows: int, what: str):
 class CacheQ8:
     """An 8-bit K/V cache (fxr_q8_cache). k, v: codes [n_rows, >= heads * 128], int8 or float8_e4m3fn;
     k_scale, v_scale: [heads, ld_scale >= n_rows, a multiple of 8] of the frame's 16-bit type. The
-    tensors are the caller's; the object keeps references to them."""
+    tensors are the caller's; the object keeps references to them. Unlike torch, the cache has no NaN
+    codes: the bytes 0x7f and 0xff of float8_e4m3fn count as 480 and -480 (a NaN scale marks a NaN vector)."""
 
     def __init__(self, k, v, k_scale, v_scale):
         import torch

@@ -1,0 +1,159 @@
+"""The 8-bit spatial cache at the edges of what its tensors may hold: e4m3 codes that other uses call NaN, scales next to
+the largest, scores in the hundreds, NaN that comes late. Attention is held against K as the kernel holds it, so that its
+rounding to T (many rows) drops out of the bars, which then are tight; derived before the first run, u = finfo(T).eps / 2:
+  a score's 128 products are summed in 32 bits, at worst with 128 truncations of 2^-23 of a partial sum that is at most
+  sum|q k|, and a few roundings of 2^-24 of the score follow: ds = (2^-16 + 2^-21) * scale * max_j sum|q k_j|, also where
+  bf16 queries are held in f16 (elements below 2^-24 of the largest round to a step of 2^-35 of it, 128 of them: 2^-28);
+  P and V are rounded to T (u each at most), exponentials to 2^-13, the output once:
+      |err| <= u |o| + (2 u + 2^-13 + expm1(2 ds)) sum(w |v|)
+"""
+import math
+
+import pytest
+import torch
+
+import fxr
+from test_q8_cache import D, TDT, cfg_of, filled_cache, randn, rng_of, stream_of, sync_ok, workspace_for
+
+FEW = 32        # rows that the kernel for few rows takes; it holds K and V exactly
+
+
+def e4m3_values():
+    """The 256 codes as numbers; 0x7f and 0xff are +-480."""
+    b = torch.arange(256, device="cuda")
+    e, m = (b >> 3) & 15, (b & 7).double()
+    x = torch.where(e == 0, m / 8 * 2.0 ** -6, (1 + m / 8) * torch.exp2(e.double() - 7))
+    return torch.where(b >= 128, -x, x)
+
+
+def held(cache, n, exact):
+    """K and V [n, heads, 128] in 64 bits as the attention holds them: codes times scales, exactly or rounded to T and
+    finite. Keys without a valid scale: K NaN."""
+    h, t = cache.n_heads, cache.k_scale.dtype
+    out, bad = [], None
+    for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        codes = c[:n, :h * D].contiguous().view(torch.int8)
+        x = codes.double() if c.dtype == torch.int8 else e4m3_values()[codes.view(torch.uint8).long()]
+        s = s[:h, :n].t().double()
+        cap = 1.9921875 * 2.0 ** 120 if t == torch.bfloat16 else 511.75
+        if c.dtype != torch.int8:
+            cap = 1.1328125 * 2.0 ** 119 if t == torch.bfloat16 else 146.125
+        invalid = ~(s.abs() <= cap)
+        bad = invalid if bad is None else bad | invalid
+        x = x.view(n, h, D) * torch.where(invalid, torch.zeros_like(s), s)[..., None]
+        out.append(x if exact else x.to(t).double().clamp(-torch.finfo(t).max, torch.finfo(t).max))
+    out[0] = torch.where(bad[..., None], torch.full_like(out[0], math.nan), out[0])
+    return out
+
+
+def check(cfg, st, max_rows, prefix=None, prefix_groups=None, what="", rows=None, telling=0.7):
+    """The stream's output against the definition (of the compact rows `rows`). telling: the share of elements whose bar
+    is below their value, so that an output of zeros would fail."""
+    n, m, h, t = cfg.n_tokens, st["m"], cfg.n_heads, TDT[cfg.dtype]
+    u = torch.finfo(t).eps / 2
+    exact = 0 < max_rows <= FEW
+    k, v = held(st["cache"], n, exact)
+    ones = lambda r: torch.full((r,), -1, dtype=torch.int32, device="cuda")  # noqa: E731
+    kg = st.get("k_groups") if st.get("k_groups") is not None else ones(n)
+    if prefix is not None:
+        pk, pv = held(prefix, prefix.n_rows, exact)
+        k, v = torch.cat([pk, k]), torch.cat([pv, v])
+        kg = torch.cat([prefix_groups if prefix_groups is not None else ones(prefix.n_rows), kg])
+    at = st["idx"][:m].long()
+    qg = st["q_groups"][at] if st.get("q_groups") is not None else ones(m)
+    seen = (qg[:, None] & kg[None]) != 0
+    scale = cfg.softmax_scale if cfg.softmax_scale > 0 else 1 / math.sqrt(D)
+    q = st["qc"][:m].double().view(m, h, D).transpose(0, 1)
+    k, v = k.transpose(0, 1), v.transpose(0, 1)
+    s = (q @ k.transpose(1, 2) * scale).masked_fill(~seen[None], -math.inf)
+    nan = torch.isnan(s).any(-1)
+    s = torch.nan_to_num(s, nan=-math.inf, neginf=-math.inf)
+    w = torch.nan_to_num(torch.softmax(s, -1), nan=0.0)              # rows that see nothing: zeros
+    o, mean_abs = w @ v, w @ v.abs()
+    ds = (q.abs() @ torch.nan_to_num(k).abs().transpose(1, 2) * scale).masked_fill(~seen[None], 0).amax(-1, keepdim=True)
+    bar = u * o.abs() + (2 * u + 2 ** -13 + torch.expm1(2 * (2 ** -16 + 2 ** -21) * ds)) * mean_abs
+    bar = bar + torch.finfo(t).smallest_normal * torch.finfo(t).eps
+    got = st["out"][at].double().view(m, h, D).transpose(0, 1)
+    if rows is not None:
+        got, o, bar, nan = got[:, rows], o[:, rows], bar[:, rows], nan[:, rows]
+    assert torch.equal(torch.isnan(got), nan[..., None].expand_as(got)), what + ": NaN in other places"
+    err = torch.where(nan[..., None], torch.zeros_like(o), (got - o).abs())
+    assert (err <= bar).all(), f"{what}: {float((err / bar).max()):.2f} of the bar"
+    told = (bar < o.abs()) | nan[..., None] | (o == 0)
+    assert float(told.double().mean()) >= telling, f"{what}: the bar tells {float(told.double().mean()):.2f}"
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[at] = False
+    assert (st["out"][rest] == 7.0).all(), what + ": rows that are not listed changed"
+
+
+def attend(cfg, st, max_rows, prefix=None, prefix_groups=None):
+    fxr.attention_q8(cfg, [st], workspace_for(cfg, [st], prefix, max_rows), prefix=prefix, prefix_groups=prefix_groups,
+                     max_rows=max_rows)
+    sync_ok()
+
+
+def fill_codes(cache, rows, *codes):
+    """The rows' K and V codes: `codes` in turn along the columns."""
+    for c in (cache.k, cache.v):
+        c = c.view(torch.uint8)
+        c[rows] = torch.tensor(codes, dtype=torch.uint8, device="cuda").repeat(c.shape[1] // len(codes))
+
+
+# ---- e4m3 codes that other uses call NaN -----------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("m", [3, 12, 30, 300])
+@pytest.mark.parametrize("scales", ["valid", "invalid"])
+@pytest.mark.parametrize("prefix", [0, 200])
+def test_rows_that_nobody_sees_hold_any_code(cuda, dtype, m, scales, prefix):
+    """Padding rows of codes 0x7f and 0xff, in the prefix and among the own, and a key of such codes that every other row
+    sees: the others must not notice, and those count them as +-480."""
+    n, heads = 333, 2
+    g = rng_of(m)
+    cfg = cfg_of(n, heads, dtype)
+    st = stream_of(g, cfg, m)
+    st["cache"] = c = filled_cache(g, cfg, n, "e4m3")
+    at = torch.arange(n, device="cuda")
+    st["q_groups"] = torch.where(at % 2 == 0, 1, 3).int()
+    st["k_groups"] = torch.full((n,), 1, dtype=torch.int32, device="cuda")
+    st["k_groups"][100:140] = 0
+    st["k_groups"][n - 1] = 0
+    st["k_groups"][7] = 2
+    hidden = st["k_groups"] == 0
+    fill_codes(c, hidden, 0x7f, 0xff)
+    fill_codes(c, at == 7, 0xff, 0x7f, 0x38, 0x7f)
+    c.k_scale[:, 7] = 2.0 ** -9        # K of about 1
+    pre = pg = None
+    if prefix:
+        pre = filled_cache(g, cfg, prefix, "e4m3")
+        pg = torch.full((prefix,), 1, dtype=torch.int32, device="cuda")
+        pg[prefix - 37:] = 0
+        fill_codes(pre, pg == 0, 0xff, 0x7f)
+    if scales == "invalid":
+        for s in (c.k_scale, c.v_scale):
+            s[:, :n][:, hidden] = math.nan
+        if prefix:
+            pre.v_scale[:, :prefix][:, pg == 0] = math.inf
+    attend(cfg, st, m, pre, pg)
+    check(cfg, st, m, pre, pg)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n, heads, m", [(90, 3, 5), (400, 2, 200), (2400, 32, 1950)])
+def test_every_code_counts_as_one_number(cuda, dtype, n, heads, m):
+    """Visible codes 0x7f and 0xff are +-480 in the read-back and in the attention of few, many and very many rows."""
+    g = rng_of(n)
+    cfg = cfg_of(n, heads, dtype)
+    st = stream_of(g, cfg, m)
+    st["cache"] = c = filled_cache(g, cfg, n, "e4m3")
+    fill_codes(c, torch.arange(n, device="cuda") % 11 == 3, 0x7f, 0x30, 0xff, 0xb8)
+    for s in (c.k_scale, c.v_scale):
+        s[:, 3:n:11] = 2.0 ** -9
+    attend(cfg, st, m)
+    check(cfg, st, m)
+    k, v = (torch.zeros(n, heads * D, dtype=TDT[dtype], device="cuda") for _ in range(2))
+    fxr.cache_read_q8(cfg, c, k, v)
+    sync_ok()
+    for got, want in zip((k, v), held(c, n, True)):
+        assert torch.equal(got, want.reshape(n, -1).to(TDT[dtype]))
