@@ -1364,12 +1364,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
                             store(c, lo, hi);
                         }
                     };
-                    if constexpr (q8::TileDecoder<T, F>::has_limit) {
-                        using Fast = typename q8::TileDecoder<T, F>::type;
-                        if (!__any_sync(0xffffffffu, f >= Fast::limit)) convert(Fast{});
-                        else convert(q8::Decoder<T, F>{});
+                    using Dec = q8::TileDecoder<T, F>;
+                    if constexpr (Dec::has_limit) {
+                        if (!__any_sync(0xffffffffu, fabsf(f) >= Dec::limit)) convert(typename Dec::small{});
+                        else convert(typename Dec::any{});
                     } else {
-                        convert(q8::Decoder<T, F>{});
+                        convert(typename Dec::any{});
                     }
                     raw_done();
                     fence_async_smem();      // the tensor core reads the tile through the async proxy

@@ -188,7 +188,7 @@ template <> struct Decoder<__nv_bfloat16, kE4m3> {
         return bits(__hmul2(__hmul2(as_bf(fields(w, a, b)), as_bf(0x7b807b80u)), s));
     }
 };
-// e4m3 -> bf16 for scales below `limit` (or NaN): one multiplication.
+// e4m3 -> bf16 for scales of magnitude below `limit` (or NaN): one multiplication.
 struct SmallScaleDecoder {
     static constexpr float limit = 128.f;
     __nv_bfloat162 s;
@@ -198,11 +198,37 @@ struct SmallScaleDecoder {
         return bits(__hmul2(as_bf(Decoder<__nv_bfloat16, kE4m3>::fields(w, a, b)), s));
     }
 };
-// The decoder for a tile whose scales are all below its limit; Decoder serves the others.
-template <typename T, int F> struct TileDecoder { static constexpr bool has_limit = false; };
+// The largest valid scales times 480 pass the largest T. In the attention such a product stops there (a NaN
+// stays one), since an infinite V row would turn a weight of 0 into NaN.
+template <typename T> __device__ __forceinline__ uint32_t to_finite2(uint32_t x);
+template <> __device__ __forceinline__ uint32_t to_finite2<__nv_bfloat16>(uint32_t x) {
+    return bits(__hmin2_nan(__hmax2_nan(as_bf(x), as_bf(0xff7fff7fu)), as_bf(0x7f7f7f7fu)));
+}
+template <> __device__ __forceinline__ uint32_t to_finite2<__half>(uint32_t x) {
+    return bits(__hmin2_nan(__hmax2_nan(as_h(x), as_h(0xfbfffbffu)), as_h(0x7bff7bffu)));
+}
+template <typename T> struct FiniteDecoder : Decoder<T, kE4m3> {
+    __device__ __forceinline__ uint32_t pair(uint32_t w, int a, int b) const {
+        return to_finite2<T>(Decoder<T, kE4m3>::pair(w, a, b));
+    }
+};
+// Decoders of the attention: `any` for every valid scale, and `small` for a tile whose scales are all of
+// magnitude below `limit` (or NaN).
+template <typename T, int F> struct TileDecoder {
+    static constexpr bool has_limit = false;
+    using any = Decoder<T, F>;
+};
 template <> struct TileDecoder<__nv_bfloat16, kE4m3> {
     static constexpr bool has_limit = true;
-    using type = SmallScaleDecoder;
+    static constexpr float limit = SmallScaleDecoder::limit;
+    using any = FiniteDecoder<__nv_bfloat16>;
+    using small = SmallScaleDecoder;
+};
+template <> struct TileDecoder<__half, kE4m3> {
+    static constexpr bool has_limit = true;
+    static constexpr float limit = 136.f;       // 480 * 136 = 65280
+    using any = FiniteDecoder<__half>;
+    using small = Decoder<__half, kE4m3>;
 };
 
 // Codes alone as a pair of f16, which holds every code exactly. word: four codes prepared by code_word;
@@ -544,7 +570,7 @@ __global__ void __launch_bounds__(kReadThreads) q8_expand_kernel(const __grid_co
         uint32_t sk = static_cast<const uint16_t*>(c.ks)[at], sv = static_cast<const uint16_t*>(c.vs)[at];
         const bool ok = valid_scale<T, F>(StoreT<T>::unpack2(sk).x) && valid_scale<T, F>(StoreT<T>::unpack2(sv).x);
         if (!ok) sk = 0;
-        Decoder<T, F> dk, dv;
+        typename TileDecoder<T, F>::any dk, dv;
         dk.scale(0x10001u * sk);
         dv.scale(0x10001u * sv);
         uint4 lo, hi;

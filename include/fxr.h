@@ -633,9 +633,10 @@ int32_t fxr_frame_forward_heads_nccl(const fxr_frame_desc* desc, const fxr_head_
  * A vector of zeros has scale 0. One that holds an infinity or NaN has
  * scale NaN and codes 0: it reads back as NaN, and an attention row that sees it is NaN. K' is
  * quantised from its 32-bit value. The e4m3 codes 0x7f and 0xff, NaN in other uses, which the write never
- * produces, count as 480 and -480 wherever a cache is read. A scale is at most (largest T) / 128 for int8 and (largest T) / 448
- * for e4m3, so that every finite vector reads back finite; codes saturate there. In the attention a
- * larger one counts as NaN. */
+ * produces, count as 480 and -480 wherever a cache is read (times a scale next to the largest that is past
+ * the largest T: read back as infinity, in the attention the largest T). A scale is at most (largest T) / 128
+ * for int8 and (largest T) / 448 for e4m3, so that every finite vector reads back finite; codes saturate
+ * there. In the attention a larger one counts as NaN. */
 typedef enum fxr_q8_format { FXR_Q8_INT8 = 0, FXR_Q8_E4M3 = 1 } fxr_q8_format;
 
 typedef struct fxr_q8_cache {

@@ -157,3 +157,44 @@ def test_every_code_counts_as_one_number(cuda, dtype, n, heads, m):
     sync_ok()
     for got, want in zip((k, v), held(c, n, True)):
         assert torch.equal(got, want.reshape(n, -1).to(TDT[dtype]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("m", [3, 30, 300])
+def test_codes_of_480_times_the_largest_scales(cuda, dtype, m):
+    """480 times a scale next to the largest valid one passes the largest T: rows that do not see such keys must not
+    notice. (f16: those that do see them too.)"""
+    n, heads = 333, 2
+    g = rng_of(m)
+    cfg = cfg_of(n, heads, dtype)
+    st = stream_of(g, cfg, m)
+    st["cache"] = c = filled_cache(g, cfg, n, "e4m3")
+    at = torch.arange(n, device="cuda")
+    st["q_groups"] = torch.where(at % 2 == 0, 1, 3).int()
+    st["k_groups"] = torch.where(at % 50 == 9, 2, 1).int()
+    st["k_groups"][200:230] = 0
+    odd = st["k_groups"] != 1
+    fill_codes(c, odd, 0x7f, 0xff)
+    top = 1.1328125 * 2.0 ** 119 if dtype == "bf16" else 146.125
+    for s in (c.k_scale, c.v_scale):
+        s[:, :n][:, odd] = top
+    if dtype == "f16":
+        c.k_scale[:, :n][:, st["k_groups"] == 2] = 2.0 ** -9
+    attend(cfg, st, m)
+    rows = st["idx"][:m].long() % 2 == 0 if dtype == "bf16" else None
+    check(cfg, st, m, rows=rows)
+
+
+@pytest.mark.gpu
+def test_codes_of_480_times_the_largest_scale_seen_by_very_many_rows(cuda):
+    """The form that expands the cache: such a V stops at the largest f16."""
+    n, heads, m = 2400, 32, 1950
+    g = rng_of(8)
+    cfg = cfg_of(n, heads, "f16")
+    st = stream_of(g, cfg, m)
+    st["cache"] = c = filled_cache(g, cfg, n, "e4m3")
+    fill_codes(c, torch.arange(n, device="cuda") == 77, 0x7f, 0xff)
+    c.k_scale[:, 77], c.v_scale[:, 77] = 2.0 ** -9, 146.125
+    attend(cfg, st, m)
+    check(cfg, st, m)
