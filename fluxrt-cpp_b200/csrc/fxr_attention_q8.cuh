@@ -1777,8 +1777,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tile_kernel(const __grid_cons
             if (!wwait(bar(kPVDone + t), (s_it - 1) & 1)) break;
             tc_fence_after();
             const bool blind = it->list != nullptr && *my_groups == 0;   // the row's set is empty
-            if (blind) m_run = -INFINITY;
-            if (m_run == -INFINITY) l_run = 0.f;      // the row saw nothing
+            if (blind) {
+                m_run = -INFINITY;
+                l_run = 0.f;
+            } else if (m_run == -INFINITY && l_run == l_run) {
+                l_run = 0.f;                          // the row saw nothing (a NaN stays the mark of a row that saw one)
+            }
             if (it->part != nullptr) {
                 cut_epilogue(it->part + t * kPartFloats, r, tO, m_run, l_run, blind, live, bar(kOFree + t));
             } else {

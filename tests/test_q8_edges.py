@@ -198,3 +198,27 @@ def test_codes_of_480_times_the_largest_scale_seen_by_very_many_rows(cuda):
     c.k_scale[:, 77], c.v_scale[:, 77] = 2.0 ** -9, 146.125
     attend(cfg, st, m)
     check(cfg, st, m)
+
+
+# ---- NaN ---------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, fmt", [("bf16", "int8"), ("f16", "e4m3")])
+@pytest.mark.parametrize("m", [5, 30, 250])
+@pytest.mark.parametrize("tiles, place", [(2, 1), (3, 1), (40, 39), (40, 20), (40, 0)])
+def test_a_nan_key_that_is_the_first_that_a_row_sees(cuda, dtype, fmt, m, tiles, place):
+    """Rows of one document see a single tile of 128 keys, shared with the others, and in it a key without a valid scale,
+    in each of the columns whose exponentials are computed in another way: NaN in its head, whole units and cut ones."""
+    n, heads = 128 * tiles, 9
+    g = rng_of(m + tiles)
+    cfg = cfg_of(n, heads, dtype)
+    st = stream_of(g, cfg, m)
+    st["cache"] = c = filled_cache(g, cfg, n, fmt)
+    at = torch.arange(n, device="cuda")
+    st["q_groups"] = torch.where(at % 2 == 0, 1, 2).int()
+    st["k_groups"] = torch.where(at // 128 == place, 3, 1).int()
+    for head in range(8):
+        (c.k_scale if head % 3 else c.v_scale)[head, 128 * place + 40 + head] = math.nan if head % 2 else math.inf
+    attend(cfg, st, m)
+    check(cfg, st, m)
+    out = st["out"][st["idx"][:m].long()].view(m, heads, D)
+    assert torch.isnan(out[:, :8]).all() and not torch.isnan(out[:, 8]).any()
