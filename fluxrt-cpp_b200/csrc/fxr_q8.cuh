@@ -483,7 +483,7 @@ struct ReadArgs {
     void* k;
     void* v;
     int64_t ld;
-    int32_t n_rows, n_heads;
+    int32_t n_rows, bound, n_heads;   // bound: rows that k and v hold, at most n_rows
 };
 
 constexpr int kReadThreads = 256;
@@ -493,7 +493,8 @@ template <typename T, int F>
 __global__ void __launch_bounds__(kReadThreads) q8_read_kernel(const __grid_constant__ ReadArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    const int32_t m_all = min(a.count ? *a.count : a.host_count, a.n_rows);
+    const int32_t asked = min(a.count ? *a.count : a.host_count, a.n_rows), m_all = min(asked, a.bound);
+    if (asked > a.bound && blockIdx.x == 0 && threadIdx.x == 0) atomicOr(&g_error_word, kErrBounds);
     const uint32_t per_row = (uint32_t)a.n_heads * (kHeadDim / 16);   // 16-code chunks of a row
     const int64_t total = (int64_t)m_all * per_row;
     const bool small = total <= 0xffffffffll;         // 32-bit divisions

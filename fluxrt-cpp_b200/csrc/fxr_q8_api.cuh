@@ -433,8 +433,9 @@ int32_t fxr_cache_read_q8(const fxr_frame_desc* desc, const fxr_q8_cache* cache,
     if (!aligned16(k) || !aligned16(v)) return fail(FXR_ERR_INVALID, "k/v must be 16-byte aligned");
     if (ld < (int64_t)desc->n_heads * desc->head_dim || (ld % 8))
         return fail(FXR_ERR_INVALID, "ld must be a multiple of 8, >= n_heads*head_dim");
-    fxr::q8::ReadArgs a{q8_arg(cache), idx, count, host_count, k, v, ld, cache->n_rows, desc->n_heads};
-    const int64_t units = (int64_t)(count ? cache->n_rows : host_count) * desc->n_heads * (fxr::kHeadDim / 16);
+    const int32_t bound = host_count > 0 ? std::min(host_count, cache->n_rows) : cache->n_rows;
+    fxr::q8::ReadArgs a{q8_arg(cache), idx, count, host_count, k, v, ld, cache->n_rows, bound, desc->n_heads};
+    const int64_t units = (int64_t)bound * desc->n_heads * (fxr::kHeadDim / 16);
     // CTAs per SM at most: short ones that the hardware balances for a whole cache (16896 rows: 58 us
     // against 67 us with 16), fewer where most may find nothing to do (1153 of 4608 rows: 6.3 against 6.8)
     const int64_t ctas = (units + fxr::q8::kReadThreads - 1) / fxr::q8::kReadThreads, sms = sm_count();

@@ -871,13 +871,36 @@ def cache_write_q8(cfg: FrameConfig, cache_k, cache_v, cache: CacheQ8, idx=None,
                                      cache.ref, _raw_stream(cache.device, stream, cache_k, cache_v, idx, count)))
 
 
+def _check_rows(t, rows: int, cols: int, dtype, what: str):
+    """Refuses a tensor that does not hold `rows` rows of `cols` adjacent elements of `dtype`."""
+    if t is None:
+        _refuse(f"{what}: null pointer")
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 2:
+        whole = shape[1] >= cols and (stride[1] == 1 or cols == 1)
+    else:                                   # rows of several dimensions
+        whole = len(shape) > 2 and (shape[0] == 0 or (t[0].is_contiguous() and t[0].numel() >= cols))
+    if t.dtype is not dtype or shape[0] < rows or not whole:
+        _refuse(f"{what}: {rows} rows of {cols} adjacent elements of {dtype} needed, got {tuple(shape)} of {t.dtype}, "
+                f"strides {stride}")
+
+
 def cache_read_q8(cfg: FrameConfig, cache: CacheQ8, k, v, idx=None, count=None, host_count: int = -1, stream=None):
-    """Cache rows back in the frame's type: k[m], v[m] = row idx[m], or by default every row of the cache."""
+    """Cache rows back in the frame's type: k[m], v[m] = row idx[m], or by default every row of the cache. With a
+    device count, rows that k and v do not hold are not written (FXR_ERR_BOUNDS from check_device_error)."""
     cache.check(cfg, 0)
+    if count is None and idx is None and host_count < 0:
+        host_count = cache.n_rows
+    rows = 0 if count is not None else host_count
+    cols, dtype = cfg.n_heads * cfg.head_dim, cache.k_scale.dtype
+    _check_rows(k, rows, cols, dtype, "k")
+    _check_rows(v, rows, cols, dtype, "v")
     if k.stride() != v.stride():
         _refuse("k and v: one row stride")
-    if idx is None and count is None and host_count < 0:
-        host_count = cache.n_rows
+    if count is not None:
+        host_count = min(k.shape[0], v.shape[0])
+    elif idx is not None and idx.numel() < host_count:
+        _refuse(f"idx: {idx.numel()} entries, host_count is {host_count}")
     _check(load().fxr_cache_read_q8(cfg.ref(), cache.ref, _ptr(idx), _ptr(count), host_count, k.data_ptr(),
                                     v.data_ptr(), k.stride(0), _raw_stream(cache.device, stream, k, v, idx, count)))
 

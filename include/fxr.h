@@ -672,7 +672,9 @@ int32_t fxr_cache_write_q8(const fxr_frame_desc* desc, const void* cache_k, cons
 
 /* Cache rows back in T: row m of k and v (stride ld elements) = cache row idx[m], or row m when idx is
  * NULL, for m < *count (or host_count when count is NULL; at most cache->n_rows). An index outside
- * [0, n_rows) is skipped and reported, its output row left untouched. */
+ * [0, n_rows) is skipped and reported, its output row left untouched. With a device count, a host_count > 0
+ * is the number of rows that k and v hold: rows past it are not written and set the device error word
+ * (FXR_ERR_BOUNDS); <= 0: the caller knows that they hold *count rows. */
 int32_t fxr_cache_read_q8(const fxr_frame_desc* desc, const fxr_q8_cache* cache, const int32_t* idx, const int32_t* count,
                           int32_t host_count, void* k, void* v, int64_t ld, void* stream);
 

@@ -222,3 +222,53 @@ def test_a_nan_key_that_is_the_first_that_a_row_sees(cuda, dtype, fmt, m, tiles,
     check(cfg, st, m)
     out = st["out"][st["idx"][:m].long()].view(m, heads, D)
     assert torch.isnan(out[:, :8]).all() and not torch.isnan(out[:, 8]).any()
+
+
+# ---- refusals (no GPU) and what a call may write ---------------------------------------------------
+def cpu_cache(rows, heads=2, fmt=torch.int8, dtype=torch.bfloat16):
+    k = torch.zeros(rows, heads * D, dtype=torch.int8).view(fmt)
+    s = torch.zeros(heads, max(8, -(-rows // 8) * 8), dtype=dtype)
+    return fxr.CacheQ8(k, k.clone(), s, s.clone())
+
+
+def test_read_back_refuses_outputs_that_do_not_hold_the_rows():
+    cfg, cache = cfg_of(16, 2, "bf16"), cpu_cache(19)          # a cache may have more rows than the frame
+    out = lambda rows, cols=2 * D, t=torch.bfloat16: torch.zeros(rows, cols, dtype=t)  # noqa: E731
+    idx = torch.zeros(5, dtype=torch.int32)
+    for k, v, more in ((out(16), out(16), {}), (out(19), out(18), {}), (out(18), out(19), {}), (out(6), out(6), {"host_count": 7}),
+                       (out(19, D), out(19, D), {}), (out(19, t=torch.float16), out(19, t=torch.float16), {}),
+                       (out(19, t=torch.float32), out(19, t=torch.float32), {}), (out(19, t=torch.int8), out(19, t=torch.int8), {}),
+                       (out(2 * D, 19).t(), out(2 * D, 19).t(), {}), (out(19), None, {}), (None, out(19), {}),
+                       (out(19).view(19, 4, 64)[:, :, :32], out(19).view(19, 4, 64)[:, :, :32], {}),
+                       (out(19).flatten(), out(19).flatten(), {}), (out(9), out(9), {"idx": idx, "host_count": 9})):
+        with pytest.raises(fxr.FxrError) as e:
+            fxr.cache_read_q8(cfg, cache, k, v, **more)
+        assert e.value.status == fxr.FXR_ERR_INVALID and "one row stride" not in str(e.value) and "the cache is on" not in str(e.value)
+    # what holds the rows passes on to the device's check
+    for k, more in ((out(19), {}), (out(30, 3 * D)[:, :2 * D], {}), (out(19).view(19, 2, D), {}), (out(7), {"host_count": 7}),
+                    (out(3), {"count": idx[:1]}), (out(5), {"idx": idx, "host_count": 5})):
+        with pytest.raises(fxr.FxrError, match="the cache is on"):
+            fxr.cache_read_q8(cfg, cache, k, k, **more)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("listed", [False, True])
+@pytest.mark.parametrize("rows, asked", [(5, 8), (8, 8), (9, 8), (1, 40), (5, 1000)])
+def test_read_back_with_a_device_count_stays_in_its_outputs(cuda, listed, rows, asked):
+    n, heads = 40, 2
+    g = rng_of(rows)
+    cfg = cfg_of(n, heads, "bf16")
+    cache = filled_cache(g, cfg, n, "int8")
+    store = [torch.full((n + 1, heads * D), 5.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    idx = torch.randperm(n, generator=g, device="cuda").int() if listed else None
+    fxr.cache_read_q8(cfg, cache, store[0][:rows], store[1][:rows], idx=idx,
+                      count=torch.tensor([asked], dtype=torch.int32, device="cuda"))
+    if min(asked, n) > rows:
+        with pytest.raises(fxr.FxrError) as e:
+            fxr.check_device_error()
+        assert e.value.status == fxr.FXR_ERR_BOUNDS
+    sync_ok()
+    at = idx.long() if listed else torch.arange(n, device="cuda")
+    written = min(rows, asked, n)
+    for a, want in zip(store, held(cache, n, True)):
+        assert torch.equal(a[:written], want.reshape(n, -1)[at[:written]].bfloat16()) and (a[written:] == 5).all()
