@@ -860,6 +860,16 @@ def gather_norm_rope_q8(cfg: FrameConfig, q, k, v, mask, idx, count, pos, norm_q
                                                       norm_k, qc, save)))
 
 
+def _check_extent(t, rows: int, ld: int, cols: int, dtype, what: str):
+    """Refuses a tensor of another type, or one that ends before `rows` rows of `cols` elements, `ld` apart."""
+    if t is None or rows <= 0:
+        return
+    held = t.numel() if t.is_contiguous() else 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    if t.dtype is not dtype or held < (rows - 1) * ld + cols:
+        _refuse(f"{what}: {rows} rows of {cols} elements of {dtype}, {ld} apart, needed: got {tuple(t.shape)} of {t.dtype}, "
+                f"strides {t.stride()}")
+
+
 def cache_write_q8(cfg: FrameConfig, cache_k, cache_v, cache: CacheQ8, idx=None, count=None, host_count: int = -1,
                    stream=None):
     """Rows of a 16-bit cache (row stride cfg.ld_cache) into an 8-bit one, listed by idx / count or, by
@@ -867,6 +877,12 @@ def cache_write_q8(cfg: FrameConfig, cache_k, cache_v, cache: CacheQ8, idx=None,
     cache.check(cfg, cfg.n_tokens)
     if idx is None and count is None and host_count < 0:
         host_count = cfg.n_tokens
+    # without a list the rows are the first ones; a listed row may be any of the frame's
+    rows, cols = host_count if idx is None and count is None else cfg.n_tokens, cfg.n_heads * cfg.head_dim
+    _check_extent(cache_k, rows, cfg.ld_cache or cols, cols, cache.k_scale.dtype, "cache_k")
+    _check_extent(cache_v, rows, cfg.ld_cache or cols, cols, cache.k_scale.dtype, "cache_v")
+    if idx is not None and count is None and idx.numel() < host_count:
+        _refuse(f"idx: {idx.numel()} entries, host_count is {host_count}")
     _check(load().fxr_cache_write_q8(cfg.ref(), _ptr(cache_k), _ptr(cache_v), _ptr(idx), _ptr(count), host_count,
                                      cache.ref, _raw_stream(cache.device, stream, cache_k, cache_v, idx, count)))
 

@@ -272,3 +272,24 @@ def test_read_back_with_a_device_count_stays_in_its_outputs(cuda, listed, rows, 
     written = min(rows, asked, n)
     for a, want in zip(store, held(cache, n, True)):
         assert torch.equal(a[:written], want.reshape(n, -1)[at[:written]].bfloat16()) and (a[written:] == 5).all()
+
+
+def test_write_refuses_sources_that_do_not_hold_the_rows():
+    cfg, cache = cfg_of(16, 2, "bf16"), cpu_cache(19)
+    wide = cfg_of(16, 2, "bf16", ld_cache=3 * D)
+    src = lambda rows, cols=2 * D, t=torch.bfloat16: torch.zeros(rows, cols, dtype=t)  # noqa: E731
+    idx = torch.zeros(5, dtype=torch.int32)
+    for c, k, v, more in ((cfg, src(15), src(16), {}), (cfg, src(16), src(15), {}), (cfg, src(6), src(6), {"host_count": 7}),
+                          (cfg, src(16, D), src(16, D), {}), (cfg, src(16, t=torch.float16), src(16, t=torch.float16), {}),
+                          (cfg, src(16, t=torch.float32), src(16), {}), (cfg, src(16), src(16, t=torch.int8), {}),
+                          (cfg, src(15), src(15), {"idx": idx, "host_count": 5}), (cfg, src(15), src(15), {"idx": idx, "count": idx[:1]}),
+                          (cfg, src(15), src(15), {"count": idx[:1]}), (wide, src(16), src(16), {}), (wide, src(15, 3 * D), src(16, 3 * D), {}),
+                          (cfg, src(16), src(16), {"idx": idx, "host_count": 6})):
+        with pytest.raises(fxr.FxrError) as e:
+            fxr.cache_write_q8(c, k, v, cache, **more)
+        assert e.value.status == fxr.FXR_ERR_INVALID and "the cache is on" not in str(e.value)
+    for c, k, more in ((cfg, src(16), {}), (cfg, src(17), {}), (cfg, src(16).view(16, 2, D), {}), (cfg, src(32, D), {}),
+                       (cfg, src(7), {"host_count": 7}), (cfg, src(16).flatten(), {"idx": idx, "count": idx[:1]}),
+                       (wide, src(16, 3 * D)[:, :2 * D], {}), (wide, src(16, 4 * D)[:, :2 * D], {}), (cfg, src(16), {"idx": idx, "host_count": 5})):
+        with pytest.raises(fxr.FxrError, match="the cache is on"):
+            fxr.cache_write_q8(c, k, k, cache, **more)
