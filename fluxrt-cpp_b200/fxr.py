@@ -792,6 +792,14 @@ def _device_of(*tensors):
     return next(iter(at)).index
 
 
+def _words(*tensors):
+    """Refuses lists, counts and masks (None entries apart) that are not 32-bit words: others were read as such."""
+    import torch
+    for t in tensors:
+        if t is not None and t.dtype is not torch.int32 and t.dtype is not torch.uint32:
+            _refuse(f"idx, count, mask and pos are 32-bit words: got {t.dtype}")
+
+
 def _groups(t, rows: int, what: str):
     import torch
     if t is not None and (t.dtype not in (torch.int32, torch.uint32) or not t.is_contiguous() or t.numel() < rows):
@@ -853,6 +861,7 @@ def gather_norm_rope_q8(cfg: FrameConfig, q, k, v, mask, idx, count, pos, norm_q
                         save=None, stream=None):
     """gather_norm_rope into an 8-bit cache (fxr_gather_norm_rope_q8). save: uint8 [N, q8_save_row_bytes(cfg)]."""
     cache.check(cfg, cfg.n_tokens)
+    _words(mask, idx, count, pos)
     _check(load().fxr_gather_norm_rope_q8(cfg.ref(), q.data_ptr(), k.data_ptr(), v.data_ptr(), mask.data_ptr(),
                                           idx.data_ptr(), count.data_ptr(), _ptr(pos), norm_q.data_ptr(),
                                           norm_k.data_ptr(), qc.data_ptr(), qc.stride(0), cache.ref, _ptr(save),
@@ -881,6 +890,7 @@ def cache_write_q8(cfg: FrameConfig, cache_k, cache_v, cache: CacheQ8, idx=None,
     rows, cols = host_count if idx is None and count is None else cfg.n_tokens, cfg.n_heads * cfg.head_dim
     _check_extent(cache_k, rows, cfg.ld_cache or cols, cols, cache.k_scale.dtype, "cache_k")
     _check_extent(cache_v, rows, cfg.ld_cache or cols, cols, cache.k_scale.dtype, "cache_v")
+    _words(idx, count)
     if idx is not None and count is None and idx.numel() < host_count:
         _refuse(f"idx: {idx.numel()} entries, host_count is {host_count}")
     _check(load().fxr_cache_write_q8(cfg.ref(), _ptr(cache_k), _ptr(cache_v), _ptr(idx), _ptr(count), host_count,
@@ -913,6 +923,7 @@ def cache_read_q8(cfg: FrameConfig, cache: CacheQ8, k, v, idx=None, count=None, 
     _check_rows(v, rows, cols, dtype, "v")
     if k.stride() != v.stride():
         _refuse("k and v: one row stride")
+    _words(idx, count)
     if count is not None:
         host_count = min(k.shape[0], v.shape[0])
     elif idx is not None and idx.numel() < host_count:
@@ -923,6 +934,7 @@ def cache_read_q8(cfg: FrameConfig, cache: CacheQ8, k, v, idx=None, count=None, 
 
 def restore_rows_q8(cfg: FrameConfig, mask, idx, count, save, cache: CacheQ8, stream=None):
     cache.check(cfg, cfg.n_tokens)
+    _words(mask, idx, count)
     _check(load().fxr_restore_rows_q8(cfg.ref(), _ptr(mask), _ptr(idx), _ptr(count), _ptr(save), cache.ref,
                                       _raw_stream(cache.device, stream, mask, idx, count, save)))
 
@@ -964,6 +976,7 @@ def q8_streams(streams) -> Q8Streams:
     if made.streams:
         _device_of(*[f.get(n) for f in made.streams for n in ("qc", "idx", "count", "out", "q_groups", "k_groups")],
                    *[f["cache"].k for f in made.streams])
+        _words(*[f[n] for f in made.streams for n in ("idx", "count")])
     return made
 
 
@@ -998,6 +1011,7 @@ def frame_forward_q8(cfg: FrameConfig, q, k, v, mask, valid, pos, norm_q, norm_k
                      max_rows: int = 0, stream=None):
     """One frame over an 8-bit cache (fxr_frame_forward_q8)."""
     cache.check(cfg, cfg.n_tokens)
+    _words(mask, pos)
     _groups(q_groups, cfg.n_tokens, "q_groups")
     _groups(k_groups, cfg.n_tokens, "k_groups")
     if prefix is not None:

@@ -293,3 +293,25 @@ def test_write_refuses_sources_that_do_not_hold_the_rows():
                        (wide, src(16, 3 * D)[:, :2 * D], {}), (wide, src(16, 4 * D)[:, :2 * D], {}), (cfg, src(16), {"idx": idx, "host_count": 5})):
         with pytest.raises(fxr.FxrError, match="the cache is on"):
             fxr.cache_write_q8(c, k, k, cache, **more)
+
+
+def test_lists_counts_and_masks_of_other_types_are_refused(monkeypatch):
+    cfg, cache = cfg_of(16, 2, "bf16"), cpu_cache(16)
+    good, x = torch.zeros(48, dtype=torch.int32), torch.zeros(16, 2 * D, dtype=torch.bfloat16)
+    w = torch.ones(D)
+    save = torch.zeros(16, 2 * 2 * D + 16, dtype=torch.uint8)
+    monkeypatch.setattr(fxr, "_device_of", lambda *t: 0)
+    st = {"qc": x, "out": x, "cache": cache}
+    for bad in (good.long(), good.float(), good.short(), good.to(torch.uint8)):
+        for call in (lambda b: fxr.cache_read_q8(cfg, cache, x, x, idx=b, count=good), lambda b: fxr.cache_read_q8(cfg, cache, x, x, idx=good, count=b),
+                     lambda b: fxr.cache_write_q8(cfg, x, x, cache, idx=b, count=good), lambda b: fxr.cache_write_q8(cfg, x, x, cache, idx=good, count=b),
+                     lambda b: fxr.restore_rows_q8(cfg, b, good, good, save, cache), lambda b: fxr.restore_rows_q8(cfg, good, b, good, save, cache),
+                     lambda b: fxr.gather_norm_rope_q8(cfg, x, x, x, b, good, good, good, w, w, x, cache),
+                     lambda b: fxr.gather_norm_rope_q8(cfg, x, x, x, good, b, good, good, w, w, x, cache),
+                     lambda b: fxr.gather_norm_rope_q8(cfg, x, x, x, good, good, b, good, w, w, x, cache),
+                     lambda b: fxr.gather_norm_rope_q8(cfg, x, x, x, good, good, good, b, w, w, x, cache),
+                     lambda b: fxr.frame_forward_q8(cfg, x, x, x, b, None, good, w, w, cache, x, save),
+                     lambda b: fxr.q8_streams([dict(st, idx=b, count=good)]), lambda b: fxr.q8_streams([dict(st, idx=good, count=b)])):
+            with pytest.raises(fxr.FxrError, match="32-bit words"):
+                call(bad)
+    fxr.q8_streams([dict(st, idx=good, count=good.to(torch.uint32))])
