@@ -771,17 +771,24 @@ def _refuse(msg: str):
     raise FxrError(FXR_ERR_INVALID, msg)
 
 
+_torch_c = None          # torch._C; these calls take a few microseconds, and an import statement a tenth of one
+_word_types = ()
+
+
 def _raw_stream(device: int, stream, *tensors) -> int:
     """The cudaStream_t of `stream` or of the current stream of `device`, which has to be the current
     device and hold the tensors (None entries apart). These calls take a few microseconds on the GPU,
     so the handle is asked for without a Stream object."""
-    import torch
+    global _torch_c
+    if _torch_c is None:
+        import torch
+        _torch_c = torch._C
     for t in tensors:
         if t is not None and t.get_device() != device:
             _refuse(f"tensor on {t.device}, the cache is on cuda:{device}")
-    if torch._C._cuda_getDevice() != device:
-        _refuse(f"tensor on cuda:{device}, the current device is cuda:{torch._C._cuda_getDevice()}")
-    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
+    if _torch_c._cuda_getDevice() != device:
+        _refuse(f"tensor on cuda:{device}, the current device is cuda:{_torch_c._cuda_getDevice()}")
+    return _torch_c._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
 def _device_of(*tensors):
@@ -793,10 +800,14 @@ def _device_of(*tensors):
 
 
 def _words(*tensors):
-    """Refuses lists, counts and masks (None entries apart) that are not 32-bit words: others were read as such."""
-    import torch
+    """Refuses lists, counts, masks and positions (None entries apart) that are not 32-bit words: others were
+    read as such."""
+    global _word_types
+    if not _word_types:
+        import torch
+        _word_types = (torch.int32, torch.uint32)
     for t in tensors:
-        if t is not None and t.dtype is not torch.int32 and t.dtype is not torch.uint32:
+        if t is not None and t.dtype not in _word_types:
             _refuse(f"idx, count, mask and pos are 32-bit words: got {t.dtype}")
 
 
@@ -828,7 +839,7 @@ class CacheQ8:
             _refuse("codes and scales on one device")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.device, self.dtype = k.device.index, {torch.bfloat16: "bf16", torch.float16: "f16"}[k_scale.dtype]
-        self.n_rows, self.n_heads = k.shape[0], k_scale.shape[0]
+        self.n_rows, self.n_heads, self.scale_type = k.shape[0], k_scale.shape[0], k_scale.dtype
         # a single row or head has no stride of its own
         ld = k.stride(0) if k.shape[0] > 1 else max(k.stride(0), k.shape[1])
         ld_scale = k_scale.stride(0) if k_scale.shape[0] > 1 else k_scale.shape[1] // 8 * 8
@@ -863,18 +874,23 @@ def gather_norm_rope_q8(cfg: FrameConfig, q, k, v, mask, idx, count, pos, norm_q
     cache.check(cfg, cfg.n_tokens)
     _words(mask, idx, count, pos)
     _check(load().fxr_gather_norm_rope_q8(cfg.ref(), q.data_ptr(), k.data_ptr(), v.data_ptr(), mask.data_ptr(),
-                                          idx.data_ptr(), count.data_ptr(), _ptr(pos), norm_q.data_ptr(),
-                                          norm_k.data_ptr(), qc.data_ptr(), qc.stride(0), cache.ref, _ptr(save),
+                                          idx.data_ptr(), count.data_ptr(), None if pos is None else pos.data_ptr(),
+                                          norm_q.data_ptr(), norm_k.data_ptr(), qc.data_ptr(), qc.stride()[0], cache.ref,
+                                          None if save is None else save.data_ptr(),
                                           _raw_stream(cache.device, stream, q, k, v, mask, idx, count, pos, norm_q,
                                                       norm_k, qc, save)))
+
+
+def _span(t) -> int:
+    """Elements from a tensor's first to its last."""
+    return t.numel() if t.is_contiguous() or t.numel() == 0 else 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
 
 
 def _check_extent(t, rows: int, ld: int, cols: int, dtype, what: str):
     """Refuses a tensor of another type, or one that ends before `rows` rows of `cols` elements, `ld` apart."""
     if t is None or rows <= 0:
         return
-    held = t.numel() if t.is_contiguous() else 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    if t.dtype is not dtype or held < (rows - 1) * ld + cols:
+    if t.dtype is not dtype or _span(t) < (rows - 1) * ld + cols:
         _refuse(f"{what}: {rows} rows of {cols} elements of {dtype}, {ld} apart, needed: got {tuple(t.shape)} of {t.dtype}, "
                 f"strides {t.stride()}")
 
@@ -888,8 +904,8 @@ def cache_write_q8(cfg: FrameConfig, cache_k, cache_v, cache: CacheQ8, idx=None,
         host_count = cfg.n_tokens
     # without a list the rows are the first ones; a listed row may be any of the frame's
     rows, cols = host_count if idx is None and count is None else cfg.n_tokens, cfg.n_heads * cfg.head_dim
-    _check_extent(cache_k, rows, cfg.ld_cache or cols, cols, cache.k_scale.dtype, "cache_k")
-    _check_extent(cache_v, rows, cfg.ld_cache or cols, cols, cache.k_scale.dtype, "cache_v")
+    _check_extent(cache_k, rows, cfg.ld_cache or cols, cols, cache.scale_type, "cache_k")
+    _check_extent(cache_v, rows, cfg.ld_cache or cols, cols, cache.scale_type, "cache_v")
     _words(idx, count)
     if idx is not None and count is None and idx.numel() < host_count:
         _refuse(f"idx: {idx.numel()} entries, host_count is {host_count}")
@@ -899,8 +915,6 @@ def cache_write_q8(cfg: FrameConfig, cache_k, cache_v, cache: CacheQ8, idx=None,
 
 def _check_rows(t, rows: int, cols: int, dtype, what: str):
     """Refuses a tensor that does not hold `rows` rows of `cols` adjacent elements of `dtype`."""
-    if t is None:
-        _refuse(f"{what}: null pointer")
     shape, stride = t.shape, t.stride()
     if len(shape) == 2:
         whole = shape[1] >= cols and (stride[1] == 1 or cols == 1)
@@ -918,18 +932,24 @@ def cache_read_q8(cfg: FrameConfig, cache: CacheQ8, k, v, idx=None, count=None, 
     if count is None and idx is None and host_count < 0:
         host_count = cache.n_rows
     rows = 0 if count is not None else host_count
-    cols, dtype = cfg.n_heads * cfg.head_dim, cache.k_scale.dtype
-    _check_rows(k, rows, cols, dtype, "k")
-    _check_rows(v, rows, cols, dtype, "v")
-    if k.stride() != v.stride():
+    cols, dtype = cfg.n_heads * cfg.head_dim, cache.scale_type
+    if k is None or v is None:
+        _refuse("k and v: null pointer")
+    shape, stride = k.shape, k.stride()
+    if stride != v.stride():
         _refuse("k and v: one row stride")
+    if v.shape != shape or len(shape) != 2 or stride[1] != 1 or shape[1] < cols or shape[0] < rows or \
+            k.dtype is not dtype or v.dtype is not dtype:
+        _check_rows(k, rows, cols, dtype, "k")
+        _check_rows(v, rows, cols, dtype, "v")
     _words(idx, count)
     if count is not None:
-        host_count = min(k.shape[0], v.shape[0])
+        host_count = min(shape[0], v.shape[0])
     elif idx is not None and idx.numel() < host_count:
         _refuse(f"idx: {idx.numel()} entries, host_count is {host_count}")
-    _check(load().fxr_cache_read_q8(cfg.ref(), cache.ref, _ptr(idx), _ptr(count), host_count, k.data_ptr(),
-                                    v.data_ptr(), k.stride(0), _raw_stream(cache.device, stream, k, v, idx, count)))
+    _check(load().fxr_cache_read_q8(cfg.ref(), cache.ref, None if idx is None else idx.data_ptr(),
+                                    None if count is None else count.data_ptr(), host_count, k.data_ptr(),
+                                    v.data_ptr(), stride[0], _raw_stream(cache.device, stream, k, v, idx, count)))
 
 
 def restore_rows_q8(cfg: FrameConfig, mask, idx, count, save, cache: CacheQ8, stream=None):
@@ -947,7 +967,7 @@ class Q8Streams:
         self.array = (Q8StreamStruct * max(len(streams), 1))()
         for b, f in enumerate(streams):
             qc, out, cache = f["qc"], f["out"], f["cache"]
-            if qc.dtype != cache.k_scale.dtype or out.dtype != qc.dtype:
+            if qc.dtype != cache.scale_type or out.dtype != qc.dtype:
                 _refuse("qc, out and the scales are of one type")
             self.array[b] = Q8StreamStruct(_ptr(qc), qc.stride(0) if qc.shape[0] > 1 else qc.shape[1], _ptr(f["idx"]),
                                            _ptr(f["count"]), _ptr(out), _ptr(f.get("q_groups")),
@@ -955,6 +975,10 @@ class Q8Streams:
         self.rows = min((f["qc"].shape[0] for f in streams), default=0)
         self.device = streams[0]["cache"].device if streams else None
         self.tokens = min((f["out"].shape[0] for f in streams), default=0)
+        # elements that the outputs span, and that a query row may at most have
+        self.out_span = min((_span(f["out"]) for f in streams), default=0)
+        self.q_cols = min((_span(f["qc"]) - (f["qc"].shape[0] - 1) * self.array[b].ld_qc for b, f in enumerate(streams)
+                           if f["qc"].shape[0]), default=1 << 62)
 
     def check(self, cfg: FrameConfig, max_rows: int = 0):
         n = cfg.n_tokens
@@ -967,6 +991,11 @@ class Q8Streams:
             f["cache"].check(cfg, n, "stream cache")
             _groups(f.get("q_groups"), n, "q_groups")
             _groups(f.get("k_groups"), n, "k_groups")
+        cols = cfg.n_heads * cfg.head_dim
+        if self.streams and n and self.out_span < (n - 1) * (cfg.ld_out or cols) + cols:
+            _refuse(f"out ends before {n} rows of {cols} elements, {cfg.ld_out or cols} apart")
+        if self.q_cols < cols:
+            _refuse(f"qc ends before {cols} elements of its last row")
 
 
 def q8_streams(streams) -> Q8Streams:

@@ -315,3 +315,22 @@ def test_lists_counts_and_masks_of_other_types_are_refused(monkeypatch):
             with pytest.raises(fxr.FxrError, match="32-bit words"):
                 call(bad)
     fxr.q8_streams([dict(st, idx=good, count=good.to(torch.uint32))])
+
+
+def test_attention_refuses_queries_and_outputs_that_end_early():
+    cfg, cache = cfg_of(16, 2, "bf16", ld_out=2 * D + 16), cpu_cache(16)
+    one = torch.zeros(16, dtype=torch.int32)
+    out = torch.zeros(16, 2 * D + 16, dtype=torch.bfloat16)[:, :2 * D]
+    make = lambda **t: fxr.Q8Streams([dict({"qc": torch.zeros(4, 2 * D, dtype=torch.bfloat16), "idx": one, "count": one, "out": out,  # noqa: E731
+                                            "cache": cache}, **t)])
+    make().check(cfg, 4)
+    make(qc=torch.zeros(4, 2, D, dtype=torch.bfloat16)).check(cfg, 4)
+    make(qc=torch.zeros(9, 4 * D, dtype=torch.bfloat16)[:4, :2 * D]).check(cfg, 4)
+    with pytest.raises(fxr.FxrError, match="out ends"):
+        make(out=torch.zeros(16, 2 * D, dtype=torch.bfloat16)).check(cfg, 4)
+    with pytest.raises(fxr.FxrError, match="out ends"):
+        make(out=torch.zeros(16, 2 * D + 8, dtype=torch.bfloat16)).check(cfg, 4)
+    with pytest.raises(fxr.FxrError, match="qc ends"):
+        make(qc=torch.zeros(4, D, dtype=torch.bfloat16)).check(cfg, 4)
+    with pytest.raises(fxr.FxrError, match="qc ends"):
+        make(qc=torch.zeros(4, 2 * D + 8, dtype=torch.bfloat16)[:, :D]).check(cfg, 4)
