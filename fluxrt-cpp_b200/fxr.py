@@ -868,6 +868,25 @@ def q8_save_row_bytes(cfg: FrameConfig) -> int:
     return int(load().fxr_q8_save_row_bytes(cfg.ref()))
 
 
+def _check_frame(cfg: FrameConfig, cache: CacheQ8, q, k, v, mask, pos, norm_q, norm_k):
+    """Refuses a frame's inputs that end before its tokens, or are of another type."""
+    import torch
+    n, cols, dtype = cfg.n_tokens, cfg.n_heads * cfg.head_dim, cache.scale_type
+    _words(mask, pos)
+    if n <= 0:
+        return
+    need = (n - 1) * (cfg.ld_qkv or cols) + cols
+    for t, what in ((q, "q"), (k, "k"), (v, "v")):
+        if t is not None and (t.dtype is not dtype or t.numel() < need or not t.is_contiguous()):
+            _check_extent(t, n, cfg.ld_qkv or cols, cols, dtype, what)
+    for t in (norm_q, norm_k):
+        if t is not None and (t.dtype is not torch.float32 or t.numel() < cfg.head_dim or not t.is_contiguous()):
+            _refuse(f"norm weights: {cfg.head_dim} contiguous float32, got {tuple(t.shape)} of {t.dtype}")
+    for t, size, what in ((mask, n, "mask"), (pos, n * len(cfg.rope_axes), "pos")):
+        if t is not None and (t.numel() < size or not t.is_contiguous()):
+            _refuse(f"{what}: {size} contiguous values needed, got {tuple(t.shape)}, strides {t.stride()}")
+
+
 def gather_norm_rope_q8(cfg: FrameConfig, q, k, v, mask, idx, count, pos, norm_q, norm_k, qc, cache: CacheQ8,
                         save=None, stream=None):
     """gather_norm_rope into an 8-bit cache (fxr_gather_norm_rope_q8). save: uint8 [N, q8_save_row_bytes(cfg)]."""
@@ -1040,7 +1059,11 @@ def frame_forward_q8(cfg: FrameConfig, q, k, v, mask, valid, pos, norm_q, norm_k
                      max_rows: int = 0, stream=None):
     """One frame over an 8-bit cache (fxr_frame_forward_q8)."""
     cache.check(cfg, cfg.n_tokens)
-    _words(mask, pos)
+    _check_frame(cfg, cache, q, k, v, mask, pos, norm_q, norm_k)
+    n, cols = cfg.n_tokens, cfg.n_heads * cfg.head_dim
+    _check_extent(out, n, cfg.ld_out or cols, cols, cache.scale_type, "out")
+    if valid is not None and (valid.numel() * valid.element_size() < n or valid.element_size() != 1):
+        _refuse(f"valid: {n} bytes needed, got {tuple(valid.shape)} of {valid.dtype}")
     _groups(q_groups, cfg.n_tokens, "q_groups")
     _groups(k_groups, cfg.n_tokens, "k_groups")
     if prefix is not None:

@@ -317,6 +317,36 @@ def test_lists_counts_and_masks_of_other_types_are_refused(monkeypatch):
     fxr.q8_streams([dict(st, idx=good, count=good.to(torch.uint32))])
 
 
+def test_frames_refuse_inputs_that_end_early_or_are_of_another_type():
+    cfg, cache = cfg_of(16, 2, "bf16", ld_qkv=2 * D + 8, ld_out=2 * D + 16), cpu_cache(16)
+    x = torch.zeros(16, 2 * D + 8, dtype=torch.bfloat16)
+    good = {"q": x, "k": x[:, :2 * D], "v": x, "mask": torch.zeros(16, dtype=torch.int32), "pos": torch.zeros(16, 3, dtype=torch.int32),
+            "norm_q": torch.ones(D), "norm_k": torch.ones(D)}
+    frame = dict(good, valid=torch.zeros(16, dtype=torch.uint8), out=torch.zeros(16, 2 * D + 16, dtype=torch.bfloat16)[:, :2 * D])
+    one, work = torch.zeros(16, dtype=torch.int32), torch.zeros(64, dtype=torch.uint8)
+
+    def whole(**t):
+        t = dict(frame, **t)
+        fxr.frame_forward_q8(cfg, t["q"], t["k"], t["v"], t["mask"], t["valid"], t["pos"], t["norm_q"], t["norm_k"], cache, t["out"], work)
+
+    for name in "qkv":
+        for bad in (x[:15], x[:, :2 * D].contiguous(), x.half(), x.float(), torch.zeros(16, 2 * D + 16, dtype=torch.bfloat16).t()[:16]):
+            with pytest.raises(fxr.FxrError, match=f"{name}: 16 rows of 256"):
+                whole(**{name: bad})
+    for bad, word in (({"mask": one[:15]}, "mask"), ({"mask": torch.zeros(32, dtype=torch.int32)[::2]}, "mask"), ({"pos": good["pos"][:15]}, "pos"),
+                      ({"pos": torch.zeros(3, 16, dtype=torch.int32).t()}, "pos"), ({"norm_q": torch.ones(D).bfloat16()}, "norm"),
+                      ({"norm_k": torch.ones(D - 1)}, "norm"), ({"norm_k": torch.ones(2 * D)[::2]}, "norm")):
+        with pytest.raises(fxr.FxrError, match=word):
+            whole(**bad)
+    for bad, word in (({"out": frame["out"][:15]}, "out"), ({"out": torch.zeros(16, 2 * D, dtype=torch.bfloat16)}, "out"),
+                      ({"out": frame["out"].half()}, "out"), ({"valid": frame["valid"][:15]}, "valid"), ({"valid": one}, "valid")):
+        with pytest.raises(fxr.FxrError, match=word):
+            whole(**bad)
+    for more in ({}, {"valid": None}, {"valid": torch.zeros(16, dtype=torch.bool)}):
+        with pytest.raises(fxr.FxrError, match="the cache is on"):
+            whole(**more)
+
+
 def test_attention_refuses_queries_and_outputs_that_end_early():
     cfg, cache = cfg_of(16, 2, "bf16", ld_out=2 * D + 16), cpu_cache(16)
     one = torch.zeros(16, dtype=torch.int32)
