@@ -327,8 +327,13 @@ def dtype_code(torch_dtype) -> int:
     return {torch.float32: FXR_F32, torch.float16: FXR_F16, torch.bfloat16: FXR_BF16}[torch_dtype]
 
 
+class _Made:
+    """Room for what a FrameConfig has made of its fields, outside its state."""
+    __slots__ = ("_made",)
+
+
 @dataclass
-class FrameConfig:
+class FrameConfig(_Made):
     n_tokens: int
     n_text: int
     n_heads: int = 24
@@ -344,13 +349,19 @@ class FrameConfig:
 
     def __setattr__(self, name, value):
         object.__setattr__(self, name, value)
-        object.__setattr__(self, "_ref", None)
+        object.__setattr__(self, "_made", None)
+
+    def __getstate__(self):
+        return dict(self.__dict__)           # copies and pickles are of the fields
 
     def ref(self):
         """A ctypes reference to desc(), built once until a field changes (for calls of a few microseconds)."""
-        if self._ref is None:
-            object.__setattr__(self, "_ref", ctypes.byref(self.desc()))
-        return self._ref
+        axes = tuple(self.rope_axes)         # which may be a list that is changed in place
+        made = getattr(self, "_made", None)
+        if made is None or made[0] != axes:
+            made = axes, ctypes.byref(self.desc())
+            object.__setattr__(self, "_made", made)
+        return made[1]
 
     def desc(self) -> FrameDesc:
         d = FrameDesc()

@@ -7,7 +7,10 @@ rounding to T (many rows) drops out of the bars, which then are tight; derived b
   P and V are rounded to T (u each at most), exponentials to 2^-13, the output once:
       |err| <= u |o| + (2 u + 2^-13 + expm1(2 ds)) sum(w |v|)
 """
+import copy
+import dataclasses
 import math
+import pickle
 
 import pytest
 import torch
@@ -364,3 +367,24 @@ def test_attention_refuses_queries_and_outputs_that_end_early():
         make(qc=torch.zeros(4, D, dtype=torch.bfloat16)).check(cfg, 4)
     with pytest.raises(fxr.FxrError, match="qc ends"):
         make(qc=torch.zeros(4, 2 * D + 8, dtype=torch.bfloat16)[:, :D]).check(cfg, 4)
+
+
+def test_a_used_configuration_is_copied_and_pickled_as_its_fields():
+    cfg = cfg_of(8, 2, "bf16", rope_axes=[16, 56, 56])
+    fresh = cfg_of(8, 2, "bf16", rope_axes=[16, 56, 56])
+    cfg.ref()
+    for other in (copy.copy(cfg), copy.deepcopy(cfg), pickle.loads(pickle.dumps(cfg)), pickle.loads(pickle.dumps(cfg, protocol=2)),
+                  dataclasses.replace(cfg), fxr.FrameConfig(**vars(cfg))):
+        assert other == cfg == fresh and vars(other) == vars(fresh) and repr(other) == repr(fresh)
+        other.n_tokens = 9
+        assert other.ref()._obj.n_tokens == 9 and cfg.ref()._obj.n_tokens == 8
+    assert dataclasses.asdict(cfg) == dataclasses.asdict(fresh)
+
+
+def test_a_configuration_s_reference_follows_axes_changed_in_place():
+    cfg = cfg_of(8, 2, "bf16", rope_axes=[16, 56, 56])
+    assert list(cfg.ref()._obj.rope_axes_dim)[:3] == [16, 56, 56]
+    cfg.rope_axes[0], cfg.rope_axes[1] = 32, 40
+    assert list(cfg.ref()._obj.rope_axes_dim)[:3] == list(cfg.desc().rope_axes_dim)[:3] == [32, 40, 56]
+    cfg.rope_axes.append(0)
+    assert cfg.ref()._obj.rope_n_axes == 4 and cfg.ref() is cfg.ref()
