@@ -306,7 +306,7 @@ def load(path: str | None = None) -> ctypes.CDLL:
 
 
 def _check(status: int):
-    if status != FXR_OK:
+    if status:
         raise FxrError(status, load().fxr_last_error_string().decode())
 
 
@@ -972,14 +972,16 @@ def cache_read_q8(cfg: FrameConfig, cache: CacheQ8, k, v, idx=None, count=None, 
             k.dtype is not dtype or v.dtype is not dtype:
         _check_rows(k, rows, cols, dtype, "k")
         _check_rows(v, rows, cols, dtype, "v")
-    _words(idx, count)
+    if idx is not None or count is not None:
+        _words(idx, count)
     if count is not None:
         host_count = min(shape[0], v.shape[0])
     elif idx is not None and idx.numel() < host_count:
         _refuse(f"idx: {idx.numel()} entries, host_count is {host_count}")
-    _check(load().fxr_cache_read_q8(cfg.ref(), cache.ref, None if idx is None else idx.data_ptr(),
-                                    None if count is None else count.data_ptr(), host_count, k.data_ptr(),
-                                    v.data_ptr(), stride[0], _raw_stream(cache.device, stream, k, v, idx, count)))
+    _check((_lib or load()).fxr_cache_read_q8(cfg.ref(), cache.ref, None if idx is None else idx.data_ptr(),
+                                              None if count is None else count.data_ptr(), host_count, k.data_ptr(),
+                                              v.data_ptr(), stride[0],
+                                              _raw_stream(cache.device, stream, k, v, idx, count)))
 
 
 def restore_rows_q8(cfg: FrameConfig, mask, idx, count, save, cache: CacheQ8, stream=None):
