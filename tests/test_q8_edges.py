@@ -5,7 +5,10 @@ rounding to T (many rows) drops out of the bars, which then are tight; derived b
   sum|q k|, and a few roundings of 2^-24 of the score follow: ds = (2^-16 + 2^-21) * scale * max_j sum|q k_j|, also where
   bf16 queries are held in f16 (elements below 2^-24 of the largest round to a step of 2^-35 of it, 128 of them: 2^-28);
   P and V are rounded to T (u each at most), exponentials to 2^-13, the output once:
-      |err| <= u |o| + (2 u + 2^-13 + expm1(2 ds)) sum(w |v|)
+      |err| <= u |o| + (2 u + 2^-13 + expm1(2 ds)) sum(w |v|) + small
+  small: P in f16 is a subnormal below 2^-14, off by up to 2^-25. The largest P of a row is at least 1 (its running maximum
+  is never above the largest score), so that is 2^-25 of the largest weight for each key: 2^-25 max(w) sum|v|. The kernel
+  for few rows holds P times the V scale in f16 for every T, whose largest is at least 1: 2^-25 max(w scale) sum|code|.
 """
 import copy
 import dataclasses
@@ -16,7 +19,7 @@ import pytest
 import torch
 
 import fxr
-from test_q8_cache import D, TDT, cfg_of, filled_cache, randn, rng_of, stream_of, sync_ok, workspace_for
+from test_q8_cache import D, TDT, cfg_of, filled_cache, frame_inputs, rng_of, stream_of, sync_ok, workspace_for
 
 FEW = 32        # rows that the kernel for few rows takes; it holds K and V exactly
 
@@ -31,7 +34,7 @@ def e4m3_values():
 
 def held(cache, n, exact):
     """K and V [n, heads, 128] in 64 bits as the attention holds them: codes times scales, exactly or rounded to T and
-    finite. Keys without a valid scale: K NaN."""
+    finite. Keys without a valid scale: K NaN. And V's scales [n, heads, 1]."""
     h, t = cache.n_heads, cache.k_scale.dtype
     out, bad = [], None
     for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
@@ -46,7 +49,7 @@ def held(cache, n, exact):
         x = x.view(n, h, D) * torch.where(invalid, torch.zeros_like(s), s)[..., None]
         out.append(x if exact else x.to(t).double().clamp(-torch.finfo(t).max, torch.finfo(t).max))
     out[0] = torch.where(bad[..., None], torch.full_like(out[0], math.nan), out[0])
-    return out
+    return out[0], out[1], torch.where(invalid, torch.zeros_like(s), s)[..., None]
 
 
 def check(cfg, st, max_rows, prefix=None, prefix_groups=None, what="", rows=None, telling=0.7):
@@ -55,19 +58,18 @@ def check(cfg, st, max_rows, prefix=None, prefix_groups=None, what="", rows=None
     n, m, h, t = cfg.n_tokens, st["m"], cfg.n_heads, TDT[cfg.dtype]
     u = torch.finfo(t).eps / 2
     exact = 0 < max_rows <= FEW
-    k, v = held(st["cache"], n, exact)
+    k, v, vs = held(st["cache"], n, exact)
     ones = lambda r: torch.full((r,), -1, dtype=torch.int32, device="cuda")  # noqa: E731
     kg = st.get("k_groups") if st.get("k_groups") is not None else ones(n)
     if prefix is not None:
-        pk, pv = held(prefix, prefix.n_rows, exact)
-        k, v = torch.cat([pk, k]), torch.cat([pv, v])
+        k, v, vs = (torch.cat(x) for x in zip(held(prefix, prefix.n_rows, exact), (k, v, vs)))
         kg = torch.cat([prefix_groups if prefix_groups is not None else ones(prefix.n_rows), kg])
     at = st["idx"][:m].long()
     qg = st["q_groups"][at] if st.get("q_groups") is not None else ones(m)
     seen = (qg[:, None] & kg[None]) != 0
     scale = cfg.softmax_scale if cfg.softmax_scale > 0 else 1 / math.sqrt(D)
     q = st["qc"][:m].double().view(m, h, D).transpose(0, 1)
-    k, v = k.transpose(0, 1), v.transpose(0, 1)
+    k, v, vs = (x.transpose(0, 1) for x in (k, v, vs))
     s = (q @ k.transpose(1, 2) * scale).masked_fill(~seen[None], -math.inf)
     nan = torch.isnan(s).any(-1)
     s = torch.nan_to_num(s, nan=-math.inf, neginf=-math.inf)
@@ -76,6 +78,12 @@ def check(cfg, st, max_rows, prefix=None, prefix_groups=None, what="", rows=None
     ds = (q.abs() @ torch.nan_to_num(k).abs().transpose(1, 2) * scale).masked_fill(~seen[None], 0).amax(-1, keepdim=True)
     bar = u * o.abs() + (2 * u + 2 ** -13 + torch.expm1(2 * (2 ** -16 + 2 ** -21) * ds)) * mean_abs
     bar = bar + torch.finfo(t).smallest_normal * torch.finfo(t).eps
+    some = seen.double()[None]
+    if exact:
+        vs = vs.abs()
+        bar = bar + 2.0 ** -25 * (w * vs.transpose(1, 2)).amax(-1, keepdim=True) * (some @ torch.where(vs > 0, v.abs() / vs, vs))
+    elif t == torch.float16:
+        bar = bar + 2.0 ** -25 * w.amax(-1, keepdim=True) * (some @ v.abs())
     got = st["out"][at].double().view(m, h, D).transpose(0, 1)
     if rows is not None:
         got, o, bar, nan = got[:, rows], o[:, rows], bar[:, rows], nan[:, rows]
@@ -158,7 +166,7 @@ def test_every_code_counts_as_one_number(cuda, dtype, n, heads, m):
     k, v = (torch.zeros(n, heads * D, dtype=TDT[dtype], device="cuda") for _ in range(2))
     fxr.cache_read_q8(cfg, c, k, v)
     sync_ok()
-    for got, want in zip((k, v), held(c, n, True)):
+    for got, want in zip((k, v), held(c, n, True)[:2]):
         assert torch.equal(got, want.reshape(n, -1).to(TDT[dtype]))
 
 
@@ -273,7 +281,7 @@ def test_read_back_with_a_device_count_stays_in_its_outputs(cuda, listed, rows, 
     sync_ok()
     at = idx.long() if listed else torch.arange(n, device="cuda")
     written = min(rows, asked, n)
-    for a, want in zip(store, held(cache, n, True)):
+    for a, want in zip(store, held(cache, n, True)[:2]):
         assert torch.equal(a[:written], want.reshape(n, -1)[at[:written]].bfloat16()) and (a[written:] == 5).all()
 
 
@@ -388,3 +396,43 @@ def test_a_configuration_s_reference_follows_axes_changed_in_place():
     assert list(cfg.ref()._obj.rope_axes_dim)[:3] == list(cfg.desc().rope_axes_dim)[:3] == [32, 40, 56]
     cfg.rope_axes.append(0)
     assert cfg.ref()._obj.rope_n_axes == 4 and cfg.ref() is cfg.ref()
+
+
+# ---- values that the bars of a rounded K leave open -------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, fmt", [("bf16", "int8"), ("bf16", "e4m3"), ("f16", "int8"), ("f16", "e4m3")])
+@pytest.mark.parametrize("n, heads, m", [(700, 2, 2), (333, 2, 30), (700, 2, 300), (2400, 32, 1950)])
+@pytest.mark.parametrize("spread", [5.0, 30.0])
+def test_scores_in_the_hundreds(cuda, dtype, fmt, n, heads, m, spread):
+    """The running maximum moves often, and a row's result is that of a few keys."""
+    g = rng_of(int(spread) + m)
+    cfg = cfg_of(n, heads, dtype, softmax_scale=spread / math.sqrt(D))
+    st = stream_of(g, cfg, m)
+    st["cache"] = filled_cache(g, cfg, n, fmt)
+    attend(cfg, st, m)
+    check(cfg, st, m, telling=0.9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, fmt", [("bf16", "int8"), ("bf16", "e4m3"), ("f16", "int8"), ("f16", "e4m3")])
+@pytest.mark.parametrize("n, heads, m", [(333, 2, 5), (333, 2, 30), (333, 2, 290), (2400, 32, 1950)])
+@pytest.mark.parametrize("groups", [False, True])
+def test_large_scales(cuda, dtype, fmt, n, heads, m, groups):
+    """Scales that the kernels decode in two steps (e4m3 from 128 and 136 on), of K (whose codes are the smallest then, so
+    that scores stay plain) and of V, in tiles with smaller ones."""
+    g = rng_of(m + n)
+    cfg = cfg_of(n, heads, dtype)
+    st = stream_of(g, cfg, m)
+    st["cache"] = c = filled_cache(g, cfg, n, fmt)
+    big = 140.0 if dtype == "f16" else 3000.0 if fmt == "e4m3" else 2.0 ** 90
+    c.v_scale[:, 5:n:7] = big
+    rows = torch.arange(3, n, 9, device="cuda")
+    small = torch.randint(-4, 5, (len(rows), heads * D), generator=g, device="cuda").to(torch.int8)
+    if fmt == "e4m3":               # +-4 times 2^-9
+        small = torch.where(small < 0, -small - 128, small).to(torch.int8)
+    c.k.view(torch.int8)[rows] = small
+    c.k_scale[:, 3:n:9] = (140.0 if dtype == "f16" else 256.0) if fmt == "e4m3" else 0.25
+    if groups:
+        st["q_groups"] = st["k_groups"] = torch.where(torch.arange(n, device="cuda") % 3 == 0, 1, 6).int()
+    attend(cfg, st, m)
+    check(cfg, st, m, telling=0.8)
