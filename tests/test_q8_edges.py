@@ -436,3 +436,83 @@ def test_large_scales(cuda, dtype, fmt, n, heads, m, groups):
         st["q_groups"] = st["k_groups"] = torch.where(torch.arange(n, device="cuda") % 3 == 0, 1, 6).int()
     attend(cfg, st, m)
     check(cfg, st, m, telling=0.8)
+
+
+# ---- the frame: groups, and very many rows ----------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, fmt", [("bf16", "e4m3"), ("f16", "int8")])
+@pytest.mark.parametrize("n, heads, rows, bound, prefix, groups", [(300, 3, 20, 24, 0, True), (300, 3, 20, 24, 150, True), (301, 2, 140, 0, 90, True),
+                                                                   (300, 2, 0, 24, 40, True), (700, 2, 300, 310, 0, False),
+                                                                   (4700, 18, 2049, 2100, 0, False), (8003, 12, 1900, 0, 0, False),
+                                                                   (4700, 18, 2049, 2100, 0, True)])
+def test_frames_with_groups_and_with_very_many_rows(cuda, dtype, fmt, n, heads, rows, bound, prefix, groups):
+    """A frame of a stream whose cache is filled: executed rows, rows that are put back, documents, a padded prefix of
+    which nobody sees the end, rows that see nothing."""
+    t = TDT[dtype]
+    g = rng_of(n + rows)
+    cfg = cfg_of(n, heads, dtype)
+    f = frame_inputs(g, cfg)
+    listed = torch.randperm(n, generator=g, device="cuda")[:rows].sort().values
+    mask = torch.zeros(n, dtype=torch.int32, device="cuda")
+    mask[listed] = torch.where(torch.rand(rows, generator=g, device="cuda") < 0.3, 1, 2).int()
+    given = mask.clone()
+    cache = filled_cache(g, cfg, n, fmt)
+    pre = filled_cache(g, cfg, prefix, fmt) if prefix else None
+    qg = kg = pg = None
+    if groups:
+        at = torch.arange(n, device="cuda")
+        kg = torch.bitwise_left_shift(torch.ones_like(at), at * 3 // n).int()
+        kg[n // 2:n // 2 + 9] = 0
+        qg = torch.where(at % 7 == 3, torch.zeros_like(kg), kg | 1)
+        if prefix:
+            pg = torch.full((prefix,), -1, dtype=torch.int32, device="cuda")
+            pg[prefix - prefix // 5:] = 0
+            pre.k_scale[:, :prefix][:, pg == 0] = math.nan
+    copy_of = lambda c: fxr.CacheQ8(*[x.clone() for x in (c.k, c.v, c.k_scale, c.v_scale)])  # noqa: E731
+    old, seen = copy_of(cache), copy_of(cache)
+    out = torch.full((n, heads * D), 7.0, dtype=t, device="cuda")
+    ws = torch.full((fxr.frame_q8_workspace_size(cfg, prefix, bound),), 171, dtype=torch.uint8, device="cuda")
+    fxr.frame_forward_q8(cfg, f["q"], f["k"], f["v"], mask, torch.ones(n, dtype=torch.uint8, device="cuda"), f["pos"], f["norm_q"],
+                         f["norm_k"], cache, out, ws, prefix=pre, prefix_groups=pg, q_groups=qg, k_groups=kg, max_rows=bound)
+    sync_ok()
+    assert torch.equal(mask, given)
+    # the same write without the rows put back: the cache that the attention saw
+    qc, idx = torch.zeros(n, heads * D, dtype=t, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda")
+    idx[:rows] = listed.int()
+    save = torch.zeros(n, fxr.q8_save_row_bytes(cfg), dtype=torch.uint8, device="cuda")
+    fxr.gather_norm_rope_q8(cfg, f["q"], f["k"], f["v"], mask, idx, torch.tensor([rows], dtype=torch.int32, device="cuda"), f["pos"],
+                            f["norm_q"], f["norm_k"], qc, seen, save)
+    sync_ok()
+    st = {"qc": qc, "idx": idx, "m": rows, "cache": seen, "out": out, "q_groups": qg, "k_groups": kg}
+    if rows:
+        check(cfg, st, bound, pre, pg)
+        if groups:
+            assert (out[listed[listed % 7 == 3]] == 0).all()
+    else:
+        assert (out == 7).all()
+    kept = mask == 1
+    for now, was, new in zip((cache.k, cache.v), (old.k, old.v), (seen.k, seen.v)):
+        now, was, new = (x.view(torch.int8) for x in (now, was, new))
+        assert torch.equal(now[kept], was[kept]) and torch.equal(now[~kept], new[~kept])
+    for now, was, new in zip((cache.k_scale, cache.v_scale), (old.k_scale, old.v_scale), (seen.k_scale, seen.v_scale)):
+        assert torch.equal(now[:, :n][:, kept], was[:, :n][:, kept]) and torch.equal(now[:, :n][:, ~kept], new[:, :n][:, ~kept])
+
+
+def test_a_call_from_another_current_device_is_refused(monkeypatch):
+    class On:
+        def __init__(self, index):
+            self.index, self.device = index, f"cuda:{index}"
+
+        def get_device(self):
+            return self.index
+    fxr._raw_stream.__globals__["_torch_c"] = torch._C
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 77)
+    assert fxr._raw_stream(0, None, On(0), None) == 77
+    with pytest.raises(fxr.FxrError, match="tensor on cuda:1, the cache is on cuda:0"):
+        fxr._raw_stream(0, None, On(0), On(1))
+    with pytest.raises(fxr.FxrError, match="the current device is cuda:0"):
+        fxr._raw_stream(1, None, On(1))
+    cache = cpu_cache(16)
+    with pytest.raises(fxr.FxrError, match="null"):
+        fxr.cache_read_q8(cfg_of(16, 2, "bf16"), cache, None, None)
