@@ -42,8 +42,9 @@ struct Params {
 // ---------------------------------------------------------------------------------------------
 // Few rows per stream: bound by reading the cache once. Work is laid on a line of columns, each the
 // keys of one source for one head and one group of 8, 16 or 32 rows: first (head, group of the packed
-// rows of all streams) against the prefix, so that the prefix is read once for every 32 rows of all
-// streams, then (stream, head, group) against the stream's own rows. Where there are at least as many
+// rows of all streams) against the prefix, so that the prefix is read once for every group of packed rows
+// (16, or 32 where a stream may have more than 16), then (stream, head, group) against the stream's own
+// rows. Where there are at least as many
 // CTAs as columns, every column is cut into parts of one length, the shortest (in units of 64 keys)
 // that gives every part a CTA of its own. Otherwise the line is cut into one range per CTA, and a range
 // covers a few items (parts of columns). An item costs its CTA about 6 us besides its keys (queries,
@@ -67,7 +68,9 @@ struct Params {
 // for elements below 2^-24 of the row's largest). K scales multiply the scores in 32 bits. V scales
 // multiply P before its one rounding; the running maximum is that of score + log2(V scale), the weight of
 // a key's codes, so that P stays in f16's range whatever the scales are, and a large V that a row hardly
-// sees, or not at all, costs the others no precision.
+// sees, or not at all, costs the others no precision. (A weight below 2^-14 of the largest is a subnormal of
+// f16, off by up to 2^-25 of the largest.) Error against 64 bits: 0.0017 of the outputs' root mean square in
+// bf16 and 0.00024 in f16, nearly all of it the rounding of the output.
 // Partial results (O, maximum, sum) meet in L2: the last of a row group's parts to arrive combines
 // them in key order, so the result does not depend on the order of arrival.
 // ---------------------------------------------------------------------------------------------
@@ -853,8 +856,11 @@ __global__ void __launch_bounds__(RowsShape<NQ>::threads, 1) rows_kernel(const _
 // scores masked. With visibility groups, visible_steps_kernel lists for every 256-row unit the tiles
 // that some row of it sees, and which of them all its rows see whole; the others are masked score by
 // score. Rows that see nothing end with a maximum of -inf and store zeros.
-// Rounded to T: K and V, as the read-back does, and P, since the products take 16-bit operands (half a step each);
-// scores, maxima, sums and O are held in 32 bits.
+// Rounded to T: K and V, as the read-back does, and P, since the products take 16-bit operands (half a step each;
+// P in f16 below 2^-14: 2^-25); scores, maxima, sums and O are held in 32 bits. Error against 64 bits: 0.0034 of
+// the outputs' root mean square in bf16 and 0.00042 in f16, twice that of the output's own rounding. Codes held
+// exactly, as for few rows, would take two multiplications (K and V scale) for every score in the softmax
+// warps, where the converters now take one for every element of a tile.
 // ---------------------------------------------------------------------------------------------
 constexpr int kBM = 128, kUnitRows = 2 * kBM, kBN = 128, kD = kHeadDim;
 constexpr int kTileThreads = 512;

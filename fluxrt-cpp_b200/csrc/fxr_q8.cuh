@@ -358,8 +358,9 @@ __device__ __forceinline__ void quantise_store(float2* y, uint8_t* codes, T* sca
 // warp runs four heads of Q, K and V at a time (a unit). The launch's units are divided evenly over the
 // warps, and a warp loads its next unit, also the next row's, while it works on one (1536 rows of 24 heads
 // 13.6 us; 16.5 with a warp per row, which leaves a third of them idle, 17.1 with three per row). Three
-// rows of T are read, one of T and two of bytes written per token: bound by memory (16896 rows of 24
-// heads: 100 us, 5.2 TB/s; two lanes' worth of shuffles and a division per code took 211 us).
+// rows of T are read, one of T and two of bytes written per token (16896 rows of 24 heads in a graph: 101 us,
+// 5.2 TB/s, with issue slots 62 % and DRAM 56 % busy; two lanes' worth of shuffles and a division per code
+// took 211 us).
 template <typename T, int F, bool kRaw>
 __global__ void __launch_bounds__(kWriteThreads, 2) q8_write_kernel(const __grid_constant__ WriteArgs a) {
     const int lane = threadIdx.x & 31, sub = lane & (kVecLanes - 1), of = lane / kVecLanes;

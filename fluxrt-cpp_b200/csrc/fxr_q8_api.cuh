@@ -152,8 +152,8 @@ Q8Work carve_q8(const fxr_frame_desc* d, int32_t n_streams, int32_t n_prefix, in
     const size_t body = off;
     if (w.few) {
         // groups as large as a stream's rows need; the packed rows of a prefix fill groups of 16 at most
-        // otherwise (of 32, and 8 warps, took 85 us where 16 rows and 16 warps take 79: 8 streams of 15
-        // rows, 4608 + 2304 keys; 3 streams 77 and 48)
+        // otherwise (8 streams, 4608 + 2304 keys, 24 heads, in a graph: 6 rows each 75.9 us, and 81.6 in groups
+        // of 32 with 8 warps; 10 rows 81.3, and 109; 15 rows 102.6, and 117; 3 streams of 15 rows 45.7, and 74.6)
         const int64_t packed = n_prefix > 0 ? std::max(R, std::min<int64_t>(S * R, 16)) : R;
         w.tiles = packed <= 8 ? 1 : packed <= 16 ? 2 : 4;
         const int64_t tile = 8 * w.tiles;
@@ -436,8 +436,8 @@ int32_t fxr_cache_read_q8(const fxr_frame_desc* desc, const fxr_q8_cache* cache,
     const int32_t bound = host_count > 0 ? std::min(host_count, cache->n_rows) : cache->n_rows;
     fxr::q8::ReadArgs a{q8_arg(cache), idx, count, host_count, k, v, ld, cache->n_rows, bound, desc->n_heads};
     const int64_t units = (int64_t)bound * desc->n_heads * (fxr::kHeadDim / 16);
-    // CTAs per SM at most: short ones that the hardware balances for a whole cache (16896 rows: 58 us
-    // against 67 us with 16), fewer where most may find nothing to do (1153 of 4608 rows: 6.3 against 6.8)
+    // CTAs per SM at most: short ones that the hardware balances for a whole cache (16896 rows in a graph:
+    // 58 us against 67 us with 16), fewer where most may find nothing to do (1153 of 4608 rows: 6.3 against 6.8)
     const int64_t ctas = (units + fxr::q8::kReadThreads - 1) / fxr::q8::kReadThreads, sms = sm_count();
     const int grid = (int)std::max<int64_t>(1, std::min(ctas, sms * (ctas > sms * 32 ? 64 : 16)));
     return q8_dispatch(desc->dtype, cache->format, [&](auto t, auto f) -> int32_t {

@@ -1049,7 +1049,8 @@ def attention_q8(cfg: FrameConfig, streams, workspace, prefix: CacheQ8 | None = 
                  max_rows: int = 0, stream=None):
     """Attention of each stream's executed rows over the prefix and its own 8-bit cache
     (fxr_attention_q8). streams: a list of dicts as for q8_streams(), or what it returned. workspace: a
-    zeroed uint8 tensor of attention_q8_workspace_size() bytes, reused as is."""
+    zeroed uint8 tensor of attention_q8_workspace_size() bytes, reused as is. max_rows: bound of a stream's
+    rows (0: the frame's tokens); 32 and less take the kernel for few rows."""
     if not isinstance(streams, Q8Streams):
         streams = q8_streams(streams)
     streams.check(cfg, max_rows)
@@ -1070,7 +1071,8 @@ def frame_q8_workspace_size(cfg: FrameConfig, n_prefix: int = 0, max_rows: int =
 def frame_forward_q8(cfg: FrameConfig, q, k, v, mask, valid, pos, norm_q, norm_k, cache: CacheQ8, out, workspace,
                      prefix: CacheQ8 | None = None, prefix_groups=None, q_groups=None, k_groups=None,
                      max_rows: int = 0, stream=None):
-    """One frame over an 8-bit cache (fxr_frame_forward_q8)."""
+    """One frame over an 8-bit cache (fxr_frame_forward_q8). max_rows: bound of the executed rows (0: the frame's
+    tokens); 32 and less take the attention for few rows."""
     cache.check(cfg, cfg.n_tokens)
     _check_frame(cfg, cache, q, k, v, mask, pos, norm_q, norm_k)
     n, cols = cfg.n_tokens, cfg.n_heads * cfg.head_dim

@@ -633,8 +633,8 @@ int32_t fxr_frame_forward_heads_nccl(const fxr_frame_desc* desc, const fxr_head_
  * A vector of zeros has scale 0. One that holds an infinity or NaN has
  * scale NaN and codes 0: it reads back as NaN, and an attention row that sees it is NaN. K' is
  * quantised from its 32-bit value. The e4m3 codes 0x7f and 0xff, NaN in other uses, which the write never
- * produces, count as 480 and -480 wherever a cache is read (times a scale next to the largest that is past
- * the largest T: read back as infinity, in the attention the largest T). A scale is at most (largest T) / 128
+ * produces, count as 480 and -480 wherever a cache is read (where that times the scale is past the largest
+ * T, the read-back gives infinity and the attention of more than 32 rows the largest T). A scale is at most (largest T) / 128
  * for int8 and (largest T) / 448 for e4m3, so that every finite vector reads back finite; codes saturate
  * there. In the attention a larger one counts as NaN. */
 typedef enum fxr_q8_format { FXR_Q8_INT8 = 0, FXR_Q8_E4M3 = 1 } fxr_q8_format;
@@ -691,8 +691,10 @@ int32_t fxr_restore_rows_q8(const fxr_frame_desc* desc, const int32_t* mask, con
  * all bits. A row that sees no key gets zeros. Masked keys contribute nothing, whatever they hold.
  * max_rows: the caller's bound of *count for every stream (<= 0: n_tokens). Rows past it are not
  * computed and set the device error word (FXR_ERR_BOUNDS). qc has to hold max_rows rows: those past
- * *count are read, never used. A tight bound lets calls of few rows take the kernel made for them. Rows of
- * out that are not listed are left as they are.
+ * *count are read, never used. A bound of 32 or less takes the kernel made for few rows, which a call
+ * without a bound never does, and which holds K and V exactly as code * scale; with a larger bound they are
+ * rounded to T, as the read-back rounds them, and so are the weights p_j (error against 64 bits 0.0034 of the
+ * outputs in bf16, 0.0017 for few rows). Rows of out that are not listed are left as they are.
  * More than FXR_MAX_BATCH streams run as consecutive groups. workspace: at least
  * fxr_attention_q8_workspace_size() bytes, 16-byte aligned, ZERO before its first use and then reused
  * as is by calls on one stream, of any bound, format and (up to 256) head count, where it is large enough
