@@ -900,7 +900,8 @@ def _check_frame(cfg: FrameConfig, cache: CacheQ8, q, k, v, mask, pos, norm_q, n
 
 def gather_norm_rope_q8(cfg: FrameConfig, q, k, v, mask, idx, count, pos, norm_q, norm_k, qc, cache: CacheQ8,
                         save=None, stream=None):
-    """gather_norm_rope into an 8-bit cache (fxr_gather_norm_rope_q8). save: uint8 [N, q8_save_row_bytes(cfg)]."""
+    """gather_norm_rope into an 8-bit cache (fxr_gather_norm_rope_q8). save: uint8 [N, q8_save_row_bytes(cfg)]. As
+    there, the tensors' sizes are the caller's: this call's host time is as long as its kernel."""
     cache.check(cfg, cfg.n_tokens)
     _words(mask, idx, count, pos)
     _check(load().fxr_gather_norm_rope_q8(cfg.ref(), q.data_ptr(), k.data_ptr(), v.data_ptr(), mask.data_ptr(),

@@ -642,7 +642,7 @@ typedef enum fxr_q8_format { FXR_Q8_INT8 = 0, FXR_Q8_E4M3 = 1 } fxr_q8_format;
 typedef struct fxr_q8_cache {
     void* k;                 /* [n_rows, ld] codes, one byte each; head h at columns [h*D, (h+1)*D) */
     void* v;
-    void* k_scale;           /* [n_heads, ld_scale] of the frame's type: entry (h, row) */
+    void* k_scale;           /* [n_heads, ld_scale] of the frame's type: entry (h, row), 0 and more or NaN */
     void* v_scale;
     int64_t ld;              /* bytes between rows: a multiple of 16, >= n_heads*head_dim */
     int64_t ld_scale;        /* elements between heads: a multiple of 8, >= n_rows */
